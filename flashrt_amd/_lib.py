@@ -12,7 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libflashrt_moe.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "flashrt_moe.h")
 
-_vp, _i, _sz, _u64, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_uint64, C.c_float
+_vp, _i, _sz, _u64, _f, _i64 = C.c_void_p, C.c_int, C.c_size_t, C.c_uint64, C.c_float, C.c_int64
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -36,6 +36,14 @@ SIGNATURES = {
     "frt_router_logits_gemm": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _sz]),
     "frt_moe_dispatch_workspace_bytes": (_sz, [_i, _i, _i]),
     "frt_moe_dispatch": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _sz]),
+    "frt_moe_sort": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "frt_moe_permute": (_i, [_vp, _vp, _i64, _i, _i, _i, _i, _vp, _vp, _i64]),
+    "frt_moe_permute_grad": (_i, [_vp, _vp, _i64, _i, _i, _i, _i, _vp, _vp, _i64]),
+    "frt_moe_unpermute": (_i, [_vp, _vp, _i64, _i, _i, _i, _i, _vp, _vp, _vp, _i64]),
+    "frt_moe_unpermute_grad": (_i, [_vp, _vp, _i64, _vp, _i64, _i, _i, _i, _i, _vp, _vp, _vp, _i64, _vp]),
+    "frt_mx4_quantize": (_i, [_vp, _vp, _i64, _i, _i, _i, _vp, _vp]),
+    "frt_mx4_dequantize": (_i, [_vp, _vp, _vp, _i, _i, _vp, _i64, _i]),
+    "frt_mx4_product": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _i64, _i]),
     "frt_moe_q2_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "frt_moe_q2_run": (_i, [_vp, _sz, _i, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _sz, _vp, _i, _i]),
     "frt_moe_hits_scratch_bytes": (_sz, [_i, _i, _i]),

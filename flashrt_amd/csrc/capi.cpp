@@ -166,6 +166,21 @@ int hits_from_ids(const int32_t* ids, int T, int K, const uint8_t* arena, size_t
                   const uint8_t** hit_ptr, int32_t* hit_n, hipStream_t stream);
 int slot_combine(int T, int K, int S, int n, const int32_t* ids, const float* wts, const float* Y, const float* sh,
                  size_t sh_stride, const float* gate, const float* resid, float* out, hipStream_t stream);
+// permute.hip
+int moe_sort(const int32_t* ids, int T, int K, int E, int32_t* bounds, int32_t* tok_of, int32_t* slot_of, int32_t* row_of,
+             hipStream_t stream);
+int moe_permute(int type, const void* x, int64_t ldx, int T, int K, int n, const int32_t* row_of, void* xs, int64_t ldxs,
+                hipStream_t stream);
+int moe_sum_rows(int type, const void* ys, int64_t ldys, int T, int K, int n, const int32_t* row_of, const float* wts, void* y,
+                 int64_t ldy, hipStream_t stream);
+int moe_unpermute_grad(int type, const void* dy, int64_t lddy, const void* ys, int64_t ldys, int T, int K, int n, const int32_t* row_of,
+                       const float* wts, void* dys, int64_t lddys, float* dwts, hipStream_t stream);
+// mx4.hip
+int mx4_quantize(int type, const void* x, int64_t ldx, int64_t rows, int cols, void* codes, void* scales, hipStream_t stream);
+int mx4_dequantize(int type, const void* codes, const void* scales, int64_t rows, int cols, void* out, int64_t ldout,
+                   hipStream_t stream);
+int mx4_product(const void* aq, const void* as, int a_rows, const int32_t* rows, const void* wq, const void* ws, const int32_t* bounds,
+                int E, int M, int N, int C, void* out, int type, int64_t ldout, hipStream_t stream);
 // decode.hip
 bool dec_shape_templated(int n, int ff);
 bool dec_shape_generic(int n, int ff);
@@ -444,6 +459,30 @@ static int scratch_ptr(void** out) {
     return kOk;
 }
 
+// ---- the checks of the row moves and the 4-bit entries
+static int type_check(const char* what, int type) {
+    if (type != FRT_GGML_F32 && type != FRT_GGML_F16 && type != FRT_GGML_BF16)
+        return set_error(kErrShape, "%s: type %d (F32, F16 or BF16)", what, type);
+    return kOk;
+}
+// rows of n values of a type at least n apart and aligned to the value
+static int rows_check(const char* what, const char* name, const void* p, int64_t ld, int n, int type) {
+    if (!p) return set_error(kErrNull, "%s: null %s", what, name);
+    if (ld < n) return set_error(kErrShape, "%s: %s rows %lld apart, %d wide", what, name, (long long)ld, n);
+    if (reinterpret_cast<uintptr_t>(p) % (type == FRT_GGML_F32 ? 4 : 2)) return set_error(kErrShape, "%s: %s misaligned", what, name);
+    return kOk;
+}
+static int move_check(const char* what, int type, int T, int K, int n) {
+    if (int rc = type_check(what, type)) return rc;
+    if (T < 0 || K < 1 || n < 1 || int64_t(T) * K > 0x7fffffff) return set_error(kErrShape, "%s: T=%d K=%d n=%d", what, T, K, n);
+    return kOk;
+}
+static int codes_check(const char* what, const char* name, const void* codes, const void* scales) {
+    if (!codes || !scales) return set_error(kErrNull, "%s: null %s", what, name);
+    if (reinterpret_cast<uintptr_t>(codes) % 16) return set_error(kErrShape, "%s: %s codes not 16-byte aligned", what, name);
+    return kOk;
+}
+
 }  // namespace frt
 
 using namespace frt;
@@ -581,6 +620,87 @@ int frt_moe_dispatch(void* stream, const int32_t* ids, int T, int K, int E, int3
                      int32_t* slot_of, void* ws, size_t ws_bytes) {
     if (!ids || !bounds || !tok_of || !slot_of || !ws) return set_error(kErrNull, "dispatch: null pointer");
     return pf_dispatch(ids, T, K, E, bounds, tok_of, slot_of, ws, ws_bytes, static_cast<hipStream_t>(stream));
+}
+
+int frt_moe_sort(void* stream, const int32_t* ids, int T, int K, int E, int32_t* bounds, int32_t* tok_of, int32_t* slot_of,
+                 int32_t* row_of) {
+    if (T < 0 || K < 1 || E < 1 || E > 1024 || int64_t(T) * K > 0x7fffffff)
+        return set_error(kErrShape, "moe_sort: T=%d K=%d E=%d", T, K, E);
+    if (!bounds || (T > 0 && (!ids || !tok_of || !slot_of || !row_of))) return set_error(kErrNull, "moe_sort: null pointer");
+    return moe_sort(ids, T, K, E, bounds, tok_of, slot_of, row_of, static_cast<hipStream_t>(stream));
+}
+
+int frt_moe_permute(void* stream, const void* x, int64_t ldx, int type, int T, int K, int n, const int32_t* row_of, void* xs,
+                    int64_t ldxs) {
+    if (int rc = move_check("moe_permute", type, T, K, n)) return rc;
+    if (T == 0) return kOk;
+    if (!row_of) return set_error(kErrNull, "moe_permute: null row_of");
+    if (int rc = rows_check("moe_permute", "x", x, ldx, n, type)) return rc;
+    if (int rc = rows_check("moe_permute", "xs", xs, ldxs, n, type)) return rc;
+    return moe_permute(type, x, ldx, T, K, n, row_of, xs, ldxs, static_cast<hipStream_t>(stream));
+}
+
+int frt_moe_permute_grad(void* stream, const void* dxs, int64_t lddxs, int type, int T, int K, int n, const int32_t* row_of,
+                         void* dx, int64_t lddx) {
+    if (int rc = move_check("moe_permute_grad", type, T, K, n)) return rc;
+    if (T == 0) return kOk;
+    if (!row_of) return set_error(kErrNull, "moe_permute_grad: null row_of");
+    if (int rc = rows_check("moe_permute_grad", "dxs", dxs, lddxs, n, type)) return rc;
+    if (int rc = rows_check("moe_permute_grad", "dx", dx, lddx, n, type)) return rc;
+    return moe_sum_rows(type, dxs, lddxs, T, K, n, row_of, nullptr, dx, lddx, static_cast<hipStream_t>(stream));
+}
+
+int frt_moe_unpermute(void* stream, const void* ys, int64_t ldys, int type, int T, int K, int n, const int32_t* row_of,
+                      const float* wts, void* y, int64_t ldy) {
+    if (int rc = move_check("moe_unpermute", type, T, K, n)) return rc;
+    if (T == 0) return kOk;
+    if (!row_of || !wts) return set_error(kErrNull, "moe_unpermute: null row_of or wts");
+    if (int rc = rows_check("moe_unpermute", "ys", ys, ldys, n, type)) return rc;
+    if (int rc = rows_check("moe_unpermute", "y", y, ldy, n, type)) return rc;
+    return moe_sum_rows(type, ys, ldys, T, K, n, row_of, wts, y, ldy, static_cast<hipStream_t>(stream));
+}
+
+int frt_moe_unpermute_grad(void* stream, const void* dy, int64_t lddy, const void* ys, int64_t ldys, int type, int T, int K,
+                           int n, const int32_t* row_of, const float* wts, void* dys, int64_t lddys, float* dwts) {
+    if (int rc = move_check("moe_unpermute_grad", type, T, K, n)) return rc;
+    if (T == 0) return kOk;
+    if (!row_of || !wts || !dwts) return set_error(kErrNull, "moe_unpermute_grad: null row_of, wts or dwts");
+    if (int rc = rows_check("moe_unpermute_grad", "dy", dy, lddy, n, type)) return rc;
+    if (int rc = rows_check("moe_unpermute_grad", "ys", ys, ldys, n, type)) return rc;
+    if (int rc = rows_check("moe_unpermute_grad", "dys", dys, lddys, n, type)) return rc;
+    return moe_unpermute_grad(type, dy, lddy, ys, ldys, T, K, n, row_of, wts, dys, lddys, dwts, static_cast<hipStream_t>(stream));
+}
+
+int frt_mx4_quantize(void* stream, const void* x, int64_t ldx, int type, int rows, int cols, void* codes, void* scales) {
+    if (int rc = type_check("mx4_quantize", type)) return rc;
+    if (rows < 0 || cols < 32 || cols % 32) return set_error(kErrShape, "mx4_quantize: rows=%d cols=%d (a multiple of 32)", rows, cols);
+    if (rows == 0) return kOk;
+    if (int rc = rows_check("mx4_quantize", "x", x, ldx, cols, type)) return rc;
+    if (int rc = codes_check("mx4_quantize", "output", codes, scales)) return rc;
+    return mx4_quantize(type, x, ldx, rows, cols, codes, scales, static_cast<hipStream_t>(stream));
+}
+
+int frt_mx4_dequantize(void* stream, const void* codes, const void* scales, int rows, int cols, void* out, int64_t ldout,
+                       int type) {
+    if (int rc = type_check("mx4_dequantize", type)) return rc;
+    if (rows < 0 || cols < 32 || cols % 32) return set_error(kErrShape, "mx4_dequantize: rows=%d cols=%d (a multiple of 32)", rows, cols);
+    if (rows == 0) return kOk;
+    if (int rc = codes_check("mx4_dequantize", "input", codes, scales)) return rc;
+    if (int rc = rows_check("mx4_dequantize", "out", out, ldout, cols, type)) return rc;
+    return mx4_dequantize(type, codes, scales, rows, cols, out, ldout, static_cast<hipStream_t>(stream));
+}
+
+int frt_mx4_product(void* stream, const void* aq, const void* asc, int a_rows, const int32_t* rows, const void* wq,
+                    const void* wsc, const int32_t* bounds, int E, int M, int N, int C, void* out, int64_t ldout, int type) {
+    if (int rc = type_check("mx4_product", type)) return rc;
+    if (M < 0 || N < 1 || C < 32 || C % 32) return set_error(kErrShape, "mx4_product: M=%d N=%d C=%d (a multiple of 32)", M, N, C);
+    if (E < 1 || E > 4096 || (!bounds && E != 1)) return set_error(kErrShape, "mx4_product: E=%d%s", E, bounds ? "" : " without bounds");
+    if (M == 0) return kOk;
+    if (a_rows < (rows ? 1 : M)) return set_error(kErrShape, "mx4_product: %d rows of activations for M=%d", a_rows, M);
+    if (int rc = codes_check("mx4_product", "activations", aq, asc)) return rc;
+    if (int rc = codes_check("mx4_product", "weights", wq, wsc)) return rc;
+    if (int rc = rows_check("mx4_product", "out", out, ldout, N, type)) return rc;
+    return mx4_product(aq, asc, a_rows, rows, wq, wsc, bounds, E, M, N, C, out, type, ldout, static_cast<hipStream_t>(stream));
 }
 
 size_t frt_moe_q2_workspace_bytes(int T, int K, int n, int ff, int E) {

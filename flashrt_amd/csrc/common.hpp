@@ -95,6 +95,17 @@ inline void launch_timed(const char* name, K kernel, dim3 grid, dim3 block, size
         hipLaunchKernelGGL(kernel, grid, block, uint32_t(shm), stream, args...);
 }
 
+// Division of n < 2^31 by a divisor fixed at launch: with l = ceil(log2 d) and m = ceil(2^(31 + l) / d), n m / 2^(31 + l) exceeds n / d
+// by less than n / 2^31 / d < 1 / d, so its floor is the quotient.
+struct FastDiv {
+    uint32_t m, s;
+    explicit FastDiv(uint32_t d) : m(0), s(31) {
+        while ((uint64_t(1) << (s - 31)) < d) ++s;
+        m = uint32_t(((uint64_t(1) << s) + d - 1) / d);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return uint32_t((uint64_t(n) * m) >> s); }
+};
+
 inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // ---- device helpers

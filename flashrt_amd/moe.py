@@ -24,7 +24,8 @@ from ._lib import LAYER_NORM_INPUT, FrtArena, FrtError, FrtExpertSlab, FrtLoadSt
 __all__ = ["FrtError", "ExpertArena", "arena_alloc", "arena_free", "moe_route_topk", "router_logits", "quantize_q8",
            "moe_dispatch", "moe_q2", "moe_hits_scratch_bytes", "moe_hits", "MoeLayer", "expert_bytes", "gen",
            "set_option", "layer_sync_error", "MoeStack", "noalloc_scratch_bytes", "q2_repack",
-           "q2_repack_expert", "load_experts"]
+           "q2_repack_expert", "load_experts", "moe_sort", "moe_permute", "moe_permute_grad", "moe_unpermute",
+           "moe_unpermute_grad", "mx4_quantize", "mx4_dequantize", "mx4_product"]
 
 
 def _p(t) -> int | None:
@@ -144,6 +145,122 @@ def moe_dispatch(ids, T: int, K: int, E: int, bounds, tok_of, slot_of, stream=No
     ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
     check(lib().frt_moe_dispatch(_s(stream), _p(ids), T, K, E, _p(bounds), _p(tok_of), _p(slot_of), _p(ws), nbytes))
     return ws
+
+
+# ---------------------------------------------------------------- rows in expert order and back; 4-bit floats
+# These check their tensors (ValueError): type, shape, layout, and that all lie on one GPU, which need not be the current one.
+
+_ROW_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}   # ggml type ids
+
+
+def _enqueue(fn, dev: int, stream, *args) -> None:
+    """check(fn(stream, *args)) on the stream (by default the current one) of GPU dev."""
+    if dev < 0:
+        raise ValueError("flashrt_amd: expected a device tensor")
+    if isinstance(stream, torch.cuda.Stream) and stream.device_index != dev:
+        raise ValueError(f"flashrt_amd: the tensors are on GPU {dev}, the stream on GPU {stream.device_index}")
+    if dev == torch.cuda.current_device():
+        check(fn(_s(stream), *args))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(_s(stream), *args))
+
+
+def _rows(t, rows: int, cols: int, like, what: str) -> int:
+    """The distance between the rows of a [rows][cols] matrix of like's type on like's GPU, each row's values adjacent."""
+    if t.dtype is not like.dtype or t.dtype not in _ROW_TYPES or t.get_device() != like.get_device():
+        raise ValueError(f"{what}: expected {like.dtype} (float32, float16 or bfloat16) on {like.device}, got {t.dtype} on {t.device}")
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+        raise ValueError(f"{what}: expected [{rows}][{cols}], got {list(t.shape)}")
+    ld, step = t.stride()
+    if rows <= 1:   # (a lone row's stride says nothing)
+        ld = cols
+    if (step != 1 and cols > 1) or ld < cols:
+        raise ValueError(f"{what}: rows of adjacent values, at least {cols} apart, expected; strides {t.stride()}")
+    return ld
+
+
+def _flat(t, count: int, dtype, like, what: str) -> int:
+    """The address of a contiguous tensor of at least count values on like's GPU."""
+    if t.dtype is not dtype or t.get_device() != like.get_device() or not t.is_contiguous() or t.numel() < count:
+        raise ValueError(f"{what}: expected {count} contiguous {dtype} on {like.device}, got {list(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def moe_sort(ids, T: int, K: int, E: int, bounds, tok_of, slot_of, row_of, stream=None) -> None:
+    """frt_moe_sort: the slots t * K + k in expert order (stable), and each slot's row (-1: its id is outside [0, E)). ids,
+    tok_of, slot_of and row_of hold T * K int32, bounds E + 1."""
+    S, i32 = T * K, torch.int32
+    _enqueue(lib().frt_moe_sort, ids.get_device(), stream, _flat(ids, S, i32, ids, "ids"), T, K, E, _flat(bounds, E + 1, i32, ids, "bounds"),
+             _flat(tok_of, S, i32, ids, "tok_of"), _flat(slot_of, S, i32, ids, "slot_of"), _flat(row_of, S, i32, ids, "row_of"))
+
+
+def moe_permute(x, T: int, K: int, row_of, xs, stream=None) -> None:
+    """frt_moe_permute: xs[row_of[s]] = x[s // K]; x [T][n], xs [T * K][n]. Rows of xs that no slot has stay as they were."""
+    n = x.shape[-1]
+    ld, lds = _rows(x, T, n, x, "x"), _rows(xs, T * K, n, x, "xs")
+    _enqueue(lib().frt_moe_permute, x.get_device(), stream, x.data_ptr(), ld, _ROW_TYPES[x.dtype], T, K, n,
+             _flat(row_of, T * K, torch.int32, x, "row_of"), xs.data_ptr(), lds)
+
+
+def moe_permute_grad(dxs, T: int, K: int, row_of, dx, stream=None) -> None:
+    """frt_moe_permute_grad: dx[t] = the sum of dxs over the token's rows; dxs [T * K][n], dx [T][n]."""
+    n = dxs.shape[-1]
+    lds, ld = _rows(dxs, T * K, n, dxs, "dxs"), _rows(dx, T, n, dxs, "dx")
+    _enqueue(lib().frt_moe_permute_grad, dxs.get_device(), stream, dxs.data_ptr(), lds, _ROW_TYPES[dxs.dtype], T, K, n,
+             _flat(row_of, T * K, torch.int32, dxs, "row_of"), dx.data_ptr(), ld)
+
+
+def moe_unpermute(ys, T: int, K: int, row_of, wts, y, stream=None) -> None:
+    """frt_moe_unpermute: y[t] = sum_k wts[t, k] ys[row_of[t * K + k]]; ys [T * K][n], wts T * K float32, y [T][n]."""
+    n = ys.shape[-1]
+    lds, ld = _rows(ys, T * K, n, ys, "ys"), _rows(y, T, n, ys, "y")
+    _enqueue(lib().frt_moe_unpermute, ys.get_device(), stream, ys.data_ptr(), lds, _ROW_TYPES[ys.dtype], T, K, n,
+             _flat(row_of, T * K, torch.int32, ys, "row_of"), _flat(wts, T * K, torch.float32, ys, "wts"), y.data_ptr(), ld)
+
+
+def moe_unpermute_grad(dy, ys, T: int, K: int, row_of, wts, dys, dwts, stream=None) -> None:
+    """frt_moe_unpermute_grad: the gradients of moe_unpermute by ys (dys [T * K][n]; rows that no slot has stay as they were)
+    and by wts (dwts T * K float32; 0 for a dropped slot), from dy [T][n]."""
+    n = dy.shape[-1]
+    ld, lds, ldd = _rows(dy, T, n, dy, "dy"), _rows(ys, T * K, n, dy, "ys"), _rows(dys, T * K, n, dy, "dys")
+    _enqueue(lib().frt_moe_unpermute_grad, dy.get_device(), stream, dy.data_ptr(), ld, ys.data_ptr(), lds, _ROW_TYPES[dy.dtype], T, K, n,
+             _flat(row_of, T * K, torch.int32, dy, "row_of"), _flat(wts, T * K, torch.float32, dy, "wts"), dys.data_ptr(), ldd,
+             _flat(dwts, T * K, torch.float32, dy, "dwts"))
+
+
+def mx4_quantize(x, codes, scales, stream=None) -> None:
+    """frt_mx4_quantize: x [rows][cols] as 4-bit floats, codes rows * cols / 2 and scales rows * cols / 32 bytes (uint8)."""
+    rows, cols = x.shape
+    ld = _rows(x, rows, cols, x, "x")
+    _enqueue(lib().frt_mx4_quantize, x.get_device(), stream, x.data_ptr(), ld, _ROW_TYPES[x.dtype], rows, cols,
+             _flat(codes, rows * cols // 2, torch.uint8, x, "codes"), _flat(scales, rows * cols // 32, torch.uint8, x, "scales"))
+
+
+def mx4_dequantize(codes, scales, out, stream=None) -> None:
+    """frt_mx4_dequantize: the values of codes and scales into out [rows][cols]."""
+    rows, cols = out.shape
+    ld = _rows(out, rows, cols, out, "out")
+    _enqueue(lib().frt_mx4_dequantize, out.get_device(), stream, _flat(codes, rows * cols // 2, torch.uint8, out, "codes"),
+             _flat(scales, rows * cols // 32, torch.uint8, out, "scales"), rows, cols, out.data_ptr(), ld, _ROW_TYPES[out.dtype])
+
+
+def mx4_product(aq, asc, wq, wsc, out, bounds=None, rows=None, stream=None) -> None:
+    """frt_mx4_product: out[r] = w_g a(r) for the rows r of group g (bounds[g] .. bounds[g + 1], int32; without bounds all
+    rows and one group). aq [a_rows][C / 2], asc [a_rows][C / 32]; wq [E][N][C / 2] (or [N][C / 2]), wsc [E][N][C / 32]; out
+    [M][N]; rows (M int32): a(r) is row rows[r] of the activations instead of r."""
+    if aq.dim() != 2 or wq.dim() not in (2, 3) or out.dim() != 2:
+        raise ValueError(f"mx4_product: aq {list(aq.shape)}, wq {list(wq.shape)}, out {list(out.shape)}")
+    a_rows, C = aq.shape[0], 2 * aq.shape[1]
+    E = wq.shape[0] if wq.dim() == 3 else 1
+    M, N = out.shape
+    if wq.shape[-1] != aq.shape[1] or wq.shape[-2] != N:
+        raise ValueError(f"mx4_product: aq {list(aq.shape)}, wq {list(wq.shape)}, out {list(out.shape)}")
+    ld, u8, i32 = _rows(out, M, N, out, "out"), torch.uint8, torch.int32
+    _enqueue(lib().frt_mx4_product, out.get_device(), stream, _flat(aq, a_rows * C // 2, u8, out, "aq"),
+             _flat(asc, a_rows * C // 32, u8, out, "asc"), a_rows, None if rows is None else _flat(rows, M, i32, out, "rows"),
+             _flat(wq, E * N * C // 2, u8, out, "wq"), _flat(wsc, E * N * C // 32, u8, out, "wsc"),
+             None if bounds is None else _flat(bounds, E + 1, i32, out, "bounds"), E, M, N, C, out.data_ptr(), ld, _ROW_TYPES[out.dtype])
 
 
 # ---------------------------------------------------------------- prefill grouped GEMM

@@ -142,6 +142,52 @@ size_t frt_moe_dispatch_workspace_bytes(int T, int K, int E);
 int frt_moe_dispatch(void* stream, const int32_t* ids, int T, int K, int E, int32_t* bounds, int32_t* tok_of,
                      int32_t* slot_of, void* ws, size_t ws_bytes);
 
+/* ---- rows in expert order and back, with the gradients (no reference counterpart: the reference's grouped products gather
+ * their rows themselves and its layer sums them; these are for other products between the two moves, and for training).
+ * S = T * K slots s = t * K + k; E <= 1024. A slot whose id is outside [0, E) (a padded token, an expert over its capacity) is
+ * dropped: it has no row. T may be 0 (nothing is read; moe_sort then writes bounds of zeros).
+ * frt_moe_sort: a stable sort of the slots by expert, as frt_moe_dispatch's, with the inverse map, in one launch without a
+ * workspace: bounds [E+1]; slot_of and tok_of (= slot_of / K) [S], of which the first bounds[E] are written; row_of [S], the
+ * slot's row or -1.
+ * The moves take rows of type FRT_GGML_F32, FRT_GGML_F16 or FRT_GGML_BF16, any n >= 1, at ld* elements from one row to the
+ * next (ld* >= n), and row_of as frt_moe_sort wrote it (an entry outside [0, S) is a dropped slot's). Sums are fp32, ascending
+ * k, rounded once. Inputs and outputs must not overlap.
+ *   permute         xs[row_of[s]] = x[s / K]; other rows of xs stay as they were
+ *   permute_grad    dx[t] = sum over the token's rows of dxs[row_of[t K + k]]
+ *   unpermute       y[t] = sum_k wts[t K + k] ys[row_of[t K + k]], wts fp32; 0 for a token without rows
+ *   unpermute_grad  dys[row] = wts[s] dy[s / K] for row = row_of[s] (other rows of dys stay as they were), and
+ *                   dwts[s] = sum_j dy[s / K][j] ys[row][j], fp32, 0 for a dropped slot */
+int frt_moe_sort(void* stream, const int32_t* ids, int T, int K, int E, int32_t* bounds, int32_t* tok_of, int32_t* slot_of,
+                 int32_t* row_of);
+int frt_moe_permute(void* stream, const void* x, int64_t ldx, int type, int T, int K, int n, const int32_t* row_of, void* xs,
+                    int64_t ldxs);
+int frt_moe_permute_grad(void* stream, const void* dxs, int64_t lddxs, int type, int T, int K, int n, const int32_t* row_of,
+                         void* dx, int64_t lddx);
+int frt_moe_unpermute(void* stream, const void* ys, int64_t ldys, int type, int T, int K, int n, const int32_t* row_of,
+                      const float* wts, void* y, int64_t ldy);
+int frt_moe_unpermute_grad(void* stream, const void* dy, int64_t lddy, const void* ys, int64_t ldys, int type, int T, int K,
+                           int n, const int32_t* row_of, const float* wts, void* dys, int64_t lddys, float* dwts);
+
+/* ---- microscaled 4-bit floats (no reference counterpart: its experts are Q2_0). Each 32 consecutive values of a row
+ * share a scale byte b, the power of two 2^(b - 127) (255: NaN), and are e2m1 codes (sign, two exponent bits, one mantissa bit: 0, 0.5,
+ * 1, 1.5, 2, 3, 4, 6): codes [rows][cols/2], value 2 j in the low half of byte j, 16-byte aligned; scales [rows][cols/32]. cols is a
+ * multiple of 32. rows may be 0.
+ * frt_mx4_quantize: x of type FRT_GGML_F32 / F16 / BF16, rows ldx elements apart (ldx >= cols). With a block's largest
+ * magnitude m 2^k (1 <= m < 2), b = max(k - 2, -127) + 127 and a code is x 2^(127 - b) rounded to nearest even, at most 6 in
+ * magnitude; a block of zeros has b = 0; a block with an infinity or a NaN has b = 255 and codes 0 (all its values read NaN).
+ * frt_mx4_dequantize: the values, rounded to nearest even where the type cannot hold them. */
+int frt_mx4_quantize(void* stream, const void* x, int64_t ldx, int type, int rows, int cols, void* codes, void* scales);
+int frt_mx4_dequantize(void* stream, const void* codes, const void* scales, int rows, int cols, void* out, int64_t ldout,
+                       int type);
+/* ---- grouped product of 4-bit operands, the sorted experts' products: out[r][j] = sum_k a(r)[k] w_g[j][k] for r in
+ * [bounds[g], bounds[g+1]), g < E <= 4096, j < N, k < C (a multiple of 32). a(r) is row r of the activations
+ * (aq [a_rows][C/2], asc [a_rows][C/32]), or row rows[r] where rows is given (frt_moe_sort's tok_of: the tokens quantized
+ * once); an index outside [0, a_rows) reads as a row of zeros. Weights wq [E][N][C/2], wsc [E][N][C/32]. bounds NULL: one
+ * group (E = 1) of M rows. Bounds ascend within [0, M]; rows of no group stay as they were. aq and wq 16-byte aligned; a_rows >= M, or >= 1
+ * with rows. out of type FRT_GGML_F32 / F16 / BF16, rows ldout >= N elements apart; sums in fp32, rounded once. M >= 0, N >= 1. */
+int frt_mx4_product(void* stream, const void* aq, const void* asc, int a_rows, const int32_t* rows, const void* wq,
+                    const void* wsc, const int32_t* bounds, int E, int M, int N, int C, void* out, int64_t ldout, int type);
+
 /* ---- prefill grouped expert GEMM (kernels/cuda/moe_q2.h:20-30 moe_q2::workspace_bytes, run).
  * yd [T*K][n]: slot t*K + k gets down(silu(gate x_t) * up x_t) of expert ids[t*K + k], expert e's
  * blob at experts + e * stride (both multiples of 16: blobs are read in pieces of 16 bytes; an arena's

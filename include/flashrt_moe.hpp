@@ -465,6 +465,44 @@ inline void run(const uint8_t* experts, size_t stride, int E, int n, int ff, con
 }
 
 }  // namespace moe_q2
+
+// ---- rows in expert order and back with the gradients, and 4-bit floats with their grouped product (no reference
+// counterpart; flashrt_moe.h states each call)
+inline void moe_sort(hipStream_t stream, const int32_t* ids, int T, int K, int E, int32_t* bounds, int32_t* tok_of,
+                     int32_t* slot_of, int32_t* row_of) {
+    detail::check(frt_moe_sort(stream, ids, T, K, E, bounds, tok_of, slot_of, row_of), "moe_sort");
+}
+inline void moe_permute(hipStream_t stream, const void* x, int64_t ldx, int type, int T, int K, int n, const int32_t* row_of,
+                        void* xs, int64_t ldxs) {
+    detail::check(frt_moe_permute(stream, x, ldx, type, T, K, n, row_of, xs, ldxs), "moe_permute");
+}
+inline void moe_permute_grad(hipStream_t stream, const void* dxs, int64_t lddxs, int type, int T, int K, int n,
+                             const int32_t* row_of, void* dx, int64_t lddx) {
+    detail::check(frt_moe_permute_grad(stream, dxs, lddxs, type, T, K, n, row_of, dx, lddx), "moe_permute_grad");
+}
+inline void moe_unpermute(hipStream_t stream, const void* ys, int64_t ldys, int type, int T, int K, int n, const int32_t* row_of,
+                          const float* wts, void* y, int64_t ldy) {
+    detail::check(frt_moe_unpermute(stream, ys, ldys, type, T, K, n, row_of, wts, y, ldy), "moe_unpermute");
+}
+inline void moe_unpermute_grad(hipStream_t stream, const void* dy, int64_t lddy, const void* ys, int64_t ldys, int type, int T,
+                               int K, int n, const int32_t* row_of, const float* wts, void* dys, int64_t lddys, float* dwts) {
+    detail::check(frt_moe_unpermute_grad(stream, dy, lddy, ys, ldys, type, T, K, n, row_of, wts, dys, lddys, dwts),
+                  "moe_unpermute_grad");
+}
+
+namespace mx4 {
+inline void quantize(hipStream_t stream, const void* x, int64_t ldx, int type, int rows, int cols, void* codes, void* scales) {
+    detail::check(frt_mx4_quantize(stream, x, ldx, type, rows, cols, codes, scales), "mx4::quantize");
+}
+inline void dequantize(hipStream_t stream, const void* codes, const void* scales, int rows, int cols, void* out, int64_t ldout,
+                       int type) {
+    detail::check(frt_mx4_dequantize(stream, codes, scales, rows, cols, out, ldout, type), "mx4::dequantize");
+}
+inline void product(hipStream_t stream, const void* aq, const void* asc, int a_rows, const int32_t* rows, const void* wq,
+                    const void* wsc, const int32_t* bounds, int E, int M, int N, int C, void* out, int64_t ldout, int type) {
+    detail::check(frt_mx4_product(stream, aq, asc, a_rows, rows, wq, wsc, bounds, E, M, N, C, out, ldout, type), "mx4::product");
+}
+}  // namespace mx4
 }  // namespace flashrt
 
 #endif
