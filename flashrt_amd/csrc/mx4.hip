@@ -5,6 +5,10 @@
 // byte j; scales [rows][cols / 32]. This is the operand format of gfx950's scaled matrix instructions: a lane takes one block
 // of 32 codes as 16 bytes and its scale as one byte.
 #include "common.hpp"
+#include "lds_dma.hpp"
+
+#include <algorithm>
+#include <type_traits>
 
 #include "../../include/flashrt_moe.h"
 
@@ -12,10 +16,15 @@ namespace frt {
 
 typedef uint32_t u4e4_t __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u4e2_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u4e1_t __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u2e1_t __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint32_t u2e2_t __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 typedef float f8_t __attribute__((ext_vector_type(8)));
 typedef int i4_t __attribute__((ext_vector_type(4)));
 typedef int i8_t __attribute__((ext_vector_type(8)));
+typedef float f16_t __attribute__((ext_vector_type(16)));
 
 // Eight values of a row as fp32, loaded at the element's own alignment
 __device__ __forceinline__ f8_t load8(const float* p) {
@@ -128,41 +137,63 @@ struct RowTile {
     int g, row0, rows;   // rows 0: no such tile
 };
 
-// Tile `index` of the groups' rows cut into tiles of BM, found by one wave from bounds (no list in memory): each lane counts the
-// tiles of its share of the groups, a scan over the lanes finds the lane, and that lane its group. Rows are clamped to
-// [0, M), so that no bounds lead outside the operands.
-template <int BM>
-__device__ __forceinline__ RowTile find_tile(const int32_t* __restrict__ bounds, int E, int M, int index) {
-    if (!bounds) return {0, index * BM, max(0, min(BM, M - index * BM))};
-    const int lane = threadIdx.x & 63;
-    const int per = (E + 63) / 64, e0 = min(lane * per, E), e1 = min(e0 + per, E);
-    auto at = [&](int e) { return min(max(bounds[e], 0), M); };
-    int n = 0;
-    for (int e = e0; e < e1; ++e) n += max(0, at(e + 1) - at(e) + BM - 1) / BM;
-    int incl = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(incl, o, 64);
-        if (lane >= o) incl += y;
+// Inclusive sum over the lanes of a wave, by DPP
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // one lane down within a row of 16, then two, four, eight
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, kDppBcast15, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, kDppBcast31, 0xC, 0xF, false);
+    return v;
+}
+
+// The tile that which(number of tiles) names, of the groups' rows cut into tiles of BM, found by one wave from bounds (no list in
+// memory): each lane counts the tiles of 8 neighbouring groups, whose loads are in flight together (one trip to memory for up to
+// 512 groups), a scan over the lanes finds the lane, and that lane its group. Rows are clamped to [0, M), so that no bounds lead
+// outside the operands.
+template <int BM, typename Which>
+__device__ __forceinline__ RowTile find_tile(const int32_t* __restrict__ bounds, int E, int M, Which which) {
+    if (!bounds) {
+        const int index = which((M + BM - 1) / BM);
+        return {0, index * BM, index < 0 ? 0 : max(0, min(BM, M - index * BM))};
     }
-    const uint64_t past = __ballot(incl > index);
-    if (!past) return {0, 0, 0};
-    const int owner = __builtin_ctzll(past);
-    RowTile t{0, 0, 0};
-    int left = index - (incl - n);
-    if (lane == owner)
-        for (int e = e0; e < e1; ++e) {
-            const int lo = at(e), hi = at(e + 1), c = max(0, hi - lo + BM - 1) / BM;
-            if (left < c) {
-                t = {e, lo + left * BM, min(BM, hi - lo - left * BM)};
-                break;
-            }
-            left -= c;
+    const int lane = threadIdx.x & 63;
+    int at[9], n = 0, incl = 0, total = 0;
+    auto block = [&](int e0) {   // groups e0 + 8 lane ..: their first rows, their tiles, and the tiles up to the lane
+#pragma unroll
+        for (int i = 0; i < 9; ++i) at[i] = gld<int>(bounds + min(e0 + 8 * lane + i, E));
+        n = 0;
+#pragma unroll
+        for (int i = 0; i < 9; ++i) at[i] = min(max(at[i], 0), M);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n += max(0, at[i + 1] - at[i] + BM - 1) / BM;
+        incl = wave_scan(n);
+    };
+    for (int e0 = 0; e0 < E; e0 += 512) {
+        block(e0);
+        total += __builtin_amdgcn_readlane(incl, 63);
+    }
+    int index = which(total), e0 = 0;
+    if (index < 0 || index >= total) return {0, 0, 0};
+    if (E > 512)
+        for (block(0); index >= __builtin_amdgcn_readlane(incl, 63); block(e0)) {   // (ends: index < total)
+            index -= __builtin_amdgcn_readlane(incl, 63);
+            e0 += 512;
         }
-    t.g = __builtin_amdgcn_readlane(t.g, owner);
-    t.row0 = __builtin_amdgcn_readlane(t.row0, owner);
-    t.rows = __builtin_amdgcn_readlane(t.rows, owner);
-    return t;
+    const int owner = __builtin_ctzll(__ballot(incl > index));
+    int left = index - (incl - n), g = 0, row0 = 0, rows = 0;   // (of use in that lane)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int c = max(0, at[i + 1] - at[i] + BM - 1) / BM;
+        if (left >= 0 && left < c) {
+            g = e0 + 8 * lane + i;
+            row0 = at[i] + left * BM;
+            rows = min(BM, at[i + 1] - row0);
+        }
+        left -= c;
+    }
+    return {__builtin_amdgcn_readlane(g, owner), __builtin_amdgcn_readlane(row0, owner), __builtin_amdgcn_readlane(rows, owner)};
 }
 // Tiles of BM rows that M rows in E groups have at most
 static int64_t tiles_at_most(int64_t M, int64_t E, int BM, bool grouped) {
@@ -183,55 +214,551 @@ struct Mx4Args {
     int64_t ldout;
 };
 
-// A wave per 16 features x 16 rows: the weights as the A operand, so a lane's four results are consecutive features of one
-// row. Lane l holds block 4 s + l / 16 of its feature and of its row in step s.
-template <typename T>
-__global__ void __launch_bounds__(256) k_mx4_rows(Mx4Args p, int ntile) {
-    const int64_t unit = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
-    const RowTile t = find_tile<16>(p.bounds, p.E, p.M, int(unit / ntile));
-    if (t.rows == 0) return;
-    const int f0 = int(unit % ntile) * 16, nb = p.C / 32;
-    int64_t a = -1;
-    if (j < t.rows) {
-        a = p.rows ? p.rows[t.row0 + j] : t.row0 + j;
-        if (a < 0 || a >= p.a_rows) a = -1;
-    }
-    const bool fok = f0 + j < p.N;
-    const int64_t w = (int64_t(t.g) * p.N + (fok ? f0 + j : 0)) * nb, x = (a < 0 ? 0 : a) * nb;
+// An operand of the matrix instructions: its 16 bytes in the low half of the register tuple
+__device__ __forceinline__ i8_t fp4(i4_t v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
+
+// Few rows: 16 features x 16 rows by KW waves that share the values of a row, straight from global memory into the registers of the
+// matrix instructions, all of a wave's loads in flight at once. The weights are the first operand, so that a lane's four results
+// are adjacent features of one row. A group of 512 values is 16 blocks: step i multiplies blocks 4 i + l / 16 of lane l's
+// feature and row, whose scales are the 16 bytes beside each other; wave w takes the groups w, w + KW, ..., and the blocks behind
+// the last whole group go one step at a time. The waves' sums are added in their order. Rows and features past the end are the last one
+// again, never stored.
+template <typename T, int KW>
+__global__ void __launch_bounds__(256) k_mx4_rows(Mx4Args p, int ntile, FastDiv ntiles) {
+    constexpr int FW = 4 / KW;   // tiles of a workgroup
+    __shared__ f4_t s_sum[4][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
+    const int kw = wave % KW;
+    const uint32_t unit = blockIdx.x * FW + wave / KW, tile = ntiles(unit);
+    const RowTile t = find_tile<16>(p.bounds, p.E, p.M, [&](int total) { return int(tile) < total ? int(tile) : -1; });
+    const int f0 = int(unit - tile * ntile) * 16, nb = p.C / 32, ng = nb / 16;
     f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int b = 0; b < nb; b += 4) {
-        i4_t wv = {0, 0, 0, 0}, xv = {0, 0, 0, 0};
-        int wsc = 127, xsc = 127;
-        if (b + g < nb) {
-            if (fok) {
-                wv = __builtin_bit_cast(i4_t, gld_u4(p.wq + (w + b + g) * 16));
-                wsc = gld<uint8_t>(p.ws + w + b + g);
+    bool ok = false;
+    if (t.rows > 0) {   // (uniform over the wave)
+        const int r = t.row0 + min(j, t.rows - 1);
+        int a = r;
+        if (p.rows) a = gld<int>(p.rows + r);   // (under way while the weights' loads are issued)
+        const int64_t w = (int64_t(t.g) * p.N + min(f0 + j, p.N - 1)) * nb;
+        struct Group {
+            i4_t w[4], x[4];
+            u4e1_t ws, xs;
+        } u, v;
+        auto load_w = [&](int q, Group& o) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o.w[i] = gld<i4_t>(p.wq + (w + 16 * q + 4 * i + g) * 16);
+            o.ws = gld<u4e1_t>(p.ws + w + 16 * q);
+        };
+        auto load_x = [&](int q, Group& o, int64_t x) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o.x[i] = gld<i4_t>(p.aq + (x + 16 * q + 4 * i + g) * 16);
+            o.xs = gld<u4e1_t>(p.as + x + 16 * q);
+        };
+        auto mma = [&](const Group& o) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4(o.w[i]), fp4(o.x[i]), acc, 4, 4, 0, int(o.ws[i] >> (8 * g)), 0,
+                                                                       int(o.xs[i] >> (8 * g)));
+        };
+        int q = kw;
+        if (q < ng) load_w(q, u);
+        if (q + KW < ng) load_w(q + KW, v);
+        __builtin_amdgcn_sched_barrier(0);
+        ok = unsigned(a) < unsigned(p.a_rows);
+        const int64_t x = int64_t(ok ? a : 0) * nb;
+        if (q < ng) load_x(q, u, x);
+        if (q + KW < ng) load_x(q + KW, v, x);
+        for (; q < ng; q += 2 * KW) {   // two groups' loads in flight
+            mma(u);
+            if (q + 2 * KW < ng) {
+                load_w(q + 2 * KW, u);
+                load_x(q + 2 * KW, u, x);
             }
-            if (a >= 0) {
-                xv = __builtin_bit_cast(i4_t, gld_u4(p.aq + (x + b + g) * 16));
-                xsc = gld<uint8_t>(p.as + x + b + g);
+            if (q + KW < ng) {
+                mma(v);
+                if (q + 3 * KW < ng) {
+                    load_w(q + 3 * KW, v);
+                    load_x(q + 3 * KW, v, x);
+                }
             }
         }
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(wv, wv, 0, 1, 2, 3, -1, -1, -1, -1),
-                                                               __builtin_shufflevector(xv, xv, 0, 1, 2, 3, -1, -1, -1, -1), acc, 4, 4, 0,
-                                                               wsc, 0, xsc);
+        for (int b = 16 * ng + 4 * kw; b < nb; b += 4 * KW) {   // the last blocks' steps, over the waves
+            const bool in = b + g < nb;
+            const i4_t zero = {0, 0, 0, 0};
+            const int c = min(b + g, nb - 1);
+            const i4_t wv = gld<i4_t>(p.wq + (w + c) * 16), xv = gld<i4_t>(p.aq + (x + c) * 16);
+            const int ws = gld<uint8_t>(p.ws + w + c), xs = gld<uint8_t>(p.as + x + c);
+            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4(in ? wv : zero), fp4(in ? xv : zero), acc, 4, 4, 0, in ? ws : 127, 0,
+                                                                   in ? xs : 127);
+        }
+    }
+    if constexpr (KW > 1) {
+        s_sum[wave][lane] = acc;
+        __syncthreads();
+        if (kw != 0) return;
+#pragma unroll
+        for (int i = 1; i < KW; ++i) acc += s_sum[wave + i][lane];
     }
     if (j < t.rows) {
-        T* o = static_cast<T*>(p.out) + (t.row0 + j) * p.ldout + f0 + 4 * g;
-        for (int i = 0; i < 4; ++i)
-            if (f0 + 4 * g + i < p.N) o[i] = T(acc[i]);
+        typedef T vec4 __attribute__((ext_vector_type(4)));
+        typedef std::conditional_t<sizeof(T) == 4, u4e4_t, u2e2_t> Raw;
+        vec4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = T(ok ? acc[i] : 0.0f);
+        T* const o = static_cast<T*>(p.out) + (t.row0 + j) * p.ldout + f0 + 4 * g;
+        if (f0 + 4 * g + 4 <= p.N) {
+            *reinterpret_cast<Raw*>(o) = __builtin_bit_cast(Raw, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (f0 + 4 * g + i < p.N) o[i] = v[i];
+        }
     }
+}
+
+// A wave's LDS accesses before are done before those after, across its lanes (they complete in order)
+__device__ __forceinline__ void wave_lds_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+}
+
+template <int BM, int BN, int NW, int ST, int SS, bool OWN>
+struct TileShape {
+    static constexpr int rows = BM + BN;                // operand rows of a stage, the activations first
+    static constexpr int code_b = rows * 128;           // a stage: 256 values (8 blocks) of each row
+    static constexpr int da = BM / (8 * NW), dw = BN / (8 * NW);   // code loads per wave and stage (8 rows each)
+    static constexpr int sa = BM * SS / (32 * NW), sw = BN * SS / (32 * NW);   // scale loads per wave and group of SS stages (256 bytes each)
+    static_assert(BM * SS % (32 * NW) == 0 && BN * SS % (32 * NW) == 0, "every wave the same loads");
+    static constexpr int scale_b = rows * SS * 8;       // a group's scales
+    // The results leave through LDS, by wave: OWN, an area beside the ring, in rows of 64 bytes; else a slot of it, in rows of 128
+    static constexpr int out_row = OWN || NW * 32 * 144 > code_b ? 64 : 128, out_b = 32 * (out_row + 16);
+    static_assert(OWN || NW * out_b <= code_b, "the results in a slot");
+    static constexpr int smem = ST * code_b + 2 * scale_b + BM * 4 + (OWN ? NW * out_b : 0);
+};
+
+// Stores through a buffer descriptor: a lane whose offset lies past its bytes stores nothing, without a branch, so that the number of
+// store instructions, which the waits on the loads behind them have to count, is fixed.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+constexpr uint32_t kNoStore = 0x80000000u;
+
+// BM rows x BN features per tile, `per` feature tiles of one row tile after one another in a workgroup of WM x WN waves, from
+// LDS. A stage is 256 values of every operand row, 128 bytes of codes in a ring of ST slots, loaded straight into it; block
+// c of row r sits at c ^ ((r >> 1) & 7), so that the sixteen rows of a read phase take sixteen different columns of the banks.
+// The scales of SS stages at a time (8 SS bytes of a row side by side: the loads' cost is lines, not bytes) go the same way where
+// the rows of scales are words (WORDS: a multiple of 128 values), else a stage's through registers. In step t (0..3) lane half h
+// multiplies block 4 h + t of its rows, so that a lane's four scales of a stage are one word and the step picks its byte. Step
+// t + 1's operands are read before step t's products, the next stage's first ones before the last step's, past the barrier. The
+// stages of the feature tiles form one sequence: the next tile's first stages load while this one's results are written.
+template <typename T, int BM, int BN, int WM, int WN, int ST, int SS, bool OWN, bool WORDS>
+__global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile, int per, FastDiv chunks, uint32_t nchunk) {
+    constexpr int NW = WM * WN, NT = 64 * NW;
+    using Sh = TileShape<BM, BN, NW, ST, SS, OWN>;
+    static_assert(SS >= 2 && (ST == 2 || (ST == 3 && !OWN)), "scales a group ahead; the counts below");
+    constexpr int FM = BM / WM / 32, FN = BN / WN / 32, DA = Sh::da, DW = Sh::dw, D = DA + DW, SR = (Sh::rows + NT - 1) / NT;
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint8_t* const s_scale = smem + ST * Sh::code_b;
+    int32_t* const s_row = reinterpret_cast<int32_t*>(s_scale + 2 * Sh::scale_b);   // [BM]: the activations' row, -1: none
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int lr = lane & 31, h = lane >> 5;
+    // Workgroup b runs on XCD b % 8. Each XCD takes an eighth of the row tiles, neighbours, with all their features: a tile's activations
+    // and, where a group has several tiles, its weights stay in one L2. Where eighths would leave more than a ninth of the chip
+    // idle, the workgroups of a tile are neighbours instead.
+    uint32_t jt = chunks(blockIdx.x >> 3), chunk = (blockIdx.x >> 3) - jt * nchunk;
+    const RowTile t = find_tile<BM>(p.bounds, p.E, p.M, [&](int total) {
+        const int each = (total + 7) / 8;
+        if (each * 8 - total > total / 8) {
+            jt = chunks(blockIdx.x);
+            chunk = blockIdx.x - jt * nchunk;
+            return int(jt) < total ? int(jt) : -1;
+        }
+        const int index = int(blockIdx.x & 7) * each + int(jt);
+        return int(jt) < each && index < total ? index : -1;
+    });
+    if (t.rows == 0) return;
+    const int nb = p.C / 32, nst = (nb + 7) / 8, nfull = nb / 8;
+    int ft = int(chunk) * per;   // this feature tile, and the end
+    const int ft1 = min(ft + per, ntile);
+    if (tid < BM) {
+        const int r = t.row0 + min(tid, t.rows - 1);
+        const int a = p.rows ? p.rows[r] : r;
+        s_row[tid] = unsigned(a) < unsigned(p.a_rows) ? a : -1;
+    }
+    __syncthreads();
+
+    // Operand rows past the group's rows and the features are the last one again (never stored). s_row is read here only: a read of
+    // LDS behind the direct loads would wait for them all.
+    const int am = (wave / WN) * FM * 32 + lr, wf = BM + (wave % WN) * FN * 32 + lr;   // the lane's first stage rows
+    uint32_t none = 0;   // bit m: the lane's row 32 m on has no activations
+#pragma unroll
+    for (int m = 0; m < FM; ++m) none |= uint32_t(s_row[am + 32 * m] < 0) << m;
+    const uint8_t* const wq = p.wq + int64_t(t.g) * p.N * nb * 16;
+    const uint8_t* const ws = p.ws + int64_t(t.g) * p.N * nb;
+    auto wgt_row = [&](int f, int r) { return int64_t(min(f * BN + r, p.N - 1)) * nb; };   // the first scale of row r of feature tile f
+    // codes: a wave loads 8 DA rows of activations and 8 DW of weights; the next stage to load is stage jst of feature tile jf, into
+    // slot jslot
+    const uint8_t* asrc[DA];
+    const uint8_t* wsrc[DW];
+    const int arow = wave * DA * 8 + (lane >> 3), wrow = wave * DW * 8 + (lane >> 3);
+#pragma unroll
+    for (int i = 0; i < DA; ++i) asrc[i] = p.aq + int64_t(max(s_row[arow + 8 * i], 0)) * nb * 16;
+    int jf = ft, jst = 0, jslot = 0;
+    auto point = [&]() {
+#pragma unroll
+        for (int i = 0; i < DW; ++i) wsrc[i] = wq + wgt_row(jf, wrow + 8 * i) * 16;
+    };
+    auto issue = [&]() {   // (blocks past the row's last read as its last: their steps are masked)
+        if (jf >= ft1) return;
+        uint8_t* const s = smem + jslot * Sh::code_b;
+#pragma unroll
+        for (int i = 0; i < DA; ++i) {
+            const int c = (lane & 7) ^ ((4 * (wave * DA + i) + (lane >> 4)) & 7);
+            ldsdma16(asrc[i] + min(8 * jst + c, nb - 1) * 16, s + (wave * DA + i) * 1024);
+        }
+#pragma unroll
+        for (int i = 0; i < DW; ++i) {
+            const int c = (lane & 7) ^ ((4 * (wave * DW + i) + (lane >> 4)) & 7);
+            ldsdma16(wsrc[i] + min(8 * jst + c, nb - 1) * 16, s + BM * 128 + (wave * DW + i) * 1024);
+        }
+        jslot = jslot == ST - 1 ? 0 : jslot + 1;
+        if (++jst == nst) {
+            jst = 0;
+            ++jf;
+            point();
+        }
+    };
+    // scales (WORDS): the next group is that of stages sq SS .. of feature tile sf, into buffer sbuf
+    constexpr int LR = 2 * SS;   // lanes (words) of a row's group
+    constexpr int NA = WORDS ? Sh::sa : 0, NS = WORDS ? Sh::sa + Sh::sw : SR;   // the first NA are the activations'
+    const uint8_t* ssrc[NS];
+    const uint8_t* slast[SR];    // (the last 8 bytes of the tensor)
+    int sf = ft, sq = 0, sbuf = 0;
+    if constexpr (WORDS) {
+#pragma unroll
+        for (int k = 0; k < NA; ++k) ssrc[k] = p.as + int64_t(max(s_row[(wave * NA + k) * (64 / LR) + lane / LR], 0)) * nb;
+    } else {
+#pragma unroll
+        for (int k = 0; k < SR; ++k) {
+            const bool act = tid + NT * k < BM;
+            ssrc[k] = p.as + int64_t(max(s_row[act ? tid + NT * k : 0], 0)) * nb;
+            slast[k] = (act ? p.as + int64_t(p.a_rows) * nb : p.ws + int64_t(p.E) * p.N * nb) - 8;
+        }
+    }
+    auto spoint = [&]() {
+#pragma unroll
+        for (int k = NA; k < NS; ++k) {
+            const int r = WORDS ? (wave * Sh::sw + k - NA) * (64 / LR) + lane / LR : min(tid + NT * k, Sh::rows - 1) - BM;
+            if (WORDS || r >= 0) ssrc[k] = ws + wgt_row(sf, r);
+        }
+    };
+    auto issue_scales = [&]() {
+        if (sf >= ft1) return;
+        const int w = min(LR * sq + lane % LR, nb / 4 - 1) * 4;
+        uint8_t* const s = s_scale + sbuf * Sh::scale_b;
+        if constexpr (WORDS) {
+#pragma unroll
+            for (int k = 0; k < NA; ++k) ldsdma4(ssrc[k] + w, s + (wave * NA + k) * 256);
+#pragma unroll
+            for (int k = NA; k < NS; ++k) ldsdma4(ssrc[k] + w, s + BM * SS * 8 + (wave * Sh::sw + k - NA) * 256);
+        }
+        sbuf ^= 1;
+        if (++sq * SS >= nst) {
+            sq = 0;
+            ++sf;
+            spoint();
+        }
+    };
+    // Without WORDS: the 8 scales of stage st of row tid (and those NT on), at any alignment; past the row's end they are the next row's
+    // (their steps are masked). At the tensor's end its last 8 bytes are loaded and shifted down.
+    u2e1_t sv[SR];
+    auto load_scales = [&](int st) {
+#pragma unroll
+        for (int k = 0; k < SR; ++k) {
+            const uint8_t* const at = ssrc[k] + 8 * st;
+            sv[k] = *reinterpret_cast<const u2e1_t*>(at < slast[k] ? at : slast[k]);
+        }
+    };
+    auto put_scales = [&](int st, int buf) {
+#pragma unroll
+        for (int k = 0; k < SR; ++k) {
+            const int64_t over = ssrc[k] + 8 * st - slast[k];
+            uint64_t w = uint64_t(sv[k][1]) << 32 | sv[k][0];
+            if (over > 0) w >>= 8 * int(over < 7 ? over : 7);
+            if (tid + NT * k < Sh::rows)
+                *reinterpret_cast<uint64_t*>(s_scale + buf * Sh::scale_b + ((tid + NT * k) * SS + st % SS) * 8) = w;
+        }
+    };
+    point();
+    spoint();
+    if constexpr (WORDS) {
+        issue_scales();
+        issue_scales();
+    } else {
+        load_scales(0);
+        put_scales(0, 0);
+    }
+#pragma unroll
+    for (int s = 0; s < ST; ++s) issue();
+
+    const int sw = (lr >> 1) & 7;
+    struct Ops {
+        i4_t a[FM], b[FN];
+    };
+    auto read = [&](int slot, int tt) {
+        const uint8_t* const s = smem + slot * Sh::code_b + ((4 * h + tt) ^ sw) * 16;
+        Ops o;
+#pragma unroll
+        for (int m = 0; m < FM; ++m) o.a[m] = *reinterpret_cast<const i4_t*>(s + (am + 32 * m) * 128);
+#pragma unroll
+        for (int f = 0; f < FN; ++f) o.b[f] = *reinterpret_cast<const i4_t*>(s + (wf + 32 * f) * 128);
+        return o;
+    };
+    struct Scales {
+        int a[FM], b[FN];
+    };
+    auto read_scales = [&](int st, int buf) {
+        const uint8_t* const s = s_scale + buf * Sh::scale_b + (st % SS) * 8 + h * 4;
+        Scales o;
+#pragma unroll
+        for (int m = 0; m < FM; ++m) o.a[m] = *reinterpret_cast<const int*>(s + (am + 32 * m) * 8 * SS);
+#pragma unroll
+        for (int f = 0; f < FN; ++f) o.b[f] = *reinterpret_cast<const int*>(s + (wf + 32 * f) * 8 * SS);
+        return o;
+    };
+    f16_t acc[FM][FN];
+    auto mma = [&](auto tc, const Ops& o, const Scales& s) {   // (features x rows: a lane's four results in a row are adjacent features)
+        constexpr int tt = decltype(tc)::value;
+#pragma unroll
+        for (int m = 0; m < FM; ++m)
+#pragma unroll
+            for (int f = 0; f < FN; ++f)
+                acc[m][f] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4(o.b[f]), fp4(o.a[m]), acc[m][f], 4, 4, tt, s.b[f], tt, s.a[m]);
+    };
+    auto pin = [&]() {   // the products before stay before what follows (else the compiler sinks them past the barrier)
+#pragma unroll
+        for (int m = 0; m < FM; ++m)
+#pragma unroll
+            for (int f = 0; f < FN; ++f) asm volatile("" : "+a"(acc[m][f]));
+    };
+
+    // Waits count the codes' loads: at the end of a stage those of the ST - 1 stages after it were issued last, the next one's first;
+    // when the last ones are under way, all are waited for. At the end of a feature tile's first stage the stores of the tile before
+    // (kStores per wave) came behind the loads that are waited for, and may be under way too.
+    constexpr int kStores = FM * FN * int(sizeof(T)), kAfter = D * (ST - 2) + (OWN || ST == 3 ? kStores : 0);
+    const int ft0 = ft;
+    if ((ft1 - ft) * nst >= ST)
+        wait_vm<D*(ST - 1)>();
+    else
+        wait_vm<0>();
+    ring_barrier();
+    int slot = 0, buf = 0;   // the stage being multiplied, and its scales
+    Ops o0 = read(0, 0);
+    Scales sc = read_scales(0, 0);
+    lds_reads_done();   // (nothing pending where the loop is entered: its waits are then for its own reads)
+    for (; ft < ft1; ++ft) {
+#pragma unroll
+        for (int m = 0; m < FM; ++m)
+#pragma unroll
+            for (int f = 0; f < FN; ++f)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[m][f][i] = 0.0f;
+        // before stage st's products: the scales of the stage after it, through registers
+        auto ahead = [&](int st) {
+            if constexpr (!WORDS) {
+                if (st + 1 == nst) {
+                    ++sf;
+                    spoint();   // (past the last feature tile: rows inside the tensor still)
+                }
+                load_scales(st + 1 == nst ? 0 : st + 1);
+            }
+        };
+        // the end of stage st: the next stage has landed, all waves have read this one; its slot and, past a group, its scales' buffer
+        // are loaded anew (the slot of a tile's last stage after its results were written through it)
+        auto finish = [&](int st) {
+            const bool last = st + 1 == nst, turn = last || (st + 1) % SS == 0;
+            const int nbuf = turn ? buf ^ 1 : buf;
+            if constexpr (!WORDS) put_scales(last ? 0 : st + 1, nbuf);
+            if (jf >= ft1)
+                wait_vm<0>();
+            else if (st == 0 && ft > ft0)
+                wait_vm<(kAfter < 63 ? kAfter : 63)>();
+            else
+                wait_vm<D*(ST - 2)>();
+            ring_barrier();
+            if (WORDS && turn) issue_scales();
+            if (OWN || !last) issue();
+            buf = nbuf;
+            slot = slot == ST - 1 ? 0 : slot + 1;
+        };
+        for (int st = 0; st < nfull; ++st) {
+            ahead(st);
+            const Ops o1 = read(slot, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            mma(std::integral_constant<int, 0>(), o0, sc);
+            __builtin_amdgcn_sched_barrier(0);
+            const Ops o2 = read(slot, 2);
+            __builtin_amdgcn_sched_barrier(0);
+            mma(std::integral_constant<int, 1>(), o1, sc);
+            __builtin_amdgcn_sched_barrier(0);
+            const Ops o3 = read(slot, 3);
+            __builtin_amdgcn_sched_barrier(0);
+            mma(std::integral_constant<int, 2>(), o2, sc);
+            pin();
+            finish(st);
+            o0 = read(slot, 0);   // (past the last stage: nothing that is used)
+            const Scales next = read_scales(st + 1 == nst ? 0 : st + 1, buf);
+            __builtin_amdgcn_sched_barrier(0);
+            mma(std::integral_constant<int, 3>(), o3, sc);
+            sc = next;
+        }
+        if (nfull < nst) {
+            // the last, shorter stage: blocks 2 i and 2 i + 1 in step i; a block past the row's end is zeros at scale one
+            ahead(nfull);
+            const uint8_t* const s = smem + slot * Sh::code_b;
+            const uint8_t* const ssc = s_scale + buf * Sh::scale_b + (nfull % SS) * 8;
+            const int left = nb - 8 * nfull;
+            const i4_t zero = {0, 0, 0, 0};
+            for (int c = h; c - h < left; c += 2) {
+                const bool in = c < left;
+                const int at = (c ^ sw) * 16;
+                i4_t b[FN];
+                int bs[FN];
+#pragma unroll
+                for (int f = 0; f < FN; ++f) {
+                    b[f] = *reinterpret_cast<const i4_t*>(s + (wf + 32 * f) * 128 + at);
+                    bs[f] = ssc[(wf + 32 * f) * 8 * SS + c];
+                    b[f] = in ? b[f] : zero;
+                    bs[f] = in ? bs[f] : 127;
+                }
+#pragma unroll
+                for (int m = 0; m < FM; ++m) {
+                    i4_t a = *reinterpret_cast<const i4_t*>(s + (am + 32 * m) * 128 + at);
+                    int as = ssc[(am + 32 * m) * 8 * SS + c];
+                    a = in ? a : zero;
+                    as = in ? as : 127;
+#pragma unroll
+                    for (int f = 0; f < FN; ++f)
+                        acc[m][f] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4(b[f]), fp4(a), acc[m][f], 4, 4, 0, bs[f], 0, as);
+                }
+            }
+            finish(nfull);
+            o0 = read(slot, 0);
+            sc = read_scales(0, buf);
+        }
+
+        // The results through LDS, 32 rows of QP fourths of a fragment (8 features each) at a time, so that whole lines are stored.
+        // Lane l's value i of a fragment: feature 8 (i / 4) + 4 h + i % 4, row l % 32.
+        constexpr int sz = sizeof(T), QP = Sh::out_row / (8 * sz) < 4 * FN ? Sh::out_row / (8 * sz) : 4 * FN, V = 16 / sz;
+        constexpr int PR = QP * 8 / V, NP = 32 * PR / 64, RS = Sh::out_row + 16;   // pieces of 16 bytes in a row, of a lane; bytes from row to row
+        static_assert(4 * FN % QP == 0 && FM * (4 * FN / QP) * NP == kStores, "the stores of a wave");
+        typedef T vec4 __attribute__((ext_vector_type(4)));
+        uint8_t* const w = OWN ? smem + ST * Sh::code_b + 2 * Sh::scale_b + BM * 4 + wave * Sh::out_b
+                               : smem + (slot == 0 ? ST - 1 : slot - 1) * Sh::code_b + wave * (Sh::code_b / NW);
+        T* const out = static_cast<T*>(p.out) + t.row0 * p.ldout;
+        const Buffer buffer = __builtin_amdgcn_make_buffer_rsrc(out, 0, int(((t.rows - 1) * p.ldout + p.N) * sz), 0x00020000);
+#pragma unroll
+        for (int m = 0; m < FM; ++m) {
+            const bool ok = !(none >> m & 1);
+#pragma unroll
+            for (int q = 0; q < 4 * FN; q += QP) {
+#pragma unroll
+                for (int g = q / 4; g <= (q + QP - 1) / 4; ++g) asm volatile("" : "+a"(acc[m][g]));   // (read one piece at a time)
+#pragma unroll
+                for (int i = 0; i < QP; ++i) {
+                    vec4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = T(ok ? acc[m][(q + i) / 4][(q + i) % 4 * 4 + e] : 0.0f);
+                    *reinterpret_cast<vec4*>(w + lr * RS + (8 * i + 4 * h) * sz) = v;
+                }
+                wave_lds_order();
+                int ln = lane;
+                asm volatile("" : "+v"(ln));   // (addresses formed piece by piece, not all kept from before the loop)
+                const int at = ft * BN + (wave % WN) * FN * 32 + q * 8 + ln % PR * V;
+                const int r0 = (wave / WN) * FM * 32 + 32 * m + ln / PR;
+                const uint8_t* const l = w + ln / PR * RS + ln % PR * 16;
+                if ((ft + 1) * BN <= p.N) {
+                    i4_t v[NP];
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) v[i] = *reinterpret_cast<const i4_t*>(l + i * (64 / PR) * RS);
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) {
+                        const int r = r0 + i * (64 / PR);
+                        const uint32_t to = r < t.rows ? uint32_t(r * int(p.ldout) + at) * sz : kNoStore;
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, v[i]), buffer, to, 0, 0);
+                    }
+                } else {   // the last feature tile, cut short
+                    for (int i = 0; i < NP && r0 + i * (64 / PR) < t.rows; ++i)
+                        for (int e = 0; e < V && at + e < p.N; ++e)
+                            out[(r0 + i * (64 / PR)) * p.ldout + at + e] = *reinterpret_cast<const T*>(l + i * (64 / PR) * RS + e * sz);
+                }
+                wave_lds_order();
+            }
+        }
+        if constexpr (OWN) continue;
+        ring_barrier();   // every wave's results have left the slot
+        issue();
+    }
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int ST, int SS, bool OWN, bool WORDS>
+static int tiles_go(const Mx4Args& p, int stages, int64_t fill, hipStream_t stream) {
+    const int ntile = (p.N + BN - 1) / BN;
+    const int64_t tiles = tiles_at_most(p.M, p.E, BM, p.bounds != nullptr);
+    // feature tiles of a workgroup: about `stages` stages, as long as `fill` workgroups remain (half a tile of each group empty)
+    const int nst = (p.C / 32 + 7) / 8;
+    const int64_t groups = std::min(p.E, p.M), likely = p.bounds ? std::max<int64_t>(p.M / BM + groups / 2, groups) : tiles;
+    int nchunk = std::max(1, std::min(stages / nst, ntile));
+    nchunk = (ntile + nchunk - 1) / nchunk;
+    while (nchunk < ntile && likely * nchunk < fill) ++nchunk;
+    const int per = (ntile + nchunk - 1) / nchunk;
+    nchunk = (ntile + per - 1) / per;
+    const int64_t wgs = (tiles + 7) / 8 * 8 * nchunk;
+    if (wgs > 0x7fffffff) return set_error(kErrShape, "mx4_product: M=%d N=%d E=%d", p.M, p.N, p.E);
+    constexpr int smem = TileShape<BM, BN, WM * WN, ST, SS, OWN>::smem;
+    static_assert(smem <= 160 * 1024, "LDS of a CU");
+    FRT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_mx4_tiles<T, BM, BN, WM, WN, ST, SS, OWN, WORDS>),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, smem));
+    launch_timed("mx4_product", k_mx4_tiles<T, BM, BN, WM, WN, ST, SS, OWN, WORDS>, dim3(uint32_t(wgs)), dim3(64 * WM * WN), smem, stream, p, ntile,
+                 per, FastDiv(nchunk), uint32_t(nchunk));
+    FRT_LAUNCHED("mx4_product");
+    return kOk;
+}
+template <typename T, int BM, int BN, int WM, int WN, int ST, int SS, bool OWN>
+static int tiles_t(const Mx4Args& p, int stages, int64_t fill, hipStream_t stream) {
+    const bool words = p.C % 128 == 0 && reinterpret_cast<uintptr_t>(p.as) % 4 == 0 && reinterpret_cast<uintptr_t>(p.ws) % 4 == 0;
+    return words ? tiles_go<T, BM, BN, WM, WN, ST, SS, OWN, true>(p, stages, fill, stream)
+                 : tiles_go<T, BM, BN, WM, WN, ST, SS, OWN, false>(p, stages, fill, stream);
+}
+
+template <typename T, int KW>
+static int rows_t(const Mx4Args& p, hipStream_t stream) {
+    const int ntile = (p.N + 15) / 16;
+    const int64_t units = tiles_at_most(p.M, p.E, 16, p.bounds != nullptr) * ntile, wgs = (units + 4 / KW - 1) / (4 / KW);
+    if (units > 0x7ffffff0) return set_error(kErrShape, "mx4_product: M=%d N=%d E=%d", p.M, p.N, p.E);
+    launch_timed("mx4_product", k_mx4_rows<T, KW>, dim3(uint32_t(wgs)), dim3(256), 0, stream, p, ntile, FastDiv(ntile));
+    FRT_LAUNCHED("mx4_product");
+    return kOk;
 }
 
 template <typename T>
 static int product_t(const Mx4Args& p, hipStream_t stream) {
-    const int ntile = (p.N + 15) / 16;
-    const int64_t units = tiles_at_most(p.M, p.E, 16, p.bounds != nullptr) * ntile, wgs = (units + 3) / 4;
-    if (wgs > 0x7fffffff) return set_error(kErrShape, "mx4_product: M=%d N=%d E=%d", p.M, p.N, p.E);
-    launch_timed("mx4_product", k_mx4_rows<T>, dim3(uint32_t(wgs)), dim3(256), 0, stream, p, ntile);
-    FRT_LAUNCHED("mx4_product");
-    return kOk;
+    // The tile by the rows of a group, were they spread evenly: with few rows the weights' bytes are all there is to read, and small
+    // tiles put more of them in flight; with many the operands pass through LDS less often. Measured, smaller against larger tile:
+    //   rows 32 / 64: 4 rows to a group (N 1024, C 2048) 79.5 / 82.7 us, 16 rows 127 / 122
+    //   64 / 128: 40 rows 139 / 154 us, 62 rows 159 / 151, 160 rows 250 / 226
+    //   128 / 256: one group of 8192 (N 8192, C 4096) 184 / 151 us, of 2048 51 / 46, of 8 groups of 512 rows (N, C 2048) 24 / 26
+    // Below one workgroup of the smallest tile per CU the waves split a row's values instead: ten groups of one row 8.6 -> 7.2 us,
+    // one row of N 8192, C 4096 10.4 -> 6.8, 16 rows 10.9 -> 8.4; at 128 rows, 256 such workgroups, 12.6 against 20.
+    const int64_t groups = p.bounds ? std::min(p.E, p.M) : 1, avg = p.M / groups;
+    auto tiles = [&](int64_t BM, int64_t BN) { return ((avg + BM - 1) / BM * groups) * ((p.N + BN - 1) / BN); };
+    const int nb = p.C / 32;   // (the tile kernels load 8 scales at a time, and store through 31-bit offsets)
+    if (tiles(32, 128) >= 256 && int64_t(p.a_rows) * nb >= 8 && int64_t(p.E) * p.N * nb >= 8 &&
+        int64_t(256) * p.ldout * int64_t(sizeof(T)) < 0x7fffffff) {
+        if (avg >= 1024 && tiles(256, 256) >= 256) return tiles_t<T, 256, 256, 2, 2, 2, 2, true>(p, 64, 256, stream);
+        if (avg > 56 && tiles(128, 128) >= 256) return tiles_t<T, 128, 128, 2, 2, 2, 2, false>(p, 32, 1536, stream);
+        if (avg > 8 && tiles(64, 128) >= 160) return tiles_t<T, 64, 128, 2, 2, 3, 2, false>(p, 16, 512, stream);
+        return tiles_t<T, 32, 128, 1, 4, 2, 4, false>(p, 16, 512, stream);
+    }
+    return nb >= 64 ? rows_t<T, 4>(p, stream) : nb >= 32 ? rows_t<T, 2>(p, stream) : rows_t<T, 1>(p, stream);
 }
 
 #define FRT_BY_TYPE(type, fn, ...)                                                            \
