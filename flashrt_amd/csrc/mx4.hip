@@ -92,14 +92,11 @@ __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint32_t* __restri
     const uint32_t r = div(i);
     const uint32_t q = codes[i];
     const float s = scale_value(scales[i >> 2]);
-    f8_t v;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t c = q >> (4 * j), m = c & 7u;
-        // the e2m1 magnitude: 0, 0.5, then (1 + (m & 1) / 2) 2^(m / 2 - 1)
-        const uint32_t bits = m < 2u ? (m ? 0x3f000000u : 0u) : ((m >> 1) + 126u) << 23 | (m & 1u) << 22;
-        v[j] = __builtin_bit_cast(float, bits | (c & 8u) << 28) * s;
-    }
+    // (the conversion's own scale is an exponent alone: one here, and an exact product for the block's, NaN and 2^-127 included)
+    typedef float f2_t __attribute__((ext_vector_type(2)));
+    const f2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 1);
+    const f2_t c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 3);
+    const f8_t v = {a.x * s, a.y * s, b.x * s, b.y * s, c.x * s, c.y * s, d.x * s, d.y * s};
     store8(out + r * ldout + (i - r * per_row) * 8, v);
 }
 
@@ -136,17 +133,6 @@ static int dequantize_t(const void* codes, const void* scales, int64_t rows, int
 struct RowTile {
     int g, row0, rows;   // rows 0: no such tile
 };
-
-// Inclusive sum over the lanes of a wave, by DPP
-__device__ __forceinline__ int wave_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // one lane down within a row of 16, then two, four, eight
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, kDppBcast15, 0xA, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, kDppBcast31, 0xC, 0xF, false);
-    return v;
-}
 
 // The tile that which(number of tiles) names, of the groups' rows cut into tiles of BM, found by one wave from bounds (no list in
 // memory): each lane counts the tiles of 8 neighbouring groups, whose loads are in flight together (one trip to memory for up to

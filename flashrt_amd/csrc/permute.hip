@@ -27,26 +27,29 @@ struct Piece {
     Vec v;
 };
 
-// Elements [c, c + V) of a row of n, zeros past its end
+// The piece of a row of n that begins at c < n. A row's last piece is moved back to end with the row (two lanes then hold, and
+// store, the same values); a row shorter than a piece is taken by elements, zeros past its end.
+template <typename T>
+__device__ __forceinline__ int piece_at(int c, int n) { return max(0, min(c, n - Piece<T>::V)); }
 template <typename T>
 __device__ __forceinline__ Piece<T> piece_load(const T* row, int c, int n) {
     Piece<T> p;
-    if (c + Piece<T>::V <= n) {
-        p.v = __builtin_bit_cast(typename Piece<T>::Vec, *reinterpret_cast<const typename Piece<T>::Raw*>(row + c));
+    if (n >= Piece<T>::V) {
+        p.v = __builtin_bit_cast(typename Piece<T>::Vec, *reinterpret_cast<const typename Piece<T>::Raw*>(row + piece_at<T>(c, n)));
     } else {
 #pragma unroll
-        for (int i = 0; i < Piece<T>::V; ++i) p.v[i] = c + i < n ? row[c + i] : T(0.0f);
+        for (int i = 0; i < Piece<T>::V; ++i) p.v[i] = i < n ? row[i] : T(0.0f);
     }
     return p;
 }
 template <typename T>
 __device__ __forceinline__ void piece_store(T* row, int c, int n, const Piece<T>& p) {
-    if (c + Piece<T>::V <= n) {
-        *reinterpret_cast<typename Piece<T>::Raw*>(row + c) = __builtin_bit_cast(typename Piece<T>::Raw, p.v);
+    if (n >= Piece<T>::V) {
+        *reinterpret_cast<typename Piece<T>::Raw*>(row + piece_at<T>(c, n)) = __builtin_bit_cast(typename Piece<T>::Raw, p.v);
     } else {
 #pragma unroll
         for (int i = 0; i < Piece<T>::V; ++i)
-            if (c + i < n) row[c + i] = p.v[i];
+            if (i < n) row[i] = p.v[i];
     }
 }
 
@@ -55,10 +58,40 @@ constexpr int kSortE = 1024;       // experts at most (a thread each)
 constexpr int kSortCopies = 16;    // histogram copies, one per lane of a row of 16 (and one per wave in the ranking)
 constexpr int kSortGrid = 256;     // workgroups at most
 
+// Up to 64 slots (a decode step): every wave has all ids, one per lane. A group's first row is the number of ids below it, a slot's
+// row the number of ids that sort before it: no histogram, scan or barrier. One token's 10 slots 8.2 -> 2.6 us.
+__global__ void __launch_bounds__(1024) k_sort_few(const int32_t* __restrict__ ids, int S, int K, int E, int32_t* __restrict__ bounds,
+                                                   int32_t* __restrict__ tok_of, int32_t* __restrict__ slot_of,
+                                                   int32_t* __restrict__ row_of) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    int id = lane < S ? ids[lane] : -1;
+    if (unsigned(id) >= unsigned(E)) id = 0x7fffffff;
+    int below = 0, row = 0;
+    for (int s = 0; s < S; ++s) {
+        const int e = __builtin_amdgcn_readlane(id, s);
+        below += e < tid;
+        row += e < id || (e == id && s < lane);
+    }
+    const int live = __popcll(__ballot(id < E));
+    if (tid < E) bounds[tid] = below;
+    if (tid == 0) bounds[E] = live;
+    if (tid < S) {
+        const bool valid = id < E;
+        row_of[tid] = valid ? row : -1;
+        if (valid) {
+            tok_of[row] = tid / K;
+            slot_of[row] = tid;
+        }
+    }
+}
+
 // One launch, no workspace: every workgroup counts all ids itself (those before its own slots, then all of them) in an LDS
 // histogram of 16 copies, one per lane of 16, so that a popular expert's atomics do not queue up behind each other; the scan of
 // the totals over the experts gives the groups' first rows, and the workgroup ranks its own slots in batches of 1024, a wave of
-// 64 at a time by ballots over the id bits (stable). Integer counts: the result does not depend on the atomics' order.
+// 64 at a time by ballots over the id bits (stable). Integer counts: the result does not depend on the atomics' order. The
+// counting reads 16 ids per thread at once (81920 slots 22.4 us one by one, 15.6 so); one launch instead of the dispatch's four costs
+// each workgroup the whole list, 328 KB from L2 at 81920 slots. ONE: a single batch, whose ranking counts it.
+template <bool ONE>
 __global__ void __launch_bounds__(1024) k_sort(const int32_t* __restrict__ ids, int S, int K, int E, int id_bits, int batches,
                                                int32_t* __restrict__ bounds, int32_t* __restrict__ tok_of,
                                                int32_t* __restrict__ slot_of, int32_t* __restrict__ row_of) {
@@ -67,46 +100,68 @@ __global__ void __launch_bounds__(1024) k_sort(const int32_t* __restrict__ ids, 
     __shared__ int s_wave[16];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int s0 = min(int64_t(S), int64_t(blockIdx.x) * batches * 1024), s1 = min(int64_t(S), int64_t(s0) + batches * 1024);
-    for (int i = tid; i < E * kSortCopies; i += 1024) hist[i] = 0;
-    __syncthreads();
-    auto count = [&](int lo, int hi) {
-        for (int s = lo + tid; s < hi; s += 1024) {
-            const int e = ids[s];
-            if (unsigned(e) < unsigned(E)) atomicAdd(&hist[e * kSortCopies + (lane & 15)], 1);
-        }
+    auto clear = [&]() {
+        for (int i = tid; i < E * kSortCopies; i += 1024) hist[i] = 0;
         __syncthreads();
-        int sum = 0;
-        if (tid < E)
-            for (int c = 0; c < kSortCopies; ++c) sum += hist[tid * kSortCopies + ((c + tid) & 15)];
-        return sum;
     };
-    const int before = count(0, s0);
-    __syncthreads();
-    const int total = count(s0, S);
-    // exclusive scan of the totals over the experts
-    int incl = total;
+    auto add = [&](int e) {
+        if (unsigned(e) < unsigned(E)) atomicAdd(&hist[e * kSortCopies + (lane & 15)], 1);
+    };
+    auto sum = [&]() {   // of expert tid's copies
+        int n = 0;
+        if (tid < E)
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(incl, o, 64);
-        if (lane >= o) incl += y;
-    }
-    if (lane == 63) s_wave[wave] = incl;
-    __syncthreads();
-    int first = incl - total;
-    for (int w = 0; w < wave; ++w) first += s_wave[w];
-    if (tid < E) {
-        s_base[tid] = first + before;
-        if (blockIdx.x == 0) {
+            for (int c = 0; c < kSortCopies; ++c) n += hist[tid * kSortCopies + ((c + tid) & 15)];
+        return n;
+    };
+    auto count = [&](int lo, int hi) {
+        int64_t s = lo;   // (past 2^31 after the last step of a list near that length)
+        for (; s + 16384 <= hi; s += 16384) {
+            Raw4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const Raw4*>(ids + s + (i * 1024 + tid) * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) add(int(v[i][k]));
+        }
+        int v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            v[i] = -1;
+            if (s + i * 1024 < hi && s + i * 1024 + tid < hi) v[i] = ids[s + i * 1024 + tid];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (s + i * 1024 < hi) add(v[i]);
+        __syncthreads();
+        return sum();
+    };
+    // the first row of expert tid's group, from its rows
+    auto starts = [&](int total) {
+        const int incl = wave_scan(total);
+        if (lane == 63) s_wave[wave] = incl;
+        __syncthreads();
+        int first = incl - total;
+        for (int w = 0; w < wave; ++w) first += s_wave[w];
+        if (tid < E && blockIdx.x == 0) {
             bounds[tid] = first;
             if (tid == E - 1) bounds[E] = first + total;
         }
+        return first;
+    };
+    clear();
+    if (!ONE) {
+        const int before = count(0, s0);
+        __syncthreads();
+        const int first = starts(count(s0, S));
+        if (tid < E) s_base[tid] = first + before;
+        __syncthreads();   // (the histogram was read)
+        clear();
     }
     const uint64_t lt = (lane == 0) ? 0ull : (~0ull >> (64 - lane));
-    for (int b0 = s0; b0 < s1; b0 += 1024) {   // (uniform over the workgroup)
-        const int s = b0 + tid;
-        __syncthreads();   // (the histogram was read; s_base is written)
-        for (int i = tid; i < E * kSortCopies; i += 1024) hist[i] = 0;
-        __syncthreads();
+    for (int64_t b0 = s0; b0 < s1; b0 += 1024) {   // (uniform over the workgroup)
+        const int64_t s = b0 + tid;
         const int e0 = s < s1 ? ids[s] : -1;
         const bool valid = unsigned(e0) < unsigned(E);
         const int e = valid ? e0 : 0;
@@ -117,25 +172,35 @@ __global__ void __launch_bounds__(1024) k_sort(const int32_t* __restrict__ ids, 
             peers &= on ? m : ~m;
         }
         const int rank = __popcll(peers & lt);
-        if (valid && rank == 0) hist[e * kSortCopies + wave] = __popcll(peers);
+        auto at = [&](int ex, int w) { return ex * kSortCopies + ((w + ex) & 15); };   // (turned by the expert: other banks)
+        if (valid && rank == 0) hist[at(e, wave)] = __popcll(peers);
         __syncthreads();
+        int run = 0;
+        if (ONE)
+            run = starts(sum());
+        else if (tid < E)
+            run = s_base[tid];
         if (tid < E) {   // each wave's first row of expert tid
-            int run = s_base[tid];
+#pragma unroll
             for (int w = 0; w < 16; ++w) {
-                const int c = hist[tid * kSortCopies + w];
-                hist[tid * kSortCopies + w] = run;
+                const int c = hist[at(tid, w)];
+                hist[at(tid, w)] = run;
                 run += c;
             }
-            s_base[tid] = run;
+            if (!ONE) s_base[tid] = run;
         }
         __syncthreads();
         if (s < s1) {
-            const int row = valid ? hist[e * kSortCopies + wave] + rank : -1;
+            const int row = valid ? hist[at(e, wave)] + rank : -1;
             row_of[s] = row;
             if (valid) {
-                tok_of[row] = s / K;
-                slot_of[row] = s;
+                tok_of[row] = int(s) / K;
+                slot_of[row] = int(s);
             }
+        }
+        if (b0 + 1024 < s1) {
+            __syncthreads();
+            clear();
         }
     }
 }
@@ -143,12 +208,17 @@ __global__ void __launch_bounds__(1024) k_sort(const int32_t* __restrict__ ids, 
 int moe_sort(const int32_t* ids, int T, int K, int E, int32_t* bounds, int32_t* tok_of, int32_t* slot_of, int32_t* row_of,
              hipStream_t stream) {
     const int S = T * K;
+    if (S <= 64) {
+        launch_timed("moe_sort", k_sort_few, dim3(1), dim3(1024), 0, stream, ids, S, K, E, bounds, tok_of, slot_of, row_of);
+        FRT_LAUNCHED("moe_sort");
+        return kOk;
+    }
     int id_bits = 1;
     while ((1 << id_bits) < E) ++id_bits;
-    const int nb = S > 0 ? (S + 1023) / 1024 : 1;
+    const int nb = int((int64_t(S) + 1023) / 1024);
     const int batches = (nb + kSortGrid - 1) / kSortGrid;
-    launch_timed("moe_sort", k_sort, dim3((nb + batches - 1) / batches), dim3(1024), size_t(E) * kSortCopies * 4, stream, ids, S, K, E,
-                 id_bits, batches, bounds, tok_of, slot_of, row_of);
+    launch_timed("moe_sort", nb == 1 ? k_sort<true> : k_sort<false>, dim3((nb + batches - 1) / batches), dim3(1024),
+                 size_t(E) * kSortCopies * 4, stream, ids, S, K, E, id_bits, batches, bounds, tok_of, slot_of, row_of);
     FRT_LAUNCHED("moe_sort");
     return kOk;
 }
@@ -172,7 +242,7 @@ __global__ void __launch_bounds__(256) k_permute(const T* __restrict__ x, int64_
     }
 }
 
-// The pieces of a token's rows summed in fp32, ascending k.
+// The pieces of a token's rows summed in fp32, ascending k; four rows' loads are in flight together.
 template <typename T, bool WTS>
 __global__ void __launch_bounds__(256) k_sum_rows(const T* __restrict__ ys, int64_t ldys, int n_tok, int K, int n, uint32_t parts, FastDiv div,
                                                   const int32_t* __restrict__ row_of, const float* __restrict__ wts,
@@ -182,14 +252,23 @@ __global__ void __launch_bounds__(256) k_sum_rows(const T* __restrict__ ys, int6
     const int t = int(div(unit)), c = int((unit - t * parts) * 64 + (threadIdx.x & 63)) * V;
     if (t >= n_tok || c >= n) return;
     const unsigned S = unsigned(n_tok) * K;
+    const size_t s0 = size_t(t) * K;
     float acc[V] = {};
-    for (int k = 0; k < K; ++k) {
-        const int row = row_of[size_t(t) * K + k];
-        if (unsigned(row) >= S) continue;
-        const Piece<T> p = piece_load(ys + row * ldys, c, n);
-        const float w = WTS ? wts[size_t(t) * K + k] : 1.0f;
+    for (int k0 = 0; k0 < K; k0 += 4) {
+        int row[4];
+        Piece<T> p[4];
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = WTS ? fmaf(w, float(p.v[i]), acc[i]) : acc[i] + float(p.v[i]);
+        for (int k = 0; k < 4; ++k) row[k] = row_of[s0 + min(k0 + k, K - 1)];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k0 + k < K && unsigned(row[k]) < S) p[k] = piece_load(ys + row[k] * ldys, c, n);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k0 + k < K && unsigned(row[k]) < S) {
+                const float w = WTS ? wts[s0 + k0 + k] : 1.0f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[i] = WTS ? fmaf(w, float(p[k].v[i]), acc[i]) : acc[i] + float(p[k].v[i]);
+            }
     }
     Piece<T> o;
 #pragma unroll
@@ -214,15 +293,30 @@ __global__ void __launch_bounds__(256) k_unpermute_grad(const T* __restrict__ dy
     if (unsigned(row) < S) {
         const float w = wts[s];
         const T* g = dy + div(s) * lddy;
-        for (int c = lane * V; c < n; c += 64 * V) {
-            const Piece<T> a = piece_load(g, c, n), b = piece_load(ys + row * ldys, c, n);
-            Piece<T> o;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                o.v[i] = T(w * float(a.v[i]));
-                dot = fmaf(float(a.v[i]), float(b.v[i]), dot);
+        const T* y = ys + row * ldys;
+        T* const d = dys + row * lddys;
+        for (int c0 = lane * V; c0 < n; c0 += 2 * 64 * V) {   // two pieces of both in flight
+            const int c1 = c0 + 64 * V;
+            const bool two = c1 < n;
+            Piece<T> a[2], b[2];
+            a[0] = piece_load(g, c0, n);
+            b[0] = piece_load(y, c0, n);
+            if (two) {
+                a[1] = piece_load(g, c1, n);
+                b[1] = piece_load(y, c1, n);
             }
-            piece_store(dys + row * lddys, c, n, o);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                if (k == 1 && !two) break;
+                const int c = k ? c1 : c0, again = c - piece_at<T>(c, n);   // the first `again` are the lane's before, too
+                Piece<T> o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    o.v[i] = T(w * float(a[k].v[i]));
+                    dot = i >= again ? fmaf(float(a[k].v[i]), float(b[k].v[i]), dot) : dot;
+                }
+                piece_store(d, c, n, o);
+            }
         }
     }
     dot = wave_sum_tree(dot);

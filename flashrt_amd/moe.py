@@ -175,11 +175,19 @@ def _enqueue(fn, dev: int, stream, *args) -> None:
         check(rc)
 
 
-def _rows(t, rows: int, cols: int, like, what: str) -> int:
-    """The distance between the rows of a [rows][cols] matrix of like's type on like's GPU, each row's values adjacent."""
-    if t.dtype is not like.dtype or t.dtype not in _ROW_TYPES or t.get_device() != like.get_device():
-        raise ValueError(f"{what}: expected {like.dtype} (float32, float16 or bfloat16) on {like.device}, got {t.dtype} on {t.device}")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+def _type(t, what: str) -> int:
+    """The ggml type id of a row matrix's values."""
+    code = _ROW_TYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what}: expected float32, float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+def _rows(t, rows: int, cols: int, like, dev: int, what: str) -> int:
+    """The distance between the rows of a [rows][cols] matrix of like's type on GPU dev, each row's values adjacent."""
+    if t.dtype is not like.dtype or t.get_device() != dev:
+        raise ValueError(f"{what}: expected {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    if t.shape != (rows, cols):
         raise ValueError(f"{what}: expected [{rows}][{cols}], got {list(t.shape)}")
     ld, step = t.stride()
     if rows <= 1:   # (a lone row's stride says nothing)
@@ -189,87 +197,81 @@ def _rows(t, rows: int, cols: int, like, what: str) -> int:
     return ld
 
 
-def _flat(t, count: int, dtype, like, what: str) -> int:
-    """The address of a contiguous tensor of at least count values on like's GPU."""
-    if t.dtype is not dtype or t.get_device() != like.get_device() or not t.is_contiguous() or t.numel() < count:
-        raise ValueError(f"{what}: expected {count} contiguous {dtype} on {like.device}, got {list(t.shape)} {t.dtype} on {t.device}")
+def _flat(t, count: int, dtype, dev: int, what: str) -> int:
+    """The address of a contiguous tensor of at least count values on GPU dev."""
+    if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous() or t.numel() < count:
+        raise ValueError(f"{what}: expected {count} contiguous {dtype} on GPU {dev}, got {list(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
 def moe_sort(ids, T: int, K: int, E: int, bounds, tok_of, slot_of, row_of, stream=None) -> None:
     """frt_moe_sort: the slots t * K + k in expert order (stable), and each slot's row (-1: its id is outside [0, E)). ids,
     tok_of, slot_of and row_of hold T * K int32, bounds E + 1."""
-    S, i32 = T * K, torch.int32
-    _enqueue(lib().frt_moe_sort, ids.get_device(), stream, _flat(ids, S, i32, ids, "ids"), T, K, E, _flat(bounds, E + 1, i32, ids, "bounds"),
-             _flat(tok_of, S, i32, ids, "tok_of"), _flat(slot_of, S, i32, ids, "slot_of"), _flat(row_of, S, i32, ids, "row_of"))
+    S, i32, dev = T * K, torch.int32, ids.get_device()
+    _enqueue(lib().frt_moe_sort, dev, stream, _flat(ids, S, i32, dev, "ids"), T, K, E, _flat(bounds, E + 1, i32, dev, "bounds"),
+             _flat(tok_of, S, i32, dev, "tok_of"), _flat(slot_of, S, i32, dev, "slot_of"), _flat(row_of, S, i32, dev, "row_of"))
 
 
 def moe_permute(x, T: int, K: int, row_of, xs, stream=None) -> None:
     """frt_moe_permute: xs[row_of[s]] = x[s // K]; x [T][n], xs [T * K][n]. Rows of xs that no slot has stay as they were."""
-    n = x.shape[-1]
-    ld, lds = _rows(x, T, n, x, "x"), _rows(xs, T * K, n, x, "xs")
-    _enqueue(lib().frt_moe_permute, x.get_device(), stream, x.data_ptr(), ld, _ROW_TYPES[x.dtype], T, K, n,
-             _flat(row_of, T * K, torch.int32, x, "row_of"), xs.data_ptr(), lds)
+    n, dev = x.shape[-1], x.get_device()
+    _enqueue(lib().frt_moe_permute, dev, stream, x.data_ptr(), _rows(x, T, n, x, dev, "x"), _type(x, "x"), T, K, n,
+             _flat(row_of, T * K, torch.int32, dev, "row_of"), xs.data_ptr(), _rows(xs, T * K, n, x, dev, "xs"))
 
 
 def moe_permute_grad(dxs, T: int, K: int, row_of, dx, stream=None) -> None:
     """frt_moe_permute_grad: dx[t] = the sum of dxs over the token's rows; dxs [T * K][n], dx [T][n]."""
-    n = dxs.shape[-1]
-    lds, ld = _rows(dxs, T * K, n, dxs, "dxs"), _rows(dx, T, n, dxs, "dx")
-    _enqueue(lib().frt_moe_permute_grad, dxs.get_device(), stream, dxs.data_ptr(), lds, _ROW_TYPES[dxs.dtype], T, K, n,
-             _flat(row_of, T * K, torch.int32, dxs, "row_of"), dx.data_ptr(), ld)
+    n, dev = dxs.shape[-1], dxs.get_device()
+    _enqueue(lib().frt_moe_permute_grad, dev, stream, dxs.data_ptr(), _rows(dxs, T * K, n, dxs, dev, "dxs"), _type(dxs, "dxs"), T, K, n,
+             _flat(row_of, T * K, torch.int32, dev, "row_of"), dx.data_ptr(), _rows(dx, T, n, dxs, dev, "dx"))
 
 
 def moe_unpermute(ys, T: int, K: int, row_of, wts, y, stream=None) -> None:
     """frt_moe_unpermute: y[t] = sum_k wts[t, k] ys[row_of[t * K + k]]; ys [T * K][n], wts T * K float32, y [T][n]."""
-    n = ys.shape[-1]
-    lds, ld = _rows(ys, T * K, n, ys, "ys"), _rows(y, T, n, ys, "y")
-    _enqueue(lib().frt_moe_unpermute, ys.get_device(), stream, ys.data_ptr(), lds, _ROW_TYPES[ys.dtype], T, K, n,
-             _flat(row_of, T * K, torch.int32, ys, "row_of"), _flat(wts, T * K, torch.float32, ys, "wts"), y.data_ptr(), ld)
+    n, dev = ys.shape[-1], ys.get_device()
+    _enqueue(lib().frt_moe_unpermute, dev, stream, ys.data_ptr(), _rows(ys, T * K, n, ys, dev, "ys"), _type(ys, "ys"), T, K, n,
+             _flat(row_of, T * K, torch.int32, dev, "row_of"), _flat(wts, T * K, torch.float32, dev, "wts"), y.data_ptr(),
+             _rows(y, T, n, ys, dev, "y"))
 
 
 def moe_unpermute_grad(dy, ys, T: int, K: int, row_of, wts, dys, dwts, stream=None) -> None:
     """frt_moe_unpermute_grad: the gradients of moe_unpermute by ys (dys [T * K][n]; rows that no slot has stay as they were)
     and by wts (dwts T * K float32; 0 for a dropped slot), from dy [T][n]."""
-    n = dy.shape[-1]
-    ld, lds, ldd = _rows(dy, T, n, dy, "dy"), _rows(ys, T * K, n, dy, "ys"), _rows(dys, T * K, n, dy, "dys")
-    _enqueue(lib().frt_moe_unpermute_grad, dy.get_device(), stream, dy.data_ptr(), ld, ys.data_ptr(), lds, _ROW_TYPES[dy.dtype], T, K, n,
-             _flat(row_of, T * K, torch.int32, dy, "row_of"), _flat(wts, T * K, torch.float32, dy, "wts"), dys.data_ptr(), ldd,
-             _flat(dwts, T * K, torch.float32, dy, "dwts"))
+    n, dev = dy.shape[-1], dy.get_device()
+    _enqueue(lib().frt_moe_unpermute_grad, dev, stream, dy.data_ptr(), _rows(dy, T, n, dy, dev, "dy"), ys.data_ptr(),
+             _rows(ys, T * K, n, dy, dev, "ys"), _type(dy, "dy"), T, K, n, _flat(row_of, T * K, torch.int32, dev, "row_of"),
+             _flat(wts, T * K, torch.float32, dev, "wts"), dys.data_ptr(), _rows(dys, T * K, n, dy, dev, "dys"),
+             _flat(dwts, T * K, torch.float32, dev, "dwts"))
 
 
 def mx4_quantize(x, codes, scales, stream=None) -> None:
     """frt_mx4_quantize: x [rows][cols] as 4-bit floats, codes rows * cols / 2 and scales rows * cols / 32 bytes (uint8)."""
-    rows, cols = x.shape
-    ld = _rows(x, rows, cols, x, "x")
-    _enqueue(lib().frt_mx4_quantize, x.get_device(), stream, x.data_ptr(), ld, _ROW_TYPES[x.dtype], rows, cols,
-             _flat(codes, rows * cols // 2, torch.uint8, x, "codes"), _flat(scales, rows * cols // 32, torch.uint8, x, "scales"))
+    (rows, cols), dev = x.shape, x.get_device()
+    _enqueue(lib().frt_mx4_quantize, dev, stream, x.data_ptr(), _rows(x, rows, cols, x, dev, "x"), _type(x, "x"), rows, cols,
+             _flat(codes, rows * cols // 2, torch.uint8, dev, "codes"), _flat(scales, rows * cols // 32, torch.uint8, dev, "scales"))
 
 
 def mx4_dequantize(codes, scales, out, stream=None) -> None:
     """frt_mx4_dequantize: the values of codes and scales into out [rows][cols]."""
-    rows, cols = out.shape
-    ld = _rows(out, rows, cols, out, "out")
-    _enqueue(lib().frt_mx4_dequantize, out.get_device(), stream, _flat(codes, rows * cols // 2, torch.uint8, out, "codes"),
-             _flat(scales, rows * cols // 32, torch.uint8, out, "scales"), rows, cols, out.data_ptr(), ld, _ROW_TYPES[out.dtype])
+    (rows, cols), dev = out.shape, out.get_device()
+    _enqueue(lib().frt_mx4_dequantize, dev, stream, _flat(codes, rows * cols // 2, torch.uint8, dev, "codes"),
+             _flat(scales, rows * cols // 32, torch.uint8, dev, "scales"), rows, cols, out.data_ptr(),
+             _rows(out, rows, cols, out, dev, "out"), _type(out, "out"))
 
 
 def mx4_product(aq, asc, wq, wsc, out, bounds=None, rows=None, stream=None) -> None:
     """frt_mx4_product: out[r] = w_g a(r) for the rows r of group g (bounds[g] .. bounds[g + 1], int32; without bounds all
     rows and one group). aq [a_rows][C / 2], asc [a_rows][C / 32]; wq [E][N][C / 2] (or [N][C / 2]), wsc [E][N][C / 32]; out
     [M][N]; rows (M int32): a(r) is row rows[r] of the activations instead of r."""
-    if aq.dim() != 2 or wq.dim() not in (2, 3) or out.dim() != 2:
-        raise ValueError(f"mx4_product: aq {list(aq.shape)}, wq {list(wq.shape)}, out {list(out.shape)}")
-    a_rows, C = aq.shape[0], 2 * aq.shape[1]
-    E = wq.shape[0] if wq.dim() == 3 else 1
-    M, N = out.shape
-    if wq.shape[-1] != aq.shape[1] or wq.shape[-2] != N:
-        raise ValueError(f"mx4_product: aq {list(aq.shape)}, wq {list(wq.shape)}, out {list(out.shape)}")
-    ld, u8, i32 = _rows(out, M, N, out, "out"), torch.uint8, torch.int32
-    _enqueue(lib().frt_mx4_product, out.get_device(), stream, _flat(aq, a_rows * C // 2, u8, out, "aq"),
-             _flat(asc, a_rows * C // 32, u8, out, "asc"), a_rows, None if rows is None else _flat(rows, M, i32, out, "rows"),
-             _flat(wq, E * N * C // 2, u8, out, "wq"), _flat(wsc, E * N * C // 32, u8, out, "wsc"),
-             None if bounds is None else _flat(bounds, E + 1, i32, out, "bounds"), E, M, N, C, out.data_ptr(), ld, _ROW_TYPES[out.dtype])
+    sa, sw, so = aq.shape, wq.shape, out.shape
+    if len(sa) != 2 or len(sw) not in (2, 3) or len(so) != 2 or sw[-1] != sa[1] or sw[-2] != so[1]:
+        raise ValueError(f"mx4_product: aq {list(sa)}, wq {list(sw)}, out {list(so)}")
+    a_rows, C, E, (M, N) = sa[0], 2 * sa[1], sw[0] if len(sw) == 3 else 1, so
+    dev, u8, i32 = out.get_device(), torch.uint8, torch.int32
+    _enqueue(lib().frt_mx4_product, dev, stream, _flat(aq, a_rows * C // 2, u8, dev, "aq"), _flat(asc, a_rows * C // 32, u8, dev, "asc"),
+             a_rows, None if rows is None else _flat(rows, M, i32, dev, "rows"), _flat(wq, E * N * C // 2, u8, dev, "wq"),
+             _flat(wsc, E * N * C // 32, u8, dev, "wsc"), None if bounds is None else _flat(bounds, E + 1, i32, dev, "bounds"), E, M, N, C,
+             out.data_ptr(), _rows(out, M, N, out, dev, "out"), _type(out, "out"))
 
 
 # ---------------------------------------------------------------- prefill grouped GEMM
