@@ -11,6 +11,10 @@ typedef const __attribute__((address_space(1))) void* gbl_ptr_t;
 __device__ __forceinline__ void ldsdma16(const void* g, void* lds_base) {
     __builtin_amdgcn_global_load_lds((gbl_ptr_t)g, (lds_ptr_t)lds_base, 16, 0, 0);
 }
+// the same as a non-temporal (streaming) load, for bytes that are read once
+__device__ __forceinline__ void ldsdma16_nt(const void* g, void* lds_base) {
+    __builtin_amdgcn_global_load_lds((gbl_ptr_t)g, (lds_ptr_t)lds_base, 16, 0, 2);
+}
 // the same with 4 bytes per lane, to lds_base + 4 lane
 __device__ __forceinline__ void ldsdma4(const void* g, void* lds_base) {
     __builtin_amdgcn_global_load_lds((gbl_ptr_t)g, (lds_ptr_t)lds_base, 4, 0, 0);

@@ -17,6 +17,7 @@ namespace frt {
 typedef uint32_t u4e4_t __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u4e2_t __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u4e1_t __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u1e1_t __attribute__((aligned(1)));
 typedef uint32_t u2e1_t __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t u2e2_t __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
@@ -132,6 +133,7 @@ static int dequantize_t(const void* codes, const void* scales, int64_t rows, int
 // A tile of a group's rows
 struct RowTile {
     int g, row0, rows;   // rows 0: no such tile
+    bool only;           // the group's only one
 };
 
 // The tile that which(number of tiles) names, of the groups' rows cut into tiles of BM, found by one wave from bounds (no list in
@@ -142,7 +144,7 @@ template <int BM, typename Which>
 __device__ __forceinline__ RowTile find_tile(const int32_t* __restrict__ bounds, int E, int M, Which which) {
     if (!bounds) {
         const int index = which((M + BM - 1) / BM);
-        return {0, index * BM, index < 0 ? 0 : max(0, min(BM, M - index * BM))};
+        return {0, index * BM, index < 0 ? 0 : max(0, min(BM, M - index * BM)), M <= BM};
     }
     const int lane = threadIdx.x & 63;
     int at[9], n = 0, incl = 0, total = 0;
@@ -161,14 +163,14 @@ __device__ __forceinline__ RowTile find_tile(const int32_t* __restrict__ bounds,
         total += __builtin_amdgcn_readlane(incl, 63);
     }
     int index = which(total), e0 = 0;
-    if (index < 0 || index >= total) return {0, 0, 0};
+    if (index < 0 || index >= total) return {0, 0, 0, false};
     if (E > 512)
         for (block(0); index >= __builtin_amdgcn_readlane(incl, 63); block(e0)) {   // (ends: index < total)
             index -= __builtin_amdgcn_readlane(incl, 63);
             e0 += 512;
         }
     const int owner = __builtin_ctzll(__ballot(incl > index));
-    int left = index - (incl - n), g = 0, row0 = 0, rows = 0;   // (of use in that lane)
+    int left = index - (incl - n), g = 0, row0 = 0, rows = 0, of = 0;   // (of use in that lane)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int c = max(0, at[i + 1] - at[i] + BM - 1) / BM;
@@ -176,10 +178,12 @@ __device__ __forceinline__ RowTile find_tile(const int32_t* __restrict__ bounds,
             g = e0 + 8 * lane + i;
             row0 = at[i] + left * BM;
             rows = min(BM, at[i + 1] - row0);
+            of = c;
         }
         left -= c;
     }
-    return {__builtin_amdgcn_readlane(g, owner), __builtin_amdgcn_readlane(row0, owner), __builtin_amdgcn_readlane(rows, owner)};
+    return {__builtin_amdgcn_readlane(g, owner), __builtin_amdgcn_readlane(row0, owner), __builtin_amdgcn_readlane(rows, owner),
+            __builtin_amdgcn_readlane(of, owner) == 1};
 }
 // Tiles of BM rows that M rows in E groups have at most
 static int64_t tiles_at_most(int64_t M, int64_t E, int BM, bool grouped) {
@@ -301,6 +305,17 @@ __global__ void __launch_bounds__(256) k_mx4_rows(Mx4Args p, int ntile, FastDiv 
     }
 }
 
+// Waits until at most n stages of D loads (n <= MOST) are under way
+template <int D, int MOST>
+__device__ __forceinline__ void wait_stages(int n) {
+    if constexpr (MOST > 0)
+        if (n >= MOST) return wait_vm<D * MOST>();
+    if constexpr (MOST > 0)
+        wait_stages<D, MOST - 1>(n);
+    else
+        wait_vm<0>();
+}
+
 // A wave's LDS accesses before are done before those after, across its lanes (they complete in order)
 __device__ __forceinline__ void wave_lds_order() {
     asm volatile("" ::: "memory");
@@ -308,15 +323,18 @@ __device__ __forceinline__ void wave_lds_order() {
     asm volatile("" ::: "memory");
 }
 
-template <int BM, int BN, int NW, int ST, int SS, bool OWN>
+template <int BM, int BN, int NW, int ST, int KB, int SS, bool OWN>
 struct TileShape {
     static constexpr int rows = BM + BN;                // operand rows of a stage, the activations first
-    static constexpr int code_b = rows * 128;           // a stage: 256 values (8 blocks) of each row
-    static constexpr int da = BM / (8 * NW), dw = BN / (8 * NW);   // code loads per wave and stage (8 rows each)
-    static constexpr int sa = BM * SS / (32 * NW), sw = BN * SS / (32 * NW);   // scale loads per wave and group of SS stages (256 bytes each)
-    static_assert(BM * SS % (32 * NW) == 0 && BN * SS % (32 * NW) == 0, "every wave the same loads");
-    static constexpr int scale_b = rows * SS * 8;       // a group's scales
-    // The results leave through LDS, by wave: OWN, an area beside the ring, in rows of 64 bytes; else a slot of it, in rows of 128
+    static constexpr int code_b = rows * KB * 16;       // a stage: KB blocks of 32 values of each row
+    static constexpr int dr = 64 / KB, sr = 256 / (KB * SS);   // rows of a code load, of a load of SS stages' scales
+    // loads per wave and stage, and per wave and group of SS stages; with fewer activation loads than waves, some are made twice
+    static constexpr int da = BM < dr * NW ? 1 : BM / (dr * NW), dw = BN / (dr * NW);
+    static constexpr int sa = BM < sr * NW ? 1 : BM / (sr * NW), sw = BN / (sr * NW);
+    static_assert((BM % (dr * NW) == 0 || (dr * NW) % BM == 0) && BN % (dr * NW) == 0 && (BM % (sr * NW) == 0 || (sr * NW) % BM == 0) &&
+                  BN % (sr * NW) == 0, "every wave the same loads");
+    static constexpr int scale_b = rows * SS * KB;      // a group's scales
+    // The results leave through LDS, by wave: OWN, an area beside the ring, else a slot of it, in rows of 64 bytes (128 where they fit)
     static constexpr int out_row = OWN || NW * 32 * 144 > code_b ? 64 : 128, out_b = 32 * (out_row + 16);
     static_assert(OWN || NW * out_b <= code_b, "the results in a slot");
     static constexpr int smem = ST * code_b + 2 * scale_b + BM * 4 + (OWN ? NW * out_b : 0);
@@ -328,18 +346,18 @@ typedef __amdgpu_buffer_rsrc_t Buffer;
 constexpr uint32_t kNoStore = 0x80000000u;
 
 // BM rows x BN features per tile, `per` feature tiles of one row tile after one another in a workgroup of WM x WN waves, from
-// LDS. A stage is 256 values of every operand row, 128 bytes of codes in a ring of ST slots, loaded straight into it; block
-// c of row r sits at c ^ ((r >> 1) & 7), so that the sixteen rows of a read phase take sixteen different columns of the banks.
-// The scales of SS stages at a time (8 SS bytes of a row side by side: the loads' cost is lines, not bytes) go the same way where
-// the rows of scales are words (WORDS: a multiple of 128 values), else a stage's through registers. In step t (0..3) lane half h
-// multiplies block 4 h + t of its rows, so that a lane's four scales of a stage are one word and the step picks its byte. Step
-// t + 1's operands are read before step t's products, the next stage's first ones before the last step's, past the barrier. The
+// LDS. A stage is KB blocks of 32 values of every operand row, in a ring of ST slots, their codes loaded straight into it; block c of
+// row r sits at c ^ (r / (16 / KB)) % KB, so that the sixteen rows of a read phase take sixteen different columns of the banks.
+// The scales of SS stages at a time (side by side in a row: the loads' cost is lines, not bytes) go the same way where the rows of
+// scales are words (WORDS: a multiple of 128 values), else a stage's through registers. In step t (0 .. KB / 2 - 1) lane half h
+// multiplies block KB / 2 h + t of its rows, so that a lane's scales of a stage lie in one word and the step picks its byte. Step t +
+// 1's operands are read before step t's products, the next stage's first ones before the last step's, past the barrier. The
 // stages of the feature tiles form one sequence: the next tile's first stages load while this one's results are written.
-template <typename T, int BM, int BN, int WM, int WN, int ST, int SS, bool OWN, bool WORDS>
-__global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile, int per, FastDiv chunks, uint32_t nchunk) {
+template <typename T, int BM, int BN, int WM, int WN, int ST, int KB, int SS, bool OWN, int PT, bool WORDS>
+__global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile, int per, FastDiv chunks, uint32_t nchunk, int stream) {
     constexpr int NW = WM * WN, NT = 64 * NW;
-    using Sh = TileShape<BM, BN, NW, ST, SS, OWN>;
-    static_assert(SS >= 2 && (ST == 2 || (ST == 3 && !OWN)), "scales a group ahead; the counts below");
+    using Sh = TileShape<BM, BN, NW, ST, KB, SS, OWN>;
+    static_assert(SS >= 2 && ST >= 2 && (KB == 4 || KB == 8) && PT <= KB / 2, "scales a group ahead; steps");
     constexpr int FM = BM / WM / 32, FN = BN / WN / 32, DA = Sh::da, DW = Sh::dw, D = DA + DW, SR = (Sh::rows + NT - 1) / NT;
     extern __shared__ __align__(16) uint8_t smem[];
     uint8_t* const s_scale = smem + ST * Sh::code_b;
@@ -361,7 +379,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
         return int(jt) < each && index < total ? index : -1;
     });
     if (t.rows == 0) return;
-    const int nb = p.C / 32, nst = (nb + 7) / 8, nfull = nb / 8;
+    const int nb = p.C / 32, nst = (nb + KB - 1) / KB, nfull = nb / KB;
     int ft = int(chunk) * per;   // this feature tile, and the end
     const int ft1 = min(ft + per, ntile);
     if (tid < BM) {
@@ -380,31 +398,41 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
     const uint8_t* const wq = p.wq + int64_t(t.g) * p.N * nb * 16;
     const uint8_t* const ws = p.ws + int64_t(t.g) * p.N * nb;
     auto wgt_row = [&](int f, int r) { return int64_t(min(f * BN + r, p.N - 1)) * nb; };   // the first scale of row r of feature tile f
-    // codes: a wave loads 8 DA rows of activations and 8 DW of weights; the next stage to load is stage jst of feature tile jf, into
+    // codes: a wave loads DA dr rows of activations and DW dr of weights; the next stage to load is stage jst of feature tile jf, into
     // slot jslot
+    constexpr int dr = Sh::dr;
     const uint8_t* asrc[DA];
     const uint8_t* wsrc[DW];
-    const int arow = wave * DA * 8 + (lane >> 3), wrow = wave * DW * 8 + (lane >> 3);
+    const int aw = wave * DA % (BM / dr), ww = wave * DW;   // the wave's first loads
 #pragma unroll
-    for (int i = 0; i < DA; ++i) asrc[i] = p.aq + int64_t(max(s_row[arow + 8 * i], 0)) * nb * 16;
+    for (int i = 0; i < DA; ++i) asrc[i] = p.aq + int64_t(max(s_row[(aw + i) * dr + lane / KB], 0)) * nb * 16;
     int jf = ft, jst = 0, jslot = 0;
     auto point = [&]() {
 #pragma unroll
-        for (int i = 0; i < DW; ++i) wsrc[i] = wq + wgt_row(jf, wrow + 8 * i) * 16;
+        for (int i = 0; i < DW; ++i) wsrc[i] = wq + wgt_row(jf, (ww + i) * dr + lane / KB) * 16;
     };
-    auto issue = [&]() {   // (blocks past the row's last read as its last: their steps are masked)
+    // Weights that no other row tile reads, in whole lines, are streamed past the activations in L2: 2048 rows over 512 experts (N
+    // 1024, C 2048) 78 -> 70 us, 20480 even ones 126 -> 115. Rows that share lines (C 640) would be fetched again: 75 -> 90.
+    const bool once = stream && t.only && nb % 8 == 0;
+    // Part k of PT of that stage's loads (blocks past the row's last read as its last: their steps are masked); the last part moves on
+    auto column = [&](int r) { return (lane % KB) ^ ((r + lane / KB) / (16 / KB) % KB); };   // the block at the lane's place in a load from row r on
+    auto issue_part = [&](auto kc) {
+        constexpr int k = decltype(kc)::value;
         if (jf >= ft1) return;
         uint8_t* const s = smem + jslot * Sh::code_b;
 #pragma unroll
-        for (int i = 0; i < DA; ++i) {
-            const int c = (lane & 7) ^ ((4 * (wave * DA + i) + (lane >> 4)) & 7);
-            ldsdma16(asrc[i] + min(8 * jst + c, nb - 1) * 16, s + (wave * DA + i) * 1024);
-        }
+        for (int i = DA * k / PT; i < DA * (k + 1) / PT; ++i)
+            ldsdma16(asrc[i] + min(KB * jst + column((aw + i) * dr), nb - 1) * 16, s + (aw + i) * 1024);
+        if (once) {
 #pragma unroll
-        for (int i = 0; i < DW; ++i) {
-            const int c = (lane & 7) ^ ((4 * (wave * DW + i) + (lane >> 4)) & 7);
-            ldsdma16(wsrc[i] + min(8 * jst + c, nb - 1) * 16, s + BM * 128 + (wave * DW + i) * 1024);
+            for (int i = DW * k / PT; i < DW * (k + 1) / PT; ++i)
+                ldsdma16_nt(wsrc[i] + min(KB * jst + column((ww + i) * dr), nb - 1) * 16, s + BM * KB * 16 + (ww + i) * 1024);
+        } else {
+#pragma unroll
+            for (int i = DW * k / PT; i < DW * (k + 1) / PT; ++i)
+                ldsdma16(wsrc[i] + min(KB * jst + column((ww + i) * dr), nb - 1) * 16, s + BM * KB * 16 + (ww + i) * 1024);
         }
+        if (k < PT - 1) return;
         jslot = jslot == ST - 1 ? 0 : jslot + 1;
         if (++jst == nst) {
             jst = 0;
@@ -412,27 +440,41 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
             point();
         }
     };
+    auto issue = [&]() {
+        issue_part(std::integral_constant<int, 0>());
+        if constexpr (PT > 1) issue_part(std::integral_constant<int, 1>());
+        if constexpr (PT > 2) issue_part(std::integral_constant<int, 2>());
+        if constexpr (PT > 3) issue_part(std::integral_constant<int, 3>());
+    };
+    bool parts = false;   // parts 1 .. of a stage's loads are still to be issued
+    auto issue_more = [&](auto kc) {
+        constexpr int k = decltype(kc)::value;
+        if constexpr (k < PT) {
+            if (parts) issue_part(kc);
+        }
+    };
     // scales (WORDS): the next group is that of stages sq SS .. of feature tile sf, into buffer sbuf
-    constexpr int LR = 2 * SS;   // lanes (words) of a row's group
+    constexpr int LR = KB * SS / 4;   // lanes (words) of a row's group
     constexpr int NA = WORDS ? Sh::sa : 0, NS = WORDS ? Sh::sa + Sh::sw : SR;   // the first NA are the activations'
     const uint8_t* ssrc[NS];
-    const uint8_t* slast[SR];    // (the last 8 bytes of the tensor)
+    const uint8_t* slast[SR];    // (the last KB bytes of the tensor)
     int sf = ft, sq = 0, sbuf = 0;
+    const int sw0 = wave * Sh::sa % (BM / Sh::sr > 0 ? BM / Sh::sr : 1);   // the wave's first load of the activations'
     if constexpr (WORDS) {
 #pragma unroll
-        for (int k = 0; k < NA; ++k) ssrc[k] = p.as + int64_t(max(s_row[(wave * NA + k) * (64 / LR) + lane / LR], 0)) * nb;
+        for (int k = 0; k < NA; ++k) ssrc[k] = p.as + int64_t(max(s_row[(sw0 + k) * Sh::sr + lane / LR], 0)) * nb;
     } else {
 #pragma unroll
         for (int k = 0; k < SR; ++k) {
             const bool act = tid + NT * k < BM;
             ssrc[k] = p.as + int64_t(max(s_row[act ? tid + NT * k : 0], 0)) * nb;
-            slast[k] = (act ? p.as + int64_t(p.a_rows) * nb : p.ws + int64_t(p.E) * p.N * nb) - 8;
+            slast[k] = (act ? p.as + int64_t(p.a_rows) * nb : p.ws + int64_t(p.E) * p.N * nb) - KB;
         }
     }
     auto spoint = [&]() {
 #pragma unroll
         for (int k = NA; k < NS; ++k) {
-            const int r = WORDS ? (wave * Sh::sw + k - NA) * (64 / LR) + lane / LR : min(tid + NT * k, Sh::rows - 1) - BM;
+            const int r = WORDS ? (wave * Sh::sw + k - NA) * Sh::sr + lane / LR : min(tid + NT * k, Sh::rows - 1) - BM;
             if (WORDS || r >= 0) ssrc[k] = ws + wgt_row(sf, r);
         }
     };
@@ -442,9 +484,9 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
         uint8_t* const s = s_scale + sbuf * Sh::scale_b;
         if constexpr (WORDS) {
 #pragma unroll
-            for (int k = 0; k < NA; ++k) ldsdma4(ssrc[k] + w, s + (wave * NA + k) * 256);
+            for (int k = 0; k < NA; ++k) ldsdma4(ssrc[k] + w, s + (sw0 + k) * 256);
 #pragma unroll
-            for (int k = NA; k < NS; ++k) ldsdma4(ssrc[k] + w, s + BM * SS * 8 + (wave * Sh::sw + k - NA) * 256);
+            for (int k = NA; k < NS; ++k) ldsdma4(ssrc[k] + w, s + BM * SS * KB + (wave * Sh::sw + k - NA) * 256);
         }
         sbuf ^= 1;
         if (++sq * SS >= nst) {
@@ -453,24 +495,26 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
             spoint();
         }
     };
-    // Without WORDS: the 8 scales of stage st of row tid (and those NT on), at any alignment; past the row's end they are the next row's
-    // (their steps are masked). At the tensor's end its last 8 bytes are loaded and shifted down.
-    u2e1_t sv[SR];
+    // Without WORDS: the KB scales of stage st of row tid (and those NT on), at any alignment; past the row's end they are the next
+    // row's (their steps are masked). At the tensor's end its last KB bytes are loaded and shifted down.
+    typedef std::conditional_t<KB == 8, u2e1_t, u1e1_t> Raw;
+    typedef std::conditional_t<KB == 8, uint64_t, uint32_t> Word;
+    Raw sv[SR];
     auto load_scales = [&](int st) {
 #pragma unroll
         for (int k = 0; k < SR; ++k) {
-            const uint8_t* const at = ssrc[k] + 8 * st;
-            sv[k] = *reinterpret_cast<const u2e1_t*>(at < slast[k] ? at : slast[k]);
+            const uint8_t* const at = ssrc[k] + KB * st;
+            sv[k] = *reinterpret_cast<const Raw*>(at < slast[k] ? at : slast[k]);
         }
     };
     auto put_scales = [&](int st, int buf) {
 #pragma unroll
         for (int k = 0; k < SR; ++k) {
-            const int64_t over = ssrc[k] + 8 * st - slast[k];
-            uint64_t w = uint64_t(sv[k][1]) << 32 | sv[k][0];
-            if (over > 0) w >>= 8 * int(over < 7 ? over : 7);
+            const int64_t over = ssrc[k] + KB * st - slast[k];
+            Word w = __builtin_bit_cast(Word, sv[k]);
+            if (over > 0) w >>= 8 * int(over < KB - 1 ? over : KB - 1);
             if (tid + NT * k < Sh::rows)
-                *reinterpret_cast<uint64_t*>(s_scale + buf * Sh::scale_b + ((tid + NT * k) * SS + st % SS) * 8) = w;
+                *reinterpret_cast<Word*>(s_scale + buf * Sh::scale_b + ((tid + NT * k) * SS + st % SS) * KB) = w;
         }
     };
     point();
@@ -485,30 +529,38 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
 #pragma unroll
     for (int s = 0; s < ST; ++s) issue();
 
-    const int sw = (lr >> 1) & 7;
+    const int sw = lr / (16 / KB) % KB;   // (of all its rows: they are 32 apart)
     struct Ops {
         i4_t a[FM], b[FN];
     };
     auto read = [&](int slot, int tt) {
-        const uint8_t* const s = smem + slot * Sh::code_b + ((4 * h + tt) ^ sw) * 16;
+        const uint8_t* const s = smem + slot * Sh::code_b + ((KB / 2 * h + tt) ^ sw) * 16;
         Ops o;
 #pragma unroll
-        for (int m = 0; m < FM; ++m) o.a[m] = *reinterpret_cast<const i4_t*>(s + (am + 32 * m) * 128);
+        for (int m = 0; m < FM; ++m) o.a[m] = *reinterpret_cast<const i4_t*>(s + (am + 32 * m) * KB * 16);
 #pragma unroll
-        for (int f = 0; f < FN; ++f) o.b[f] = *reinterpret_cast<const i4_t*>(s + (wf + 32 * f) * 128);
+        for (int f = 0; f < FN; ++f) o.b[f] = *reinterpret_cast<const i4_t*>(s + (wf + 32 * f) * KB * 16);
         return o;
     };
     struct Scales {
         int a[FM], b[FN];
     };
     auto read_scales = [&](int st, int buf) {
-        const uint8_t* const s = s_scale + buf * Sh::scale_b + (st % SS) * 8 + h * 4;
+        const uint8_t* const s = s_scale + buf * Sh::scale_b + (st % SS) * KB + (KB == 8 ? h * 4 : 0);
         Scales o;
 #pragma unroll
-        for (int m = 0; m < FM; ++m) o.a[m] = *reinterpret_cast<const int*>(s + (am + 32 * m) * 8 * SS);
+        for (int m = 0; m < FM; ++m) o.a[m] = *reinterpret_cast<const int*>(s + (am + 32 * m) * KB * SS);
 #pragma unroll
-        for (int f = 0; f < FN; ++f) o.b[f] = *reinterpret_cast<const int*>(s + (wf + 32 * f) * 8 * SS);
+        for (int f = 0; f < FN; ++f) o.b[f] = *reinterpret_cast<const int*>(s + (wf + 32 * f) * KB * SS);
         return o;
+    };
+    auto own_half = [&](Scales& o) {   // (4 blocks: the half's two scales at the word's low end)
+        if constexpr (KB == 4) {
+#pragma unroll
+            for (int m = 0; m < FM; ++m) o.a[m] = int(uint32_t(o.a[m]) >> 16 * h);
+#pragma unroll
+            for (int f = 0; f < FN; ++f) o.b[f] = int(uint32_t(o.b[f]) >> 16 * h);
+        }
     };
     f16_t acc[FM][FN];
     auto mma = [&](auto tc, const Ops& o, const Scales& s) {   // (features x rows: a lane's four results in a row are adjacent features)
@@ -526,11 +578,12 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
             for (int f = 0; f < FN; ++f) asm volatile("" : "+a"(acc[m][f]));
     };
 
-    // Waits count the codes' loads: at the end of a stage those of the ST - 1 stages after it were issued last, the next one's first;
-    // when the last ones are under way, all are waited for. At the end of a feature tile's first stage the stores of the tile before
-    // (kStores per wave) came behind the loads that are waited for, and may be under way too.
-    constexpr int kStores = FM * FN * int(sizeof(T)), kAfter = D * (ST - 2) + (OWN || ST == 3 ? kStores : 0);
+    // Waits count the codes' loads: at the end of a stage those of `under` (ST - 1, fewer at the sequence's end) stages after it have
+    // been issued last, the next one's first. In a feature tile's first stages the stores of the tile before (kStores per wave)
+    // came behind the loads that are waited for, and may be under way too.
+    constexpr int kStores = FM * FN * int(sizeof(T)), kAfter = D * (ST - 2) + kStores, kEarly = OWN ? ST - 1 : ST - 2;
     const int ft0 = ft;
+    int under = min(ST, (ft1 - ft) * nst) - 1;
     if ((ft1 - ft) * nst >= ST)
         wait_vm<D*(ST - 1)>();
     else
@@ -563,45 +616,63 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
             const bool last = st + 1 == nst, turn = last || (st + 1) % SS == 0;
             const int nbuf = turn ? buf ^ 1 : buf;
             if constexpr (!WORDS) put_scales(last ? 0 : st + 1, nbuf);
-            if (jf >= ft1)
-                wait_vm<0>();
-            else if (st == 0 && ft > ft0)
-                wait_vm<(kAfter < 63 ? kAfter : 63)>();
-            else
-                wait_vm<D*(ST - 2)>();
+            if (under == ST - 1) {
+                if (st < kEarly && ft > ft0)
+                    wait_vm<(kAfter < 63 ? kAfter : 63)>();
+                else
+                    wait_vm<D*(ST - 2)>();
+            } else {
+                wait_stages<D, ST - 3>(under - 1);
+            }
+            if (jf >= ft1) --under;
             ring_barrier();
             if (WORDS && turn) issue_scales();
-            if (OWN || !last) issue();
+            parts = PT > 1 && !last;
+            if (parts)
+                issue_part(std::integral_constant<int, 0>());
+            else if (OWN || !last)
+                issue();
             buf = nbuf;
             slot = slot == ST - 1 ? 0 : slot + 1;
         };
         for (int st = 0; st < nfull; ++st) {
             ahead(st);
-            const Ops o1 = read(slot, 1);
+            own_half(sc);
+            Ops o1 = read(slot, 1);
+            issue_more(std::integral_constant<int, 1>());
             __builtin_amdgcn_sched_barrier(0);
             mma(std::integral_constant<int, 0>(), o0, sc);
-            __builtin_amdgcn_sched_barrier(0);
-            const Ops o2 = read(slot, 2);
-            __builtin_amdgcn_sched_barrier(0);
-            mma(std::integral_constant<int, 1>(), o1, sc);
-            __builtin_amdgcn_sched_barrier(0);
-            const Ops o3 = read(slot, 3);
-            __builtin_amdgcn_sched_barrier(0);
-            mma(std::integral_constant<int, 2>(), o2, sc);
+            if constexpr (KB == 8) {
+                if constexpr (PT > 1) pin();
+                __builtin_amdgcn_sched_barrier(0);
+                const Ops o2 = read(slot, 2);
+                issue_more(std::integral_constant<int, 2>());
+                __builtin_amdgcn_sched_barrier(0);
+                mma(std::integral_constant<int, 1>(), o1, sc);
+                if constexpr (PT > 1) pin();
+                __builtin_amdgcn_sched_barrier(0);
+                o1 = read(slot, 3);
+                issue_more(std::integral_constant<int, 3>());
+                __builtin_amdgcn_sched_barrier(0);
+                mma(std::integral_constant<int, 2>(), o2, sc);
+            }
             pin();
             finish(st);
             o0 = read(slot, 0);   // (past the last stage: nothing that is used)
             const Scales next = read_scales(st + 1 == nst ? 0 : st + 1, buf);
             __builtin_amdgcn_sched_barrier(0);
-            mma(std::integral_constant<int, 3>(), o3, sc);
+            mma(std::integral_constant<int, KB / 2 - 1>(), o1, sc);
             sc = next;
         }
         if (nfull < nst) {
             // the last, shorter stage: blocks 2 i and 2 i + 1 in step i; a block past the row's end is zeros at scale one
             ahead(nfull);
+            issue_more(std::integral_constant<int, 1>());
+            issue_more(std::integral_constant<int, 2>());
+            issue_more(std::integral_constant<int, 3>());
             const uint8_t* const s = smem + slot * Sh::code_b;
-            const uint8_t* const ssc = s_scale + buf * Sh::scale_b + (nfull % SS) * 8;
-            const int left = nb - 8 * nfull;
+            const uint8_t* const ssc = s_scale + buf * Sh::scale_b + (nfull % SS) * KB;
+            const int left = nb - KB * nfull;
             const i4_t zero = {0, 0, 0, 0};
             for (int c = h; c - h < left; c += 2) {
                 const bool in = c < left;
@@ -610,15 +681,15 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
                 int bs[FN];
 #pragma unroll
                 for (int f = 0; f < FN; ++f) {
-                    b[f] = *reinterpret_cast<const i4_t*>(s + (wf + 32 * f) * 128 + at);
-                    bs[f] = ssc[(wf + 32 * f) * 8 * SS + c];
+                    b[f] = *reinterpret_cast<const i4_t*>(s + (wf + 32 * f) * KB * 16 + at);
+                    bs[f] = ssc[(wf + 32 * f) * KB * SS + c];
                     b[f] = in ? b[f] : zero;
                     bs[f] = in ? bs[f] : 127;
                 }
 #pragma unroll
                 for (int m = 0; m < FM; ++m) {
-                    i4_t a = *reinterpret_cast<const i4_t*>(s + (am + 32 * m) * 128 + at);
-                    int as = ssc[(am + 32 * m) * 8 * SS + c];
+                    i4_t a = *reinterpret_cast<const i4_t*>(s + (am + 32 * m) * KB * 16 + at);
+                    int as = ssc[(am + 32 * m) * KB * SS + c];
                     a = in ? a : zero;
                     as = in ? as : 127;
 #pragma unroll
@@ -669,7 +740,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
                     for (int i = 0; i < NP; ++i) {
                         const int r = r0 + i * (64 / PR);
                         const uint32_t to = r < t.rows ? uint32_t(r * int(p.ldout) + at) * sz : kNoStore;
-                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, v[i]), buffer, to, 0, 0);
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, v[i]), buffer, to, 0, 2);   // (non-temporal)
                     }
                 } else {   // the last feature tile, cut short
                     for (int i = 0; i < NP && r0 + i * (64 / PR) < t.rows; ++i)
@@ -685,7 +756,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
     }
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int ST, int SS, bool OWN, bool WORDS>
+template <typename T, int BM, int BN, int WM, int WN, int ST, int KB, int SS, bool OWN, int PT, bool WORDS>
 static int tiles_go(const Mx4Args& p, int stages, int64_t fill, hipStream_t stream) {
     const int ntile = (p.N + BN - 1) / BN;
     const int64_t tiles = tiles_at_most(p.M, p.E, BM, p.bounds != nullptr);
@@ -697,22 +768,25 @@ static int tiles_go(const Mx4Args& p, int stages, int64_t fill, hipStream_t stre
     while (nchunk < ntile && likely * nchunk < fill) ++nchunk;
     const int per = (ntile + nchunk - 1) / nchunk;
     nchunk = (ntile + per - 1) / per;
+    // (few rows to a group: only weights beyond the 256 MB of the last cache; 80 experts, 84 MB, read again and again 15.2 against 21.1 us)
+    const int stream_w = BM > 32 || groups * p.N * (p.C / 2) > (int64_t(256) << 20);
     const int64_t wgs = (tiles + 7) / 8 * 8 * nchunk;
     if (wgs > 0x7fffffff) return set_error(kErrShape, "mx4_product: M=%d N=%d E=%d", p.M, p.N, p.E);
-    constexpr int smem = TileShape<BM, BN, WM * WN, ST, SS, OWN>::smem;
+    constexpr int smem = TileShape<BM, BN, WM * WN, ST, KB, SS, OWN>::smem;
     static_assert(smem <= 160 * 1024, "LDS of a CU");
-    FRT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_mx4_tiles<T, BM, BN, WM, WN, ST, SS, OWN, WORDS>),
+    FRT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_mx4_tiles<T, BM, BN, WM, WN, ST, KB, SS, OWN, PT, WORDS>),
                                 hipFuncAttributeMaxDynamicSharedMemorySize, smem));
-    launch_timed("mx4_product", k_mx4_tiles<T, BM, BN, WM, WN, ST, SS, OWN, WORDS>, dim3(uint32_t(wgs)), dim3(64 * WM * WN), smem, stream, p, ntile,
-                 per, FastDiv(nchunk), uint32_t(nchunk));
+    launch_timed("mx4_product", k_mx4_tiles<T, BM, BN, WM, WN, ST, KB, SS, OWN, PT, WORDS>, dim3(uint32_t(wgs)), dim3(64 * WM * WN), smem, stream, p, ntile,
+                 per, FastDiv(nchunk), uint32_t(nchunk), stream_w);
     FRT_LAUNCHED("mx4_product");
     return kOk;
 }
-template <typename T, int BM, int BN, int WM, int WN, int ST, int SS, bool OWN>
+template <typename T, int BM, int BN, int WM, int WN, int ST, int KB, int SS, bool OWN, int PT>
 static int tiles_t(const Mx4Args& p, int stages, int64_t fill, hipStream_t stream) {
     const bool words = p.C % 128 == 0 && reinterpret_cast<uintptr_t>(p.as) % 4 == 0 && reinterpret_cast<uintptr_t>(p.ws) % 4 == 0;
-    return words ? tiles_go<T, BM, BN, WM, WN, ST, SS, OWN, true>(p, stages, fill, stream)
-                 : tiles_go<T, BM, BN, WM, WN, ST, SS, OWN, false>(p, stages, fill, stream);
+    if (words) return tiles_go<T, BM, BN, WM, WN, ST, KB, SS, OWN, PT, true>(p, stages, fill, stream);
+    // (the scales' way through registers waits for all loads: a third slot only takes LDS; 20480 rows, N 1000, C 1056 127 -> 119 us)
+    return tiles_go<T, BM, BN, WM, WN, 2, KB, SS, OWN, PT, false>(p, stages, fill, stream);
 }
 
 template <typename T, int KW>
@@ -739,10 +813,10 @@ static int product_t(const Mx4Args& p, hipStream_t stream) {
     const int nb = p.C / 32;   // (the tile kernels load 8 scales at a time, and store through 31-bit offsets)
     if (tiles(32, 128) >= 256 && int64_t(p.a_rows) * nb >= 8 && int64_t(p.E) * p.N * nb >= 8 &&
         int64_t(256) * p.ldout * int64_t(sizeof(T)) < 0x7fffffff) {
-        if (avg >= 1024 && tiles(256, 256) >= 256) return tiles_t<T, 256, 256, 2, 2, 2, 2, true>(p, 64, 256, stream);
-        if (avg > 56 && tiles(128, 128) >= 256) return tiles_t<T, 128, 128, 2, 2, 2, 2, false>(p, 32, 1536, stream);
-        if (avg > 8 && tiles(64, 128) >= 160) return tiles_t<T, 64, 128, 2, 2, 3, 2, false>(p, 16, 512, stream);
-        return tiles_t<T, 32, 128, 1, 4, 2, 4, false>(p, 16, 512, stream);
+        if (avg >= 1024 && tiles(256, 256) >= 256) return tiles_t<T, 256, 256, 2, 2, 2, 8, 2, true, 3>(p, 64, 256, stream);
+        if (avg > 56 && tiles(128, 128) >= 256) return tiles_t<T, 128, 128, 2, 2, 2, 8, 2, false, 1>(p, 32, 1536, stream);
+        if (avg > 8 && tiles(64, 128) >= 160) return tiles_t<T, 64, 128, 2, 2, 3, 8, 2, false, 1>(p, 16, 512, stream);
+        return tiles_t<T, 32, 128, 1, 4, 2, 8, 4, false, 1>(p, 16, 512, stream);
     }
     return nb >= 64 ? rows_t<T, 4>(p, stream) : nb >= 32 ? rows_t<T, 2>(p, stream) : rows_t<T, 1>(p, stream);
 }
