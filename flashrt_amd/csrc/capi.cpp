@@ -474,7 +474,8 @@ static int rows_check(const char* what, const char* name, const void* p, int64_t
 }
 static int move_check(const char* what, int type, int T, int K, int n) {
     if (int rc = type_check(what, type)) return rc;
-    if (T < 0 || K < 1 || n < 1 || int64_t(T) * K > 0x7fffffff) return set_error(kErrShape, "%s: T=%d K=%d n=%d", what, T, K, n);
+    if (T < 0 || K < 1 || n < 1 || n > (1 << 30) || int64_t(T) * K > 0x7fffffff)
+        return set_error(kErrShape, "%s: T=%d K=%d n=%d", what, T, K, n);
     return kOk;
 }
 static int codes_check(const char* what, const char* name, const void* codes, const void* scales) {
@@ -693,7 +694,8 @@ int frt_mx4_dequantize(void* stream, const void* codes, const void* scales, int 
 int frt_mx4_product(void* stream, const void* aq, const void* asc, int a_rows, const int32_t* rows, const void* wq,
                     const void* wsc, const int32_t* bounds, int E, int M, int N, int C, void* out, int64_t ldout, int type) {
     if (int rc = type_check("mx4_product", type)) return rc;
-    if (M < 0 || N < 1 || C < 32 || C % 32) return set_error(kErrShape, "mx4_product: M=%d N=%d C=%d (a multiple of 32)", M, N, C);
+    if (M < 0 || N < 1 || N > (1 << 30) || C < 32 || C % 32 || C > (1 << 30))
+        return set_error(kErrShape, "mx4_product: M=%d N=%d C=%d (a multiple of 32)", M, N, C);
     if (E < 1 || E > 4096 || (!bounds && E != 1)) return set_error(kErrShape, "mx4_product: E=%d%s", E, bounds ? "" : " without bounds");
     if (M == 0) return kOk;
     if (a_rows < (rows ? 1 : M)) return set_error(kErrShape, "mx4_product: %d rows of activations for M=%d", a_rows, M);

@@ -164,11 +164,15 @@ __device__ __forceinline__ RowTile find_tile(const int32_t* __restrict__ bounds,
     }
     int index = which(total), e0 = 0;
     if (index < 0 || index >= total) return {0, 0, 0, false};
-    if (E > 512)
-        for (block(0); index >= __builtin_amdgcn_readlane(incl, 63); block(e0)) {   // (ends: index < total)
-            index -= __builtin_amdgcn_readlane(incl, 63);
-            e0 += 512;
+    if (E > 512) {   // (the last block is in the registers: from the first one again)
+        for (; e0 < E; e0 += 512) {
+            block(e0);
+            const int here = __builtin_amdgcn_readlane(incl, 63);
+            if (index < here) break;
+            index -= here;
         }
+        if (e0 >= E) return {0, 0, 0, false};
+    }
     const int owner = __builtin_ctzll(__ballot(incl > index));
     int left = index - (incl - n), g = 0, row0 = 0, rows = 0, of = 0;   // (of use in that lane)
 #pragma unroll

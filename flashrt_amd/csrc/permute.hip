@@ -217,8 +217,12 @@ int moe_sort(const int32_t* ids, int T, int K, int E, int32_t* bounds, int32_t* 
     while ((1 << id_bits) < E) ++id_bits;
     const int nb = int((int64_t(S) + 1023) / 1024);
     const int batches = (nb + kSortGrid - 1) / kSortGrid;
-    launch_timed("moe_sort", nb == 1 ? k_sort<true> : k_sort<false>, dim3((nb + batches - 1) / batches), dim3(1024),
-                 size_t(E) * kSortCopies * 4, stream, ids, S, K, E, id_bits, batches, bounds, tok_of, slot_of, row_of);
+    const size_t lds = size_t(E) * kSortCopies * 4;
+    const auto kernel = nb == 1 ? k_sort<true> : k_sort<false>;
+    if (lds + 8192 > 65536)
+        FRT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
+    launch_timed("moe_sort", kernel, dim3((nb + batches - 1) / batches), dim3(1024),
+                 lds, stream, ids, S, K, E, id_bits, batches, bounds, tok_of, slot_of, row_of);
     FRT_LAUNCHED("moe_sort");
     return kOk;
 }

@@ -69,7 +69,7 @@ def test_refusals_before_any_launch():
                                                    (7, None, -4), (6, p + 8, -1), (1, p + 2, -1)]),
                           (L.frt_mx4_dequantize, d, [(6, 63, -1), (7, 2, -1), (3, -1, -1), (4, 16, -1), (1, None, -4), (2, None, -4), (5, None, -4),
                                                      (1, p + 1, -1), (5, p + 1, -1)]),
-                          (L.frt_mx4_product, m, [(14, 7, -1), (13, 23, -1), (8, 0, -1), (8, 4097, -1), (9, -1, -1), (10, 0, -1), (11, 48, -1),
+                          (L.frt_mx4_product, m, [(14, 7, -1), (13, 23, -1), (8, 0, -1), (8, 4097, -1), (9, -1, -1), (10, 0, -1), (10, (1 << 30) + 1, -1), (11, 48, -1),
                                                   (3, 0, -1), (1, None, -4), (2, None, -4), (5, None, -4), (6, None, -4), (12, None, -4), (1, p + 4, -1),
                                                   (5, p + 4, -1), (12, p + 1, -1), (7, None, -1)])):
         for i, v, rc in bad:
@@ -263,6 +263,72 @@ def test_product_groups(groups, N, C, gather, kind):
     check_product(run_product(F, ops, M, kind, bounds, rows, pad=1), ops, M, kind, bounds, rows)
 
 
+# groups and features that fill the chip with tiles of 32, 64, 128 and 256 rows; ragged, with empty and far larger groups among them
+TILES = {
+    "rows32": ([(5 * i) % 9 for i in range(90)] + [70, 0], 395),
+    "rows64": ([17 + (7 * i) % 23 for i in range(62)] + [0, 129], 424),
+    "rows128": ([60 + (31 * i) % 150 for i in range(20)] + [0, 300], 1608),
+    "rows256": ([4200], 4104),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("tile", list(TILES))
+@pytest.mark.parametrize("C", [64, 256, 544, 640, 1408])
+def test_product_tiles(tile, C, kind):
+    """Every tile size, with rows of fewer than one stage (256 values) to several, whole words of scales (C % 128 = 0) and not; tokens
+    picked by index, some outside, and rows behind the last group."""
+    import flashrt_amd as F
+    sizes, N = TILES[tile]
+    bounds = cut(sizes)
+    M = bounds[-1] + 5
+    gather = kind is not torch.float16
+    ops = operands(57 if gather else M, len(sizes), N, C, C)
+    rows = None
+    if gather:
+        rows = np.random.default_rng(C).integers(0, 57, M)
+        rows[::29], rows[1::31] = -1, 57
+    check_product(run_product(F, ops, M, kind, bounds, rows, pad=3), ops, M, kind, bounds, rows)
+
+
+@pytest.mark.gpu
+def test_product_many_groups():
+    """More than 512 groups (their bounds are read in blocks): 1500, most of one row or none, over tiles and over few features."""
+    import flashrt_amd as F
+    sizes = [(i * 7) % 3 for i in range(1500)]
+    bounds = cut(sizes)
+    for N in (8, 200):
+        ops = operands(bounds[-1], 1500, N, 96, N)
+        check_product(run_product(F, ops, bounds[-1], torch.float32, bounds), ops, bounds[-1], torch.float32, bounds)
+
+
+@pytest.mark.gpu
+def test_product_tiles_captured():
+    """The tile kernels in a graph, replayed on other activations and bounds with eager work between, each replay equal to the eager call."""
+    import flashrt_amd as F
+    E, N, C, M = 64, 512, 512, 1500
+    ops = operands(M, E, N, C, 3)
+    aq, asc, wq, wsc = (torch.from_numpy(v).cuda() for v in ops)
+    bounds = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    out, want = torch.zeros(M, N, device="cuda"), torch.zeros(M, N, device="cuda")
+    F.mx4_product(aq, asc, wq, wsc, out, bounds=bounds)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        F.mx4_product(aq, asc, wq, wsc, out, bounds=bounds)
+    for seed in range(3):
+        aq.copy_(torch.from_numpy(operands(M, 1, 1, C, 40 + seed)[0]))
+        cuts = np.sort(np.random.default_rng(seed).integers(0, M + 1, E + 1)).astype(np.int32)
+        bounds.copy_(torch.from_numpy(cuts))
+        out.zero_(), want.zero_()
+        F.mx4_product(aq, asc, wq, wsc, want, bounds=bounds)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and bool((out[:int(cuts[0])] == 0).all()) and bool((out[int(cuts[-1]):] == 0).all())
+
+
 @pytest.mark.gpu
 def test_product_scales():
     """Scales far apart whose products stay in range; and a NaN block reaches its own row, or its own feature, alone."""
@@ -308,10 +374,12 @@ def test_bounds_out_of_order_stay_inside():
 
 
 @pytest.mark.gpu
-def test_weights_past_32_bits():
-    """The last experts of a weight tensor of more than 2^32 bytes: 1100 experts of 2048 x 4096."""
+@pytest.mark.parametrize("M", [6, 70])
+def test_weights_past_32_bits(M):
+    """The last experts of a weight tensor of more than 2^32 bytes, 1100 experts of 2048 x 4096: for few rows, and in tiles with the
+    weights streamed."""
     import flashrt_amd as F
-    E, N, C, M = 1100, 2048, 4096, 6
+    E, N, C = 1100, 2048, 4096
     wq = torch.zeros((E, N, C // 2), dtype=torch.uint8, device="cuda")
     wsc = torch.full((E, N, C // 32), 127, dtype=torch.uint8, device="cuda")
     assert wq.numel() > 2 ** 32
@@ -319,10 +387,10 @@ def test_weights_past_32_bits():
     aq, asc, q, s = (torch.from_numpy(v).cuda() for v in ops)
     wq[E - 2:], wsc[E - 2:] = q, s
     bounds = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
-    bounds[E - 1], bounds[E] = 4, 6
+    bounds[E - 1], bounds[E] = 4, M
     out = torch.empty(M, N, device="cuda")
     F.mx4_product(aq, asc, wq, wsc, out, bounds=bounds)
-    check_product(out, ops, M, torch.float32, [0, 4, 6])
+    check_product(out, ops, M, torch.float32, [0, 4, M])
 
 
 @pytest.mark.gpu

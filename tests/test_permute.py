@@ -87,7 +87,7 @@ def test_refusals_before_any_launch():
              (L.frt_moe_unpermute, [None, p, 8, 0, 2, 2, 8, p, p, p, 8], 3, (1, 7, 8, 9), (2, 10)),
              (L.frt_moe_unpermute_grad, [None, p, 8, p, 8, 0, 2, 2, 8, p, p, p, 8, p], 5, (1, 3, 9, 10, 11, 13), (2, 4, 12))]
     for fn, good, at, ptrs, lds in calls:
-        for i, v, rc in [(at, 2, -1), (at, -1, -1), (at + 1, -1, -1), (at + 2, 0, -1), (at + 3, 0, -1), (at + 1, 1 << 30, -1)] + \
+        for i, v, rc in [(at, 2, -1), (at, -1, -1), (at + 1, -1, -1), (at + 2, 0, -1), (at + 3, 0, -1), (at + 3, (1 << 30) + 1, -1), (at + 1, 1 << 30, -1)] + \
                 [(i, None, -4) for i in ptrs] + [(i, 7, -1) for i in lds]:
             a = list(good)
             a[i] = v
@@ -124,7 +124,7 @@ def test_python_refusals():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["flat", "hot", "drop", "none"])
-@pytest.mark.parametrize("T,K,E", [(1, 1, 1), (1, 10, 512), (1, 32, 1024), (3, 5, 7), (64, 1, 2), (93, 11, 65), (128, 8, 128), (205, 10, 1000),
+@pytest.mark.parametrize("T,K,E", [(1, 1, 1), (1, 10, 512), (1, 32, 1024), (3, 5, 7), (64, 1, 2), (65, 1, 1), (50, 10, 1024), (93, 11, 65), (128, 8, 128), (205, 10, 1000),
                                    (1024, 1, 1), (2048, 10, 512), (5003, 3, 8)])
 def test_sort(T, K, E, kind):
     import flashrt_amd as F
