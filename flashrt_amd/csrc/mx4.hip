@@ -17,7 +17,6 @@ namespace frt {
 typedef uint32_t u4e4_t __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u4e2_t __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u4e1_t __attribute__((ext_vector_type(4), aligned(1)));
-typedef uint32_t u1e1_t __attribute__((aligned(1)));
 typedef uint32_t u2e1_t __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t u2e2_t __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
@@ -327,7 +326,8 @@ __device__ __forceinline__ void wave_lds_order() {
     asm volatile("" ::: "memory");
 }
 
-template <int BM, int BN, int NW, int ST, int KB, int SS, bool OWN>
+constexpr int KB = 8;   // blocks of a row in a stage
+template <int BM, int BN, int NW, int ST, int SS>
 struct TileShape {
     static constexpr int rows = BM + BN;                // operand rows of a stage, the activations first
     static constexpr int code_b = rows * KB * 16;       // a stage: KB blocks of 32 values of each row
@@ -338,10 +338,10 @@ struct TileShape {
     static_assert((BM % (dr * NW) == 0 || (dr * NW) % BM == 0) && BN % (dr * NW) == 0 && (BM % (sr * NW) == 0 || (sr * NW) % BM == 0) &&
                   BN % (sr * NW) == 0, "every wave the same loads");
     static constexpr int scale_b = rows * SS * KB;      // a group's scales
-    // The results leave through LDS, by wave: OWN, an area beside the ring, else a slot of it, in rows of 64 bytes (128 where they fit)
-    static constexpr int out_row = OWN || NW * 32 * 144 > code_b ? 64 : 128, out_b = 32 * (out_row + 16);
-    static_assert(OWN || NW * out_b <= code_b, "the results in a slot");
-    static constexpr int smem = ST * code_b + 2 * scale_b + BM * 4 + (OWN ? NW * out_b : 0);
+    // The results leave through LDS, each wave its part of a slot, in rows of 128 bytes (64 where those do not fit)
+    static constexpr int out_row = NW * 32 * 144 > code_b ? 64 : 128, out_b = 32 * (out_row + 16);
+    static_assert(NW * out_b <= code_b, "the results in a slot");
+    static constexpr int smem = ST * code_b + 2 * scale_b + BM * 4;
 };
 
 // Stores through a buffer descriptor: a lane whose offset lies past its bytes stores nothing, without a branch, so that the number of
@@ -351,17 +351,17 @@ constexpr uint32_t kNoStore = 0x80000000u;
 
 // BM rows x BN features per tile, `per` feature tiles of one row tile after one another in a workgroup of WM x WN waves, from
 // LDS. A stage is KB blocks of 32 values of every operand row, in a ring of ST slots, their codes loaded straight into it; block c of
-// row r sits at c ^ (r / (16 / KB)) % KB, so that the sixteen rows of a read phase take sixteen different columns of the banks.
+// row r sits at c ^ (r / 2 % 8), so that the sixteen rows of a read phase take sixteen different columns of the banks.
 // The scales of SS stages at a time (side by side in a row: the loads' cost is lines, not bytes) go the same way where the rows of
-// scales are words (WORDS: a multiple of 128 values), else a stage's through registers. In step t (0 .. KB / 2 - 1) lane half h
-// multiplies block KB / 2 h + t of its rows, so that a lane's scales of a stage lie in one word and the step picks its byte. Step t +
+// scales are words (WORDS: a multiple of 128 values), else a stage's through registers. In step t (0..3) lane half h
+// multiplies block 4 h + t of its rows, so that a lane's four scales of a stage are one word and the step picks its byte. Step t +
 // 1's operands are read before step t's products, the next stage's first ones before the last step's, past the barrier. The
 // stages of the feature tiles form one sequence: the next tile's first stages load while this one's results are written.
-template <typename T, int BM, int BN, int WM, int WN, int ST, int KB, int SS, bool OWN, int PT, bool WORDS>
+template <typename T, int BM, int BN, int WM, int WN, int ST, int SS, int PT, bool WORDS>
 __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile, int per, FastDiv chunks, uint32_t nchunk, int stream) {
     constexpr int NW = WM * WN, NT = 64 * NW;
-    using Sh = TileShape<BM, BN, NW, ST, KB, SS, OWN>;
-    static_assert(SS >= 2 && ST >= 2 && (KB == 4 || KB == 8) && PT <= KB / 2, "scales a group ahead; steps");
+    using Sh = TileShape<BM, BN, NW, ST, SS>;
+    static_assert(SS >= 2 && ST >= 2 && PT <= 4, "scales a group ahead; four steps");
     constexpr int FM = BM / WM / 32, FN = BN / WN / 32, DA = Sh::da, DW = Sh::dw, D = DA + DW, SR = (Sh::rows + NT - 1) / NT;
     extern __shared__ __align__(16) uint8_t smem[];
     uint8_t* const s_scale = smem + ST * Sh::code_b;
@@ -501,24 +501,22 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
     };
     // Without WORDS: the KB scales of stage st of row tid (and those NT on), at any alignment; past the row's end they are the next
     // row's (their steps are masked). At the tensor's end its last KB bytes are loaded and shifted down.
-    typedef std::conditional_t<KB == 8, u2e1_t, u1e1_t> Raw;
-    typedef std::conditional_t<KB == 8, uint64_t, uint32_t> Word;
-    Raw sv[SR];
+    u2e1_t sv[SR];
     auto load_scales = [&](int st) {
 #pragma unroll
         for (int k = 0; k < SR; ++k) {
             const uint8_t* const at = ssrc[k] + KB * st;
-            sv[k] = *reinterpret_cast<const Raw*>(at < slast[k] ? at : slast[k]);
+            sv[k] = *reinterpret_cast<const u2e1_t*>(at < slast[k] ? at : slast[k]);
         }
     };
     auto put_scales = [&](int st, int buf) {
 #pragma unroll
         for (int k = 0; k < SR; ++k) {
             const int64_t over = ssrc[k] + KB * st - slast[k];
-            Word w = __builtin_bit_cast(Word, sv[k]);
+            uint64_t w = uint64_t(sv[k][1]) << 32 | sv[k][0];
             if (over > 0) w >>= 8 * int(over < KB - 1 ? over : KB - 1);
             if (tid + NT * k < Sh::rows)
-                *reinterpret_cast<Word*>(s_scale + buf * Sh::scale_b + ((tid + NT * k) * SS + st % SS) * KB) = w;
+                *reinterpret_cast<uint64_t*>(s_scale + buf * Sh::scale_b + ((tid + NT * k) * SS + st % SS) * KB) = w;
         }
     };
     point();
@@ -550,21 +548,13 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
         int a[FM], b[FN];
     };
     auto read_scales = [&](int st, int buf) {
-        const uint8_t* const s = s_scale + buf * Sh::scale_b + (st % SS) * KB + (KB == 8 ? h * 4 : 0);
+        const uint8_t* const s = s_scale + buf * Sh::scale_b + (st % SS) * KB + h * 4;
         Scales o;
 #pragma unroll
         for (int m = 0; m < FM; ++m) o.a[m] = *reinterpret_cast<const int*>(s + (am + 32 * m) * KB * SS);
 #pragma unroll
         for (int f = 0; f < FN; ++f) o.b[f] = *reinterpret_cast<const int*>(s + (wf + 32 * f) * KB * SS);
         return o;
-    };
-    auto own_half = [&](Scales& o) {   // (4 blocks: the half's two scales at the word's low end)
-        if constexpr (KB == 4) {
-#pragma unroll
-            for (int m = 0; m < FM; ++m) o.a[m] = int(uint32_t(o.a[m]) >> 16 * h);
-#pragma unroll
-            for (int f = 0; f < FN; ++f) o.b[f] = int(uint32_t(o.b[f]) >> 16 * h);
-        }
     };
     f16_t acc[FM][FN];
     auto mma = [&](auto tc, const Ops& o, const Scales& s) {   // (features x rows: a lane's four results in a row are adjacent features)
@@ -585,7 +575,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
     // Waits count the codes' loads: at the end of a stage those of `under` (ST - 1, fewer at the sequence's end) stages after it have
     // been issued last, the next one's first. In a feature tile's first stages the stores of the tile before (kStores per wave)
     // came behind the loads that are waited for, and may be under way too.
-    constexpr int kStores = FM * FN * int(sizeof(T)), kAfter = D * (ST - 2) + kStores, kEarly = OWN ? ST - 1 : ST - 2;
+    constexpr int kStores = FM * FN * int(sizeof(T)), kAfter = D * (ST - 2) + kStores;
     const int ft0 = ft;
     int under = min(ST, (ft1 - ft) * nst) - 1;
     if ((ft1 - ft) * nst >= ST)
@@ -621,7 +611,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
             const int nbuf = turn ? buf ^ 1 : buf;
             if constexpr (!WORDS) put_scales(last ? 0 : st + 1, nbuf);
             if (under == ST - 1) {
-                if (st < kEarly && ft > ft0)
+                if (st < ST - 2 && ft > ft0)
                     wait_vm<(kAfter < 63 ? kAfter : 63)>();
                 else
                     wait_vm<D*(ST - 2)>();
@@ -634,38 +624,35 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
             parts = PT > 1 && !last;
             if (parts)
                 issue_part(std::integral_constant<int, 0>());
-            else if (OWN || !last)
+            else if (!last)
                 issue();
             buf = nbuf;
             slot = slot == ST - 1 ? 0 : slot + 1;
         };
         for (int st = 0; st < nfull; ++st) {
             ahead(st);
-            own_half(sc);
             Ops o1 = read(slot, 1);
             issue_more(std::integral_constant<int, 1>());
             __builtin_amdgcn_sched_barrier(0);
             mma(std::integral_constant<int, 0>(), o0, sc);
-            if constexpr (KB == 8) {
-                if constexpr (PT > 1) pin();
-                __builtin_amdgcn_sched_barrier(0);
-                const Ops o2 = read(slot, 2);
-                issue_more(std::integral_constant<int, 2>());
-                __builtin_amdgcn_sched_barrier(0);
-                mma(std::integral_constant<int, 1>(), o1, sc);
-                if constexpr (PT > 1) pin();
-                __builtin_amdgcn_sched_barrier(0);
-                o1 = read(slot, 3);
-                issue_more(std::integral_constant<int, 3>());
-                __builtin_amdgcn_sched_barrier(0);
-                mma(std::integral_constant<int, 2>(), o2, sc);
-            }
+            if constexpr (PT > 1) pin();
+            __builtin_amdgcn_sched_barrier(0);
+            const Ops o2 = read(slot, 2);
+            issue_more(std::integral_constant<int, 2>());
+            __builtin_amdgcn_sched_barrier(0);
+            mma(std::integral_constant<int, 1>(), o1, sc);
+            if constexpr (PT > 1) pin();
+            __builtin_amdgcn_sched_barrier(0);
+            o1 = read(slot, 3);
+            issue_more(std::integral_constant<int, 3>());
+            __builtin_amdgcn_sched_barrier(0);
+            mma(std::integral_constant<int, 2>(), o2, sc);
             pin();
             finish(st);
             o0 = read(slot, 0);   // (past the last stage: nothing that is used)
             const Scales next = read_scales(st + 1 == nst ? 0 : st + 1, buf);
             __builtin_amdgcn_sched_barrier(0);
-            mma(std::integral_constant<int, KB / 2 - 1>(), o1, sc);
+            mma(std::integral_constant<int, 3>(), o1, sc);
             sc = next;
         }
         if (nfull < nst) {
@@ -712,8 +699,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
         constexpr int PR = QP * 8 / V, NP = 32 * PR / 64, RS = Sh::out_row + 16;   // pieces of 16 bytes in a row, of a lane; bytes from row to row
         static_assert(4 * FN % QP == 0 && FM * (4 * FN / QP) * NP == kStores, "the stores of a wave");
         typedef T vec4 __attribute__((ext_vector_type(4)));
-        uint8_t* const w = OWN ? smem + ST * Sh::code_b + 2 * Sh::scale_b + BM * 4 + wave * Sh::out_b
-                               : smem + (slot == 0 ? ST - 1 : slot - 1) * Sh::code_b + wave * (Sh::code_b / NW);
+        uint8_t* const w = smem + (slot == 0 ? ST - 1 : slot - 1) * Sh::code_b + wave * (Sh::code_b / NW);
         T* const out = static_cast<T*>(p.out) + t.row0 * p.ldout;
         const Buffer buffer = __builtin_amdgcn_make_buffer_rsrc(out, 0, int(((t.rows - 1) * p.ldout + p.N) * sz), 0x00020000);
 #pragma unroll
@@ -754,13 +740,12 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
                 wave_lds_order();
             }
         }
-        if constexpr (OWN) continue;
         ring_barrier();   // every wave's results have left the slot
         issue();
     }
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int ST, int KB, int SS, bool OWN, int PT, bool WORDS>
+template <typename T, int BM, int BN, int WM, int WN, int ST, int SS, int PT, bool WORDS>
 static int tiles_go(const Mx4Args& p, int stages, int64_t fill, hipStream_t stream) {
     const int ntile = (p.N + BN - 1) / BN;
     const int64_t tiles = tiles_at_most(p.M, p.E, BM, p.bounds != nullptr);
@@ -776,21 +761,21 @@ static int tiles_go(const Mx4Args& p, int stages, int64_t fill, hipStream_t stre
     const int stream_w = BM > 32 || groups * p.N * (p.C / 2) > (int64_t(256) << 20);
     const int64_t wgs = (tiles + 7) / 8 * 8 * nchunk;
     if (wgs > 0x7fffffff) return set_error(kErrShape, "mx4_product: M=%d N=%d E=%d", p.M, p.N, p.E);
-    constexpr int smem = TileShape<BM, BN, WM * WN, ST, KB, SS, OWN>::smem;
+    constexpr int smem = TileShape<BM, BN, WM * WN, ST, SS>::smem;
     static_assert(smem <= 160 * 1024, "LDS of a CU");
-    FRT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_mx4_tiles<T, BM, BN, WM, WN, ST, KB, SS, OWN, PT, WORDS>),
+    FRT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_mx4_tiles<T, BM, BN, WM, WN, ST, SS, PT, WORDS>),
                                 hipFuncAttributeMaxDynamicSharedMemorySize, smem));
-    launch_timed("mx4_product", k_mx4_tiles<T, BM, BN, WM, WN, ST, KB, SS, OWN, PT, WORDS>, dim3(uint32_t(wgs)), dim3(64 * WM * WN), smem, stream, p, ntile,
+    launch_timed("mx4_product", k_mx4_tiles<T, BM, BN, WM, WN, ST, SS, PT, WORDS>, dim3(uint32_t(wgs)), dim3(64 * WM * WN), smem, stream, p, ntile,
                  per, FastDiv(nchunk), uint32_t(nchunk), stream_w);
     FRT_LAUNCHED("mx4_product");
     return kOk;
 }
-template <typename T, int BM, int BN, int WM, int WN, int ST, int KB, int SS, bool OWN, int PT>
+template <typename T, int BM, int BN, int WM, int WN, int ST, int SS, int PT>
 static int tiles_t(const Mx4Args& p, int stages, int64_t fill, hipStream_t stream) {
     const bool words = p.C % 128 == 0 && reinterpret_cast<uintptr_t>(p.as) % 4 == 0 && reinterpret_cast<uintptr_t>(p.ws) % 4 == 0;
-    if (words) return tiles_go<T, BM, BN, WM, WN, ST, KB, SS, OWN, PT, true>(p, stages, fill, stream);
+    if (words) return tiles_go<T, BM, BN, WM, WN, ST, SS, PT, true>(p, stages, fill, stream);
     // (the scales' way through registers waits for all loads: a third slot only takes LDS; 20480 rows, N 1000, C 1056 127 -> 119 us)
-    return tiles_go<T, BM, BN, WM, WN, 2, KB, SS, OWN, PT, false>(p, stages, fill, stream);
+    return tiles_go<T, BM, BN, WM, WN, 2, SS, PT, false>(p, stages, fill, stream);
 }
 
 template <typename T, int KW>
@@ -817,10 +802,10 @@ static int product_t(const Mx4Args& p, hipStream_t stream) {
     const int nb = p.C / 32;   // (the tile kernels load 8 scales at a time, and store through 31-bit offsets)
     if (tiles(32, 128) >= 256 && int64_t(p.a_rows) * nb >= 8 && int64_t(p.E) * p.N * nb >= 8 &&
         int64_t(256) * p.ldout * int64_t(sizeof(T)) < 0x7fffffff) {
-        if (avg >= 1024 && tiles(256, 256) >= 256) return tiles_t<T, 256, 256, 2, 2, 2, 8, 2, true, 3>(p, 64, 256, stream);
-        if (avg > 56 && tiles(128, 128) >= 256) return tiles_t<T, 128, 128, 2, 2, 2, 8, 2, false, 1>(p, 32, 1536, stream);
-        if (avg > 8 && tiles(64, 128) >= 160) return tiles_t<T, 64, 128, 2, 2, 3, 8, 2, false, 1>(p, 16, 512, stream);
-        return tiles_t<T, 32, 128, 1, 4, 2, 8, 4, false, 1>(p, 16, 512, stream);
+        if (avg >= 1024 && tiles(256, 256) >= 256) return tiles_t<T, 256, 256, 4, 2, 2, 2, 3>(p, 64, 256, stream);
+        if (avg > 56 && tiles(128, 128) >= 256) return tiles_t<T, 128, 128, 2, 2, 2, 2, 1>(p, 32, 1536, stream);
+        if (avg > 8 && tiles(64, 128) >= 160) return tiles_t<T, 64, 128, 2, 2, 3, 2, 1>(p, 16, 512, stream);
+        return tiles_t<T, 32, 128, 1, 4, 2, 4, 1>(p, 16, 512, stream);
     }
     return nb >= 64 ? rows_t<T, 4>(p, stream) : nb >= 32 ? rows_t<T, 2>(p, stream) : rows_t<T, 1>(p, stream);
 }
