@@ -308,17 +308,6 @@ __global__ void __launch_bounds__(256) k_mx4_rows(Mx4Args p, int ntile, FastDiv 
     }
 }
 
-// Waits until at most n stages of D loads (n <= MOST) are under way
-template <int D, int MOST>
-__device__ __forceinline__ void wait_stages(int n) {
-    if constexpr (MOST > 0)
-        if (n >= MOST) return wait_vm<D * MOST>();
-    if constexpr (MOST > 0)
-        wait_stages<D, MOST - 1>(n);
-    else
-        wait_vm<0>();
-}
-
 // A wave's LDS accesses before are done before those after, across its lanes (they complete in order)
 __device__ __forceinline__ void wave_lds_order() {
     asm volatile("" ::: "memory");
@@ -361,7 +350,7 @@ template <typename T, int BM, int BN, int WM, int WN, int ST, int SS, int PT, bo
 __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile, int per, FastDiv chunks, uint32_t nchunk, int stream) {
     constexpr int NW = WM * WN, NT = 64 * NW;
     using Sh = TileShape<BM, BN, NW, ST, SS>;
-    static_assert(SS >= 2 && ST >= 2 && PT <= 4, "scales a group ahead; four steps");
+    static_assert(SS >= 2 && (ST == 2 || ST == 3) && PT <= 3, "scales a group ahead; the waits; the steps before a stage's end");
     constexpr int FM = BM / WM / 32, FN = BN / WN / 32, DA = Sh::da, DW = Sh::dw, D = DA + DW, SR = (Sh::rows + NT - 1) / NT;
     extern __shared__ __align__(16) uint8_t smem[];
     uint8_t* const s_scale = smem + ST * Sh::code_b;
@@ -448,7 +437,6 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
         issue_part(std::integral_constant<int, 0>());
         if constexpr (PT > 1) issue_part(std::integral_constant<int, 1>());
         if constexpr (PT > 2) issue_part(std::integral_constant<int, 2>());
-        if constexpr (PT > 3) issue_part(std::integral_constant<int, 3>());
     };
     bool parts = false;   // parts 1 .. of a stage's loads are still to be issued
     auto issue_more = [&](auto kc) {
@@ -616,7 +604,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
                 else
                     wait_vm<D*(ST - 2)>();
             } else {
-                wait_stages<D, ST - 3>(under - 1);
+                wait_vm<0>();
             }
             if (jf >= ft1) --under;
             ring_barrier();
@@ -644,7 +632,6 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
             if constexpr (PT > 1) pin();
             __builtin_amdgcn_sched_barrier(0);
             o1 = read(slot, 3);
-            issue_more(std::integral_constant<int, 3>());
             __builtin_amdgcn_sched_barrier(0);
             mma(std::integral_constant<int, 2>(), o2, sc);
             pin();
@@ -660,7 +647,6 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
             ahead(nfull);
             issue_more(std::integral_constant<int, 1>());
             issue_more(std::integral_constant<int, 2>());
-            issue_more(std::integral_constant<int, 3>());
             const uint8_t* const s = smem + slot * Sh::code_b;
             const uint8_t* const ssc = s_scale + buf * Sh::scale_b + (nfull % SS) * KB;
             const int left = nb - KB * nfull;
@@ -790,19 +776,21 @@ static int rows_t(const Mx4Args& p, hipStream_t stream) {
 
 template <typename T>
 static int product_t(const Mx4Args& p, hipStream_t stream) {
-    // The tile by the rows of a group, were they spread evenly: with few rows the weights' bytes are all there is to read, and small
-    // tiles put more of them in flight; with many the operands pass through LDS less often. Measured, smaller against larger tile:
-    //   rows 32 / 64: 4 rows to a group (N 1024, C 2048) 79.5 / 82.7 us, 16 rows 127 / 122
-    //   64 / 128: 40 rows 139 / 154 us, 62 rows 159 / 151, 160 rows 250 / 226
-    //   128 / 256: one group of 8192 (N 8192, C 4096) 184 / 151 us, of 2048 51 / 46, of 8 groups of 512 rows (N, C 2048) 24 / 26
-    // Below one workgroup of the smallest tile per CU the waves split a row's values instead: ten groups of one row 8.6 -> 7.2 us,
-    // one row of N 8192, C 4096 10.4 -> 6.8, 16 rows 10.9 -> 8.4; at 128 rows, 256 such workgroups, 12.6 against 20.
+    // The kernel by the rows of a group, were they spread evenly. With few rows the weights' bytes are all there is to read, and small
+    // tiles put more of them in flight; with many the operands pass through LDS less often. us, smaller against larger:
+    //   values split over the waves / tiles of 32, by the weights that tiles of 16 rows read: one token's ten experts (N 1024, C 2048,
+    //     10 MB) 7.2 / 7.8, two tokens' 11.2 / 9.4, one group (N 8192, C 4096) of 16 rows (16 MB) 8.4 / 12.4, of 24 13.3 / 12.5
+    //   32 / 64 (512 experts, N 1024, C 2048): 4 rows to an expert 68 / 74, 16 rows 108 / 107, 40 rows 143 / 123
+    //   64 / 128: 40 rows 123 / 149, 62 rows 147 / 140, 160 rows 264 / 240; one group of 512 (N, C 2560) 10.3 / 12.1
+    //   128 / 256: 160 rows 240 / 276; 16 experts (N, C 2048) of 300 rows 24.3 / 23.1, 8 of 512 23.4 / 21.5; one group of 8192 (N 8192,
+    //     C 4096) 201 / 149
     const int64_t groups = p.bounds ? std::min(p.E, p.M) : 1, avg = p.M / groups;
-    auto tiles = [&](int64_t BM, int64_t BN) { return ((avg + BM - 1) / BM * groups) * ((p.N + BN - 1) / BN); };
+    auto rows = [&](int64_t BM) { return (avg + BM - 1) / BM * groups; };   // tiles of BM rows
+    auto tiles = [&](int64_t BM, int64_t BN) { return rows(BM) * ((p.N + BN - 1) / BN); };
     const int nb = p.C / 32;   // (the tile kernels load 8 scales at a time, and store through 31-bit offsets)
-    if (tiles(32, 128) >= 256 && int64_t(p.a_rows) * nb >= 8 && int64_t(p.E) * p.N * nb >= 8 &&
+    if (rows(16) * p.N * (p.C / 2) > (int64_t(16) << 20) && int64_t(p.a_rows) * nb >= 8 && int64_t(p.E) * p.N * nb >= 8 &&
         int64_t(256) * p.ldout * int64_t(sizeof(T)) < 0x7fffffff) {
-        if (avg >= 1024 && tiles(256, 256) >= 256) return tiles_t<T, 256, 256, 4, 2, 2, 2, 3>(p, 64, 256, stream);
+        if (avg >= 256 && tiles(256, 256) >= 128) return tiles_t<T, 256, 256, 4, 2, 2, 2, 3>(p, 64, 256, stream);
         if (avg > 56 && tiles(128, 128) >= 256) return tiles_t<T, 128, 128, 2, 2, 2, 2, 1>(p, 32, 1536, stream);
         if (avg > 8 && tiles(64, 128) >= 160) return tiles_t<T, 64, 128, 2, 2, 3, 2, 1>(p, 16, 512, stream);
         return tiles_t<T, 32, 128, 1, 4, 2, 4, 1>(p, 16, 512, stream);

@@ -263,7 +263,8 @@ def test_product_groups(groups, N, C, gather, kind):
     check_product(run_product(F, ops, M, kind, bounds, rows, pad=1), ops, M, kind, bounds, rows)
 
 
-# groups and features that fill the chip with tiles of 32, 64, 128 and 256 rows; ragged, with empty and far larger groups among them
+# (rows of the groups, features) for the tiles of 32, 64, 128 and 256 rows; ragged, with empty and far larger groups among them. The
+# groups are repeated until their weights, read by tiles of 16 rows, are over the 16 MB below which the values are split instead.
 TILES = {
     "rows32": ([(5 * i) % 9 for i in range(90)] + [70, 0], 395),
     "rows64": ([17 + (7 * i) % 23 for i in range(62)] + [0, 129], 424),
@@ -273,14 +274,17 @@ TILES = {
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("tile", list(TILES))
-@pytest.mark.parametrize("C", [64, 256, 544, 640, 1408])
+@pytest.mark.parametrize("C,kind", [(64, torch.bfloat16), (256, torch.float32), (544, torch.float16), (544, torch.float32), (640, torch.bfloat16),
+                                    (1408, torch.float32), (1408, torch.float16)])
 def test_product_tiles(tile, C, kind):
     """Every tile size, with rows of fewer than one stage (256 values) to several, whole words of scales (C % 128 = 0) and not; tokens
     picked by index, some outside, and rows behind the last group."""
     import flashrt_amd as F
     sizes, N = TILES[tile]
+    if len(sizes) > 1:
+        avg = sum(sizes) // len(sizes)
+        sizes = sizes * max(1, -(-(17 << 20) // (-(-avg // 16) * len(sizes) * N * C // 2)))
     bounds = cut(sizes)
     M = bounds[-1] + 5
     gather = kind is not torch.float16
@@ -298,7 +302,7 @@ def test_product_many_groups():
     import flashrt_amd as F
     sizes = [(i * 7) % 3 for i in range(1500)]
     bounds = cut(sizes)
-    for N in (8, 200):
+    for N in (8, 300):
         ops = operands(bounds[-1], 1500, N, 96, N)
         check_product(run_product(F, ops, bounds[-1], torch.float32, bounds), ops, bounds[-1], torch.float32, bounds)
 
@@ -307,7 +311,7 @@ def test_product_many_groups():
 def test_product_tiles_captured():
     """The tile kernels in a graph, replayed on other activations and bounds with eager work between, each replay equal to the eager call."""
     import flashrt_amd as F
-    E, N, C, M = 64, 512, 512, 1500
+    E, N, C, M = 128, 512, 512, 3000   # (two tiles of 16 rows to a group: 34 MB)
     ops = operands(M, E, N, C, 3)
     aq, asc, wq, wsc = (torch.from_numpy(v).cuda() for v in ops)
     bounds = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
