@@ -229,6 +229,9 @@ int moe_sort(const int32_t* ids, int T, int K, int E, int32_t* bounds, int32_t* 
 
 // ---------------------------------------------------------------- the moves
 // A wave takes 64 pieces of 16 bytes of one token's row (a workgroup four such parts, of consecutive tokens where a row has fewer).
+// All four are bound by HBM: 8192 tokens of 2560 bf16 values and their 81920 sorted rows 92 us to permute (5.0 TB/s; a large copy
+// reaches 4.8 to 5.1), 91 us to sum, 179 us for the weighted sum's gradient (4.9); short calls by one trip to memory and the
+// launch (one token of ten slots 2.8 to 3.8 us).
 
 // The token's piece is read once and written to each of its rows.
 template <typename T>

@@ -113,6 +113,26 @@ def test_reference_rounds_to_even_codes():
     assert values(codes, scales)[0, :16].tolist() == [4, 0, 1, 1, 2, 2, 4, 4, 6, 6, 6, -0.0, -4, 0.5, 0.5, -0.0]
 
 
+def _client(arg):
+    import os
+    import subprocess
+    exe = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "_build", "test_ops")
+    assert os.path.exists(exe), "build first: make -C flashrt_amd/csrc"
+    r = subprocess.run([exe, arg], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and "all passed" in r.stdout, r.stdout + r.stderr
+
+
+def test_cpp_client_host():
+    """The C++ mirror's calls turn refusals into std::runtime_error."""
+    _client("--host")
+
+
+@pytest.mark.gpu
+def test_cpp_client_gpu():
+    """The C++ mirror's calls in a run: sort, permute, quantize, product, unpermute and the gradients, exact values."""
+    _client("--gpu")
+
+
 # ---------------------------------------------------------------- quantisation
 
 @pytest.mark.gpu
