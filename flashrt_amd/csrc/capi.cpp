@@ -694,7 +694,7 @@ int frt_mx4_dequantize(void* stream, const void* codes, const void* scales, int 
 int frt_mx4_product(void* stream, const void* aq, const void* asc, int a_rows, const int32_t* rows, const void* wq,
                     const void* wsc, const int32_t* bounds, int E, int M, int N, int C, void* out, int64_t ldout, int type) {
     if (int rc = type_check("mx4_product", type)) return rc;
-    if (M < 0 || N < 1 || N > (1 << 30) || C < 32 || C % 32 || C > (1 << 30))
+    if (M < 0 || M > (1 << 30) || N < 1 || N > (1 << 30) || C < 32 || C % 32 || C > (1 << 30))
         return set_error(kErrShape, "mx4_product: M=%d N=%d C=%d (a multiple of 32)", M, N, C);
     if (E < 1 || E > 4096 || (!bounds && E != 1)) return set_error(kErrShape, "mx4_product: E=%d%s", E, bounds ? "" : " without bounds");
     if (M == 0) return kOk;

@@ -214,6 +214,14 @@ __device__ __forceinline__ float half_max(float v) {
     const float b = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
     return (threadIdx.x & 32) ? b : a;
 }
+// A grid of fewer than 2^31 workgroups of up to 256 threads, in two dimensions where one would pass the launch's 2^32 threads; a few
+// workgroups may lie past the last one asked for.
+inline dim3 wide_grid(uint32_t wgs) {
+    const uint32_t y = uint32_t((uint64_t(wgs) + (1u << 23) - 1) >> 23);
+    return dim3((wgs + y - 1) / y, y);
+}
+__device__ __forceinline__ uint32_t wide_block() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
 // Inclusive sum over the lanes of a wave, by DPP
 __device__ __forceinline__ int wave_scan(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // one lane down within a row of 16, then two, four, eight

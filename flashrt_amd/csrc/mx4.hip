@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(256) k_mx4_rows(Mx4Args p, int ntile, FastDiv 
     __shared__ f4_t s_sum[4][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
     const int kw = wave % KW;
-    const uint32_t unit = blockIdx.x * FW + wave / KW, tile = ntiles(unit);
+    const uint32_t unit = wide_block() * FW + wave / KW, tile = ntiles(unit);
     const RowTile t = find_tile<16>(p.bounds, p.E, p.M, [&](int total) { return int(tile) < total ? int(tile) : -1; });
     const int f0 = int(unit - tile * ntile) * 16, nb = p.C / 32, ng = nb / 16;
     f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -757,7 +757,7 @@ static int tiles_go(const Mx4Args& p, int stages, int64_t fill, hipStream_t stre
     // (few rows to a group: only weights beyond the 256 MB of the last cache; 80 experts, 84 MB, read again and again 15.2 against 21.1 us)
     const int stream_w = BM > 32 || groups * p.N * (p.C / 2) > (int64_t(256) << 20);
     const int64_t wgs = (tiles + 7) / 8 * 8 * nchunk;
-    if (wgs > 0x7fffffff) return set_error(kErrShape, "mx4_product: M=%d N=%d E=%d", p.M, p.N, p.E);
+    if (wgs * (64 * WM * WN) > 0xffffffff) return set_error(kErrShape, "mx4_product: M=%d N=%d E=%d", p.M, p.N, p.E);   // (the launch's threads)
     constexpr int smem = TileShape<BM, BN, WM * WN, ST, SS>::smem;
     static_assert(smem <= 160 * 1024, "LDS of a CU");
     FRT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_mx4_tiles<T, BM, BN, WM, WN, ST, SS, PT, WORDS>),
@@ -779,8 +779,8 @@ template <typename T, int KW>
 static int rows_t(const Mx4Args& p, hipStream_t stream) {
     const int ntile = (p.N + 15) / 16;
     const int64_t units = tiles_at_most(p.M, p.E, 16, p.bounds != nullptr) * ntile, wgs = (units + 4 / KW - 1) / (4 / KW);
-    if (units > 0x7ffffff0) return set_error(kErrShape, "mx4_product: M=%d N=%d E=%d", p.M, p.N, p.E);
-    launch_timed("mx4_product", k_mx4_rows<T, KW>, dim3(uint32_t(wgs)), dim3(256), 0, stream, p, ntile, FastDiv(ntile));
+    if (units > 0x7ffff000) return set_error(kErrShape, "mx4_product: M=%d N=%d E=%d", p.M, p.N, p.E);
+    launch_timed("mx4_product", k_mx4_rows<T, KW>, wide_grid(uint32_t(wgs)), dim3(256), 0, stream, p, ntile, FastDiv(ntile));
     FRT_LAUNCHED("mx4_product");
     return kOk;
 }

@@ -238,7 +238,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) k_permute(const T* __restrict__ x, int64_t ldx, int n_tok, int K, int n, uint32_t parts, FastDiv div,
                                                  const int32_t* __restrict__ row_of, T* __restrict__ xs, int64_t ldxs) {
     constexpr int V = 16 / sizeof(T);
-    const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t unit = wide_block() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t = int(div(unit)), c = int((unit - t * parts) * 64 + (threadIdx.x & 63)) * V;
     if (t >= n_tok || c >= n) return;
     const unsigned S = unsigned(n_tok) * K;
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(256) k_sum_rows(const T* __restrict__ ys, int6
                                                   const int32_t* __restrict__ row_of, const float* __restrict__ wts,
                                                   T* __restrict__ y, int64_t ldy) {
     constexpr int V = 16 / sizeof(T);
-    const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t unit = wide_block() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t = int(div(unit)), c = int((unit - t * parts) * 64 + (threadIdx.x & 63)) * V;
     if (t >= n_tok || c >= n) return;
     const unsigned S = unsigned(n_tok) * K;
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(256) k_unpermute_grad(const T* __restrict__ dy
                                                         const float* __restrict__ wts, T* __restrict__ dys, int64_t lddys,
                                                         float* __restrict__ dwts) {
     constexpr int V = 16 / sizeof(T);
-    const uint32_t s = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t s = wide_block() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     const unsigned S = unsigned(n_tok) * K;
     if (s >= S) return;
@@ -335,8 +335,8 @@ template <typename T>
 static uint32_t row_parts(int n) { return (uint32_t(n) + 1024 / sizeof(T) - 1) / (1024 / sizeof(T)); }
 // workgroups of four waves; false where the units would not fit 31 bits (rows of 2^31 KiB in all)
 static bool grid_of(int64_t units, dim3* g) {
-    if (units > 0x7ffffff0) return false;
-    *g = dim3(uint32_t((units + 3) / 4));
+    if (units > 0x7fffffff) return false;
+    *g = wide_grid(uint32_t((units + 3) / 4));
     return true;
 }
 

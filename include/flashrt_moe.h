@@ -149,10 +149,9 @@ int frt_moe_dispatch(void* stream, const int32_t* ids, int T, int K, int E, int3
  * frt_moe_sort: a stable sort of the slots by expert, as frt_moe_dispatch's, with the inverse map, in one launch without a
  * workspace: bounds [E+1]; slot_of and tok_of (= slot_of / K) [S], of which the first bounds[E] are written; row_of [S], the
  * slot's row or -1.
- * The moves take rows of type FRT_GGML_F32, FRT_GGML_F16 or FRT_GGML_BF16, any n from 1 to
- * 2^30, at ld* elements from one row to the
- * next (ld* >= n), and row_of as frt_moe_sort wrote it (an entry outside [0, S) is a dropped slot's). Sums are fp32, ascending
- * k, rounded once. Inputs and outputs must not overlap.
+ * The moves take rows of type FRT_GGML_F32, FRT_GGML_F16 or FRT_GGML_BF16, any n from 1 to 2^30, at ld* elements from one row
+ * to the next (ld* >= n), and row_of as frt_moe_sort wrote it (an entry outside [0, S) is a dropped slot's). Sums are fp32,
+ * ascending k, rounded once. Inputs and outputs must not overlap.
  *   permute         xs[row_of[s]] = x[s / K]; other rows of xs stay as they were
  *   permute_grad    dx[t] = sum over the token's rows of dxs[row_of[t K + k]]
  *   unpermute       y[t] = sum_k wts[t K + k] ys[row_of[t K + k]], wts fp32; 0 for a token without rows
@@ -183,9 +182,10 @@ int frt_mx4_dequantize(void* stream, const void* codes, const void* scales, int 
 /* ---- grouped product of 4-bit operands, the sorted experts' products: out[r][j] = sum_k a(r)[k] w_g[j][k] for r in
  * [bounds[g], bounds[g+1]), g < E <= 4096, j < N, k < C (a multiple of 32). a(r) is row r of the activations
  * (aq [a_rows][C/2], asc [a_rows][C/32]), or row rows[r] where rows is given (frt_moe_sort's tok_of: the tokens quantized
- * once); an index outside [0, a_rows) reads as a row of zeros. Weights wq [E][N][C/2], wsc [E][N][C/32]. bounds NULL: one
+ * once); an index outside [0, a_rows) gives a row of zeros. Weights wq [E][N][C/2], wsc [E][N][C/32]. bounds NULL: one
  * group (E = 1) of M rows. Bounds ascend within [0, M]; rows of no group stay as they were. aq and wq 16-byte aligned; a_rows >= M, or >= 1
- * with rows. out of type FRT_GGML_F32 / F16 / BF16, rows ldout >= N elements apart; sums in fp32, rounded once. M >= 0; N and C up to 2^30. */
+ * with rows. out of type FRT_GGML_F32 / F16 / BF16, rows ldout >= N elements apart; sums in fp32, rounded once. M (may be 0), N and C up to
+ * 2^30. */
 int frt_mx4_product(void* stream, const void* aq, const void* asc, int a_rows, const int32_t* rows, const void* wq,
                     const void* wsc, const int32_t* bounds, int E, int M, int N, int C, void* out, int64_t ldout, int type);
 

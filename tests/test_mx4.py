@@ -86,6 +86,13 @@ def test_refusals_before_any_launch():
         assert fn(*a) == 0   # no rows: nothing to do
 
 
+def test_product_refuses_more_rows_than_it_numbers():
+    from flashrt_amd import _lib
+    L, p = _lib.lib(), 1 << 20
+    assert L.frt_mx4_product(None, p, p, 5, p, p, p, p, 4, (1 << 30) + 1, 24, 64, p, 24, 0) == -1
+    assert L.frt_mx4_product(None, p, p, 0x7fffffff, None, p, p, None, 1, 0x7fffffff, 24, 64, p, 24, 0) == -1
+
+
 def test_python_refusals():
     import flashrt_amd as F
     u8 = lambda *s: torch.zeros(s, dtype=torch.uint8)  # noqa: E731
@@ -415,6 +422,25 @@ def test_weights_past_32_bits(M):
     out = torch.empty(M, N, device="cuda")
     F.mx4_product(aq, asc, wq, wsc, out, bounds=bounds)
     check_product(out, ops, M, torch.float32, [0, 4, M])
+
+
+@pytest.mark.gpu
+def test_results_past_32_bits():
+    """2^20 rows of the same few activations against 8200 features, 8.6 G results: more workgroups than one grid dimension holds, and
+    offsets past 32 bits. The columns' extremes over the rows with activations are the one row's results; the others are 0."""
+    import flashrt_amd as F
+    M, N, C = 2 ** 20, 8200, 32
+    ops = operands(1, 1, N, C, 11)
+    aq, asc, wq, wsc = (torch.from_numpy(v).cuda() for v in ops)
+    rows = torch.where(torch.arange(M, device="cuda") % 5 == 2, -1, 0).to(torch.int32)
+    one, out = torch.empty(1, N, device="cuda"), torch.empty(M, N, dtype=torch.bfloat16, device="cuda")
+    F.mx4_product(aq, asc, wq, wsc, one)
+    check_product(one, ops, 1, torch.float32)
+    F.mx4_product(aq, asc, wq, wsc, out, rows=rows)
+    want, step = one.to(torch.bfloat16), 2 ** 16
+    for r in range(0, M, step):
+        none = (rows[r:r + step] < 0)[:, None]
+        assert torch.equal(out[r:r + step], torch.where(none, torch.zeros_like(want), want)), r
 
 
 @pytest.mark.gpu

@@ -397,3 +397,24 @@ def test_other_stream_and_graph():
         torch.cuda.synchronize()
         for k in buf:
             assert torch.equal(buf[k], want[k]), (seed, k)
+
+
+@pytest.mark.gpu
+def test_more_tokens_than_one_grid_dimension():
+    """2^26 + 37 tokens of two values, one slot each: more waves than 2^32 threads in one dimension hold. Powers of two and small
+    integers, so every result is exact."""
+    import flashrt_amd as F
+    T = 2 ** 26 + 37
+    x = ((torch.arange(2 * T, device="cuda", dtype=torch.int32) * 7) % 1021).to(torch.float16).reshape(T, 2)
+    row = torch.arange(T - 1, -1, -1, dtype=torch.int32, device="cuda")
+    w = torch.where(torch.arange(T, device="cuda") % 3 == 0, 2.0, 0.5)
+    xs, y, dw = torch.zeros_like(x), torch.zeros_like(x), torch.zeros(T, device="cuda")
+    F.moe_permute(x, T, 1, row, xs)
+    assert torch.equal(xs, x.flip(0))
+    F.moe_permute_grad(xs, T, 1, row, y)
+    assert torch.equal(y, x)
+    F.moe_unpermute(xs, T, 1, row, w, y)
+    assert torch.equal(y, (x * w[:, None]).half())
+    F.moe_unpermute_grad(x, xs, T, 1, row, w, y, dw)
+    assert torch.equal(y, (x * w[:, None]).half().flip(0))
+    assert torch.equal(dw, x[:, 0].float() ** 2 + x[:, 1].float() ** 2)   # (integers below 2^24)
