@@ -17,7 +17,6 @@ namespace frt {
 typedef uint32_t u4e4_t __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u4e2_t __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u4e1_t __attribute__((ext_vector_type(4), aligned(1)));
-typedef uint32_t u2e1_t __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t u2e2_t __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
@@ -345,8 +344,9 @@ constexpr uint32_t kNoStore = 0x80000000u;
 // BM rows x BN features per tile, `per` feature tiles of one row tile after one another in a workgroup of WM x WN waves, from
 // LDS. A stage is KB blocks of 32 values of every operand row, in a ring of ST slots, their codes loaded straight into it; block c of
 // row r sits at c ^ (r / 2 % 8), so that the sixteen rows of a read phase take sixteen different columns of the banks.
-// The scales of SS stages at a time (side by side in a row: the loads' cost is lines, not bytes) go the same way where the rows of
-// scales are words (WORDS: a multiple of 128 values), else a stage's through registers. In step t (0..3) lane half h
+// The scales go the same way, 2 SS words of each row at a time (side by side: the loads' cost is lines, not bytes): those of SS stages
+// where the rows of scales are words (WORDS: a multiple of 128 values), else the aligned words around those of SS - 1 stages, of
+// which a lane takes its bytes by a shift (a row's first and last word may reach three bytes past the row). In step t (0..3) lane half h
 // multiplies block 4 h + t of its rows, so that a lane's four scales of a stage are one word and the step picks its byte. Step t +
 // 1's operands are read before step t's products, the next stage's first ones before the last step's, past the barrier. The
 // stages of the feature tiles form one sequence: the next tile's first stages load while this one's results are written.
@@ -359,10 +359,11 @@ constexpr uint32_t kNoStore = 0x80000000u;
 // in each workgroup.
 template <typename T, int BM, int BN, int WM, int WN, int ST, int SS, int PT, bool WORDS>
 __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile, int per, FastDiv chunks, uint32_t nchunk, int stream) {
-    constexpr int NW = WM * WN, NT = 64 * NW;
+    constexpr int NW = WM * WN;
     using Sh = TileShape<BM, BN, NW, ST, SS>;
-    static_assert(SS >= 2 && (ST == 2 || ST == 3) && PT <= 3, "scales a group ahead; the waits; the steps before a stage's end");
-    constexpr int FM = BM / WM / 32, FN = BN / WN / 32, DA = Sh::da, DW = Sh::dw, D = DA + DW, SR = (Sh::rows + NT - 1) / NT;
+    static_assert(SS >= 2 && (ST == 2 || ST == 3) && PT <= 3, "whole words of scales; the waits; the steps before a stage's end");
+    constexpr int GS = WORDS ? SS : SS - 1;   // the stages of a group of scales
+    constexpr int FM = BM / WM / 32, FN = BN / WN / 32, DA = Sh::da, DW = Sh::dw, D = DA + DW;
     extern __shared__ __align__(16) uint8_t smem[];
     uint8_t* const s_scale = smem + ST * Sh::code_b;
     int32_t* const s_row = reinterpret_cast<int32_t*>(s_scale + 2 * Sh::scale_b);   // [BM]: the activations' row, -1: none
@@ -456,77 +457,44 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
             if (parts) issue_part(kc);
         }
     };
-    // scales (WORDS): the next group is that of stages sq SS .. of feature tile sf, into buffer sbuf
+    // scales: the next group is that of stages sq GS .. of feature tile sf, into buffer sbuf
     constexpr int LR = KB * SS / 4;   // lanes (words) of a row's group
-    constexpr int NA = WORDS ? Sh::sa : 0, NS = WORDS ? Sh::sa + Sh::sw : SR;   // the first NA are the activations'
+    constexpr int NA = Sh::sa, NS = Sh::sa + Sh::sw;   // the first NA are the activations'
     const uint8_t* ssrc[NS];
-    const uint8_t* slast[SR];    // (the last KB bytes of the tensor)
     int sf = ft, sq = 0, sbuf = 0;
     const int sw0 = wave * Sh::sa % (BM / Sh::sr > 0 ? BM / Sh::sr : 1);   // the wave's first load of the activations'
-    if constexpr (WORDS) {
 #pragma unroll
-        for (int k = 0; k < NA; ++k) ssrc[k] = p.as + int64_t(max(s_row[(sw0 + k) * Sh::sr + lane / LR], 0)) * nb;
-    } else {
-#pragma unroll
-        for (int k = 0; k < SR; ++k) {
-            const bool act = tid + NT * k < BM;
-            ssrc[k] = p.as + int64_t(max(s_row[act ? tid + NT * k : 0], 0)) * nb;
-            slast[k] = (act ? p.as + int64_t(p.a_rows) * nb : p.ws + int64_t(p.E) * p.N * nb) - KB;
-        }
-    }
+    for (int k = 0; k < NA; ++k) ssrc[k] = p.as + int64_t(max(s_row[(sw0 + k) * Sh::sr + lane / LR], 0)) * nb;
     auto spoint = [&]() {
 #pragma unroll
-        for (int k = NA; k < NS; ++k) {
-            const int r = WORDS ? (wave * Sh::sw + k - NA) * Sh::sr + lane / LR : min(tid + NT * k, Sh::rows - 1) - BM;
-            if (WORDS || r >= 0) ssrc[k] = ws + wgt_row(sf, r);
-        }
+        for (int k = NA; k < NS; ++k) ssrc[k] = ws + wgt_row(sf, (wave * Sh::sw + k - NA) * Sh::sr + lane / LR);
     };
+    auto byte_of = [](const uint8_t* q) { return WORDS ? 0 : int(reinterpret_cast<uintptr_t>(q) & 3); };   // in its word
     auto issue_scales = [&]() {
         if (sf >= ft1) return;
-        const int w = min(LR * sq + lane % LR, nb / 4 - 1) * 4;
         uint8_t* const s = s_scale + sbuf * Sh::scale_b;
-        if constexpr (WORDS) {
 #pragma unroll
-            for (int k = 0; k < NA; ++k) ldsdma4(ssrc[k] + w, s + (sw0 + k) * 256);
-#pragma unroll
-            for (int k = NA; k < NS; ++k) ldsdma4(ssrc[k] + w, s + BM * SS * KB + (wave * Sh::sw + k - NA) * 256);
+        for (int k = 0; k < NS; ++k) {   // (words past the row's end read as its last)
+            const int off = byte_of(ssrc[k]), w = min(2 * GS * sq + lane % LR, (off + nb - 1) / 4) * 4 - off;
+            ldsdma4(ssrc[k] + w, s + (k < NA ? (sw0 + k) * 256 : BM * SS * KB + (wave * Sh::sw + k - NA) * 256));
         }
         sbuf ^= 1;
-        if (++sq * SS >= nst) {
+        if (++sq * GS >= nst) {
             sq = 0;
             ++sf;
             spoint();
         }
     };
-    // Without WORDS: the KB scales of stage st of row tid (and those NT on), at any alignment; past the row's end they are the next
-    // row's (their steps are masked). At the tensor's end its last KB bytes are loaded and shifted down.
-    u2e1_t sv[SR];
-    auto load_scales = [&](int st) {
+    // The first byte of the lane's rows' scales (the weights' rows are a multiple of 32 apart, over the feature tiles too; of a row past
+    // the last feature the bytes are another's, and not used)
+    int a_off[FM];
 #pragma unroll
-        for (int k = 0; k < SR; ++k) {
-            const uint8_t* const at = ssrc[k] + KB * st;
-            sv[k] = *reinterpret_cast<const u2e1_t*>(at < slast[k] ? at : slast[k]);
-        }
-    };
-    auto put_scales = [&](int st, int buf) {
-#pragma unroll
-        for (int k = 0; k < SR; ++k) {
-            const int64_t over = ssrc[k] + KB * st - slast[k];
-            uint64_t w = uint64_t(sv[k][1]) << 32 | sv[k][0];
-            if (over > 0) w >>= 8 * int(over < KB - 1 ? over : KB - 1);
-            if (tid + NT * k < Sh::rows)
-                *reinterpret_cast<uint64_t*>(s_scale + buf * Sh::scale_b + ((tid + NT * k) * SS + st % SS) * KB) = w;
-        }
-    };
+    for (int m = 0; m < FM; ++m) a_off[m] = byte_of(p.as + int64_t(max(s_row[am + 32 * m], 0)) * nb);
+    const int w_off = byte_of(ws + int64_t(wf - BM) * nb);
     point();
     spoint();
-    if constexpr (WORDS) {
-        issue_scales();
-        issue_scales();
-    } else {
-        load_scales(0);
-        put_scales(0, 0);
-    }
+    issue_scales();
+    issue_scales();
 #pragma unroll
     for (int s = 0; s < ST; ++s) issue();
 
@@ -547,12 +515,16 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
         int a[FM], b[FN];
     };
     auto read_scales = [&](int st, int buf) {
-        const uint8_t* const s = s_scale + buf * Sh::scale_b + (st % SS) * KB + h * 4;
+        const uint8_t* const s = s_scale + buf * Sh::scale_b + (st % GS) * KB + h * 4;
+        auto four = [&](int row, int off) {
+            const int* const w = reinterpret_cast<const int*>(s + row * KB * SS);
+            return WORDS ? w[0] : int(__builtin_amdgcn_alignbyte(w[1], w[0], off));
+        };
         Scales o;
 #pragma unroll
-        for (int m = 0; m < FM; ++m) o.a[m] = *reinterpret_cast<const int*>(s + (am + 32 * m) * KB * SS);
+        for (int m = 0; m < FM; ++m) o.a[m] = four(am + 32 * m, a_off[m]);
 #pragma unroll
-        for (int f = 0; f < FN; ++f) o.b[f] = *reinterpret_cast<const int*>(s + (wf + 32 * f) * KB * SS);
+        for (int f = 0; f < FN; ++f) o.b[f] = four(wf + 32 * f, w_off);
         return o;
     };
     f16_t acc[FM][FN];
@@ -593,22 +565,11 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
             for (int f = 0; f < FN; ++f)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[m][f][i] = 0.0f;
-        // before stage st's products: the scales of the stage after it, through registers
-        auto ahead = [&](int st) {
-            if constexpr (!WORDS) {
-                if (st + 1 == nst) {
-                    ++sf;
-                    spoint();   // (past the last feature tile: rows inside the tensor still)
-                }
-                load_scales(st + 1 == nst ? 0 : st + 1);
-            }
-        };
         // the end of stage st: the next stage has landed, all waves have read this one; its slot and, past a group, its scales' buffer
         // are loaded anew (the slot of a tile's last stage after its results were written through it)
         auto finish = [&](int st) {
-            const bool last = st + 1 == nst, turn = last || (st + 1) % SS == 0;
+            const bool last = st + 1 == nst, turn = last || (st + 1) % GS == 0;
             const int nbuf = turn ? buf ^ 1 : buf;
-            if constexpr (!WORDS) put_scales(last ? 0 : st + 1, nbuf);
             if (under == ST - 1) {
                 if (st < ST - 2 && ft > ft0)
                     wait_vm<(kAfter < 63 ? kAfter : 63)>();
@@ -619,7 +580,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
             }
             if (jf >= ft1) --under;
             ring_barrier();
-            if (WORDS && turn) issue_scales();
+            if (turn) issue_scales();
             parts = PT > 1 && !last;
             if (parts)
                 issue_part(std::integral_constant<int, 0>());
@@ -629,7 +590,6 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
             slot = slot == ST - 1 ? 0 : slot + 1;
         };
         for (int st = 0; st < nfull; ++st) {
-            ahead(st);
             Ops o1 = read(slot, 1);
             issue_more(std::integral_constant<int, 1>());
             __builtin_amdgcn_sched_barrier(0);
@@ -655,11 +615,10 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
         }
         if (nfull < nst) {
             // the last, shorter stage: blocks 2 i and 2 i + 1 in step i; a block past the row's end is zeros at scale one
-            ahead(nfull);
             issue_more(std::integral_constant<int, 1>());
             issue_more(std::integral_constant<int, 2>());
             const uint8_t* const s = smem + slot * Sh::code_b;
-            const uint8_t* const ssc = s_scale + buf * Sh::scale_b + (nfull % SS) * KB;
+            const uint8_t* const ssc = s_scale + buf * Sh::scale_b + (nfull % GS) * KB;
             const int left = nb - KB * nfull;
             const i4_t zero = {0, 0, 0, 0};
             for (int c = h; c - h < left; c += 2) {
@@ -670,14 +629,14 @@ __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile
 #pragma unroll
                 for (int f = 0; f < FN; ++f) {
                     b[f] = *reinterpret_cast<const i4_t*>(s + (wf + 32 * f) * KB * 16 + at);
-                    bs[f] = ssc[(wf + 32 * f) * KB * SS + c];
+                    bs[f] = ssc[(wf + 32 * f) * KB * SS + w_off + c];
                     b[f] = in ? b[f] : zero;
                     bs[f] = in ? bs[f] : 127;
                 }
 #pragma unroll
                 for (int m = 0; m < FM; ++m) {
                     i4_t a = *reinterpret_cast<const i4_t*>(s + (am + 32 * m) * KB * 16 + at);
-                    int as = ssc[(am + 32 * m) * KB * SS + c];
+                    int as = ssc[(am + 32 * m) * KB * SS + a_off[m] + c];
                     a = in ? a : zero;
                     as = in ? as : 127;
 #pragma unroll
@@ -770,9 +729,9 @@ static int tiles_go(const Mx4Args& p, int stages, int64_t fill, hipStream_t stre
 template <typename T, int BM, int BN, int WM, int WN, int ST, int SS, int PT>
 static int tiles_t(const Mx4Args& p, int stages, int64_t fill, hipStream_t stream) {
     const bool words = p.C % 128 == 0 && reinterpret_cast<uintptr_t>(p.as) % 4 == 0 && reinterpret_cast<uintptr_t>(p.ws) % 4 == 0;
-    if (words) return tiles_go<T, BM, BN, WM, WN, ST, SS, PT, true>(p, stages, fill, stream);
-    // (the scales' way through registers waits for all loads: a third slot only takes LDS; 20480 rows, N 1000, C 1056 127 -> 119 us)
-    return tiles_go<T, BM, BN, WM, WN, 2, SS, PT, false>(p, stages, fill, stream);
+    // (20480 rows, N 1000, C 1056: 112 us; through registers, which wait for all loads, 119)
+    return words ? tiles_go<T, BM, BN, WM, WN, ST, SS, PT, true>(p, stages, fill, stream)
+                 : tiles_go<T, BM, BN, WM, WN, ST, SS, PT, false>(p, stages, fill, stream);
 }
 
 template <typename T, int KW>
@@ -798,9 +757,8 @@ static int product_t(const Mx4Args& p, hipStream_t stream) {
     const int64_t groups = p.bounds ? std::min(p.E, p.M) : 1, avg = p.M / groups;
     auto rows = [&](int64_t BM) { return (avg + BM - 1) / BM * groups; };   // tiles of BM rows
     auto tiles = [&](int64_t BM, int64_t BN) { return rows(BM) * ((p.N + BN - 1) / BN); };
-    const int nb = p.C / 32;   // (the tile kernels load 8 scales at a time, and store through 31-bit offsets)
-    if (rows(16) * p.N * (p.C / 2) > (int64_t(16) << 20) && int64_t(p.a_rows) * nb >= 8 && int64_t(p.E) * p.N * nb >= 8 &&
-        int64_t(256) * p.ldout * int64_t(sizeof(T)) < 0x7fffffff) {
+    const int nb = p.C / 32;   // (the tile kernels store through 31-bit offsets)
+    if (rows(16) * p.N * (p.C / 2) > (int64_t(16) << 20) && int64_t(256) * p.ldout * int64_t(sizeof(T)) < 0x7fffffff) {
         if (avg >= 256 && tiles(256, 256) >= 128) return tiles_t<T, 256, 256, 4, 2, 2, 2, 3>(p, 64, 256, stream);
         if (avg > 56 && tiles(128, 128) >= 256) return tiles_t<T, 128, 128, 2, 2, 2, 2, 1>(p, 32, 1536, stream);
         if (avg > 8 && tiles(64, 128) >= 160) return tiles_t<T, 64, 128, 2, 2, 3, 2, 1>(p, 16, 512, stream);

@@ -185,7 +185,7 @@ int frt_mx4_dequantize(void* stream, const void* codes, const void* scales, int 
  * once); an index outside [0, a_rows) gives a row of zeros. Weights wq [E][N][C/2], wsc [E][N][C/32]. bounds NULL: one
  * group (E = 1) of M rows. Bounds ascend within [0, M]; rows of no group stay as they were. aq and wq 16-byte aligned; a_rows >= M, or >= 1
  * with rows. out of type FRT_GGML_F32 / F16 / BF16, rows ldout >= N elements apart; sums in fp32, rounded once. M (may be 0), N and C up to
- * 2^30. */
+ * 2^30. The scales are read in whole aligned words: up to three bytes beside asc and wsc are read, and not used. */
 int frt_mx4_product(void* stream, const void* aq, const void* asc, int a_rows, const int32_t* rows, const void* wq,
                     const void* wsc, const int32_t* bounds, int E, int M, int N, int C, void* out, int64_t ldout, int type);
 

@@ -324,6 +324,35 @@ def test_product_tiles(tile, C, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shift", [1, 2, 3])
+@pytest.mark.parametrize("tile", list(TILES))
+def test_product_scales_at_any_byte(tile, shift):
+    """Every tile size with 17 scales to a row that start at every byte of a word, bytes of NaN scales beside both tensors; activations
+    picked by index."""
+    import flashrt_amd as F
+    sizes, N = TILES[tile]
+    C = 544
+    if len(sizes) > 1:
+        avg = sum(sizes) // len(sizes)
+        sizes = sizes * max(1, -(-(17 << 20) // (-(-avg // 16) * len(sizes) * N * C // 2)))
+    bounds = cut(sizes)
+    M = bounds[-1]
+    ops = operands(301, len(sizes), N, C, shift)
+    aq, asc, wq, wsc = (torch.from_numpy(v).cuda() for v in ops)
+
+    def moved(v, by):
+        buf = torch.full((v.numel() + 8,), 255, dtype=torch.uint8, device="cuda")
+        buf[by:by + v.numel()] = v.reshape(-1)
+        return buf[by:by + v.numel()].view(v.shape)
+
+    rows = np.random.default_rng(shift).integers(0, 301, M).astype(np.int32)
+    out = torch.empty(M, N, device="cuda")
+    F.mx4_product(aq, moved(asc, shift), wq, moved(wsc, 4 - shift), out, bounds=torch.tensor(bounds, dtype=torch.int32, device="cuda"),
+                  rows=torch.from_numpy(rows).cuda())
+    check_product(out, ops, M, torch.float32, bounds, rows)
+
+
+@pytest.mark.gpu
 def test_product_many_groups():
     """More than 512 groups (their bounds are read in blocks): 1500, most of one row or none, over tiles and over few features."""
     import flashrt_amd as F
@@ -426,8 +455,8 @@ def test_weights_past_32_bits(M):
 
 @pytest.mark.gpu
 def test_results_past_32_bits():
-    """2^20 rows of the same few activations against 8200 features, 8.6 G results: more workgroups than one grid dimension holds, and
-    offsets past 32 bits. The columns' extremes over the rows with activations are the one row's results; the others are 0."""
+    """2^20 rows of the same few activations against 8200 features, 8.6 G results: offsets
+    past 32 bits. The columns' extremes over the rows with activations are the one row's results; the others are 0."""
     import flashrt_amd as F
     M, N, C = 2 ** 20, 8200, 32
     ops = operands(1, 1, N, C, 11)
@@ -441,6 +470,29 @@ def test_results_past_32_bits():
     for r in range(0, M, step):
         none = (rows[r:r + step] < 0)[:, None]
         assert torch.equal(out[r:r + step], torch.where(none, torch.zeros_like(want), want)), r
+
+
+@pytest.mark.gpu
+def test_rows_past_31_bits_apart():
+    """Results too far apart for the tiles' offsets (rows of 2^22 half-precision features), so that the kernel of few rows takes 33 row
+    tiles: more workgroups than one grid dimension holds. Small codes at scale one: every sum is exact in fp32, whatever its order."""
+    import flashrt_amd as F
+    M, N, C, n = 528, 2 ** 22, 2048, 300
+    g = torch.Generator(device="cuda").manual_seed(3)
+    wq = torch.empty((N, C // 2), dtype=torch.uint8, device="cuda")   # 0 to 1.5 in halves, and every other value 0: sums below 2^12
+    for f in range(0, N, N // 16):
+        wq[f:f + N // 16] = torch.randint(0, 4, (N // 16, C // 2), generator=g, device="cuda", dtype=torch.uint8)
+    aq = torch.randint(0, 4, (3, C // 2), generator=g, device="cuda", dtype=torch.uint8)
+    wsc, asc = (torch.full((r, C // 32), 127, dtype=torch.uint8, device="cuda") for r in (N, 3))
+    rows = (torch.arange(M, device="cuda") * 7 % 4 - 1).to(torch.int32)
+    out = torch.empty(M, N, dtype=torch.float16, device="cuda")
+    F.mx4_product(aq, asc, wq, wsc, out, rows=rows)
+    few = torch.zeros(4, N, dtype=torch.float16, device="cuda")   # row 0: none
+    F.mx4_product(aq, asc, wq, wsc, few[1:])
+    assert torch.equal(out, few[rows.long() + 1])
+    for f in (0, N // 2, N - n):
+        a, w = values(aq.cpu().numpy(), asc.cpu().numpy()), values(wq[f:f + n].cpu().numpy(), wsc[f:f + n].cpu().numpy())
+        assert torch.equal(few[1:, f:f + n].cpu().double(), torch.from_numpy(a @ w.T).half().double())
 
 
 @pytest.mark.gpu
