@@ -85,57 +85,59 @@ __global__ void __launch_bounds__(1024) k_sort_few(const int32_t* __restrict__ i
     }
 }
 
-// One launch, no workspace: every workgroup counts all ids itself (those before its own slots, then all of them) in an LDS
-// histogram of 16 copies, one per lane of 16, so that a popular expert's atomics do not queue up behind each other; the scan of
+// One launch, no workspace: every workgroup counts all ids itself, in two LDS histograms (the slots before its own, and the
+// others) of 16 copies, one per lane of 16, so that a popular expert's atomics do not queue up behind each other; the scan of
 // the totals over the experts gives the groups' first rows, and the workgroup ranks its own slots in batches of 1024, a wave of
 // 64 at a time by ballots over the id bits (stable). Integer counts: the result does not depend on the atomics' order. The
-// counting reads 16 ids per thread at once (81920 slots 22.4 us one by one, 15.6 so); one launch instead of the dispatch's four costs
-// each workgroup the whole list, 328 KB from L2 at 81920 slots. ONE: a single batch, whose ranking counts it.
+// counting reads 16 ids per thread at once and spends three instructions on an id: ids outside are counted in a bin of their own,
+// and the histogram is the wave's choice (81920 slots of 512 experts 11.8 us; with two passes and a branch per id 13.7, reading
+// one by one 22.4; many more slots are bound by the LDS atomics, about 8 clocks per 64 ids). One launch instead of the dispatch's four costs each workgroup the whole list, 328 KB from L2 at 81920
+// slots. ONE: a single batch, whose ranking counts it.
 template <bool ONE>
 __global__ void __launch_bounds__(1024) k_sort(const int32_t* __restrict__ ids, int S, int K, int E, int id_bits, int batches,
                                                int32_t* __restrict__ bounds, int32_t* __restrict__ tok_of,
                                                int32_t* __restrict__ slot_of, int32_t* __restrict__ row_of) {
-    extern __shared__ int32_t hist[];   // [E][16]
+    // [E + 1][16], the last for ids outside; twice unless ONE: of the slots before the workgroup's own, and of the others
+    extern __shared__ int32_t hist[];
     __shared__ int s_base[kSortE];      // the next row of each expert for this workgroup's slots
     __shared__ int s_wave[16];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int s0 = min(int64_t(S), int64_t(blockIdx.x) * batches * 1024), s1 = min(int64_t(S), int64_t(s0) + batches * 1024);
-    auto clear = [&]() {
-        for (int i = tid; i < E * kSortCopies; i += 1024) hist[i] = 0;
+    auto clear = [&](int n) {
+        for (int i = tid; i < n; i += 1024) hist[i] = 0;
         __syncthreads();
     };
-    auto add = [&](int e) {
-        if (unsigned(e) < unsigned(E)) atomicAdd(&hist[e * kSortCopies + (lane & 15)], 1);
-    };
-    auto sum = [&]() {   // of expert tid's copies
+    const int one = (E + 1) * kSortCopies;   // a histogram
+    auto sum = [&](const int32_t* h) {       // of expert tid's copies
         int n = 0;
         if (tid < E)
 #pragma unroll
-            for (int c = 0; c < kSortCopies; ++c) n += hist[tid * kSortCopies + ((c + tid) & 15)];
+            for (int c = 0; c < kSortCopies; ++c) n += h[tid * kSortCopies + ((c + tid) & 15)];
         return n;
     };
-    auto count = [&](int lo, int hi) {
-        int64_t s = lo;   // (past 2^31 after the last step of a list near that length)
-        for (; s + 16384 <= hi; s += 16384) {
+    auto count = [&]() {   // all ids
+        // a wave's ids are all before s0, a multiple of 1024, or none
+        auto add = [&](uint32_t e, int32_t* h) { atomicAdd(h + min(e, uint32_t(E)) * kSortCopies, 1); };
+        int32_t* const mine = hist + (lane & 15);
+        int64_t s = 0;   // (past 2^31 after the last step of a list near that length)
+        for (; s + 16384 <= S; s += 16384) {
             Raw4 v[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const Raw4*>(ids + s + (i * 1024 + tid) * 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i) {
+                int32_t* const h = mine + (s + (i * 1024 + wave * 64) * 4 < s0 ? 0 : one);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) add(int(v[i][k]));
+                for (int k = 0; k < 4; ++k) add(v[i][k], h);
+            }
         }
-        int v[16];
+        uint32_t v[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            v[i] = -1;
-            if (s + i * 1024 < hi && s + i * 1024 + tid < hi) v[i] = ids[s + i * 1024 + tid];
-        }
+        for (int i = 0; i < 16; ++i) v[i] = s + i * 1024 + tid < S ? ids[s + i * 1024 + tid] : -1;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            if (s + i * 1024 < hi) add(v[i]);
+            if (s + i * 1024 < S) add(v[i], mine + (s + i * 1024 < s0 ? 0 : one));
         __syncthreads();
-        return sum();
     };
     // the first row of expert tid's group, from its rows
     auto starts = [&](int total) {
@@ -150,14 +152,12 @@ __global__ void __launch_bounds__(1024) k_sort(const int32_t* __restrict__ ids, 
         }
         return first;
     };
-    clear();
+    clear(ONE ? one : 2 * one);
     if (!ONE) {
-        const int before = count(0, s0);
-        __syncthreads();
-        const int first = starts(count(s0, S));
+        count();
+        const int before = sum(hist), first = starts(before + sum(hist + one));
         if (tid < E) s_base[tid] = first + before;
-        __syncthreads();   // (the histogram was read)
-        clear();
+        clear(one);   // (read before the barrier in starts)
     }
     const uint64_t lt = (lane == 0) ? 0ull : (~0ull >> (64 - lane));
     for (int64_t b0 = s0; b0 < s1; b0 += 1024) {   // (uniform over the workgroup)
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(1024) k_sort(const int32_t* __restrict__ ids, 
         __syncthreads();
         int run = 0;
         if (ONE)
-            run = starts(sum());
+            run = starts(sum(hist));
         else if (tid < E)
             run = s_base[tid];
         if (tid < E) {   // each wave's first row of expert tid
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(1024) k_sort(const int32_t* __restrict__ ids, 
         }
         if (b0 + 1024 < s1) {
             __syncthreads();
-            clear();
+            clear(one);
         }
     }
 }
@@ -217,7 +217,7 @@ int moe_sort(const int32_t* ids, int T, int K, int E, int32_t* bounds, int32_t* 
     while ((1 << id_bits) < E) ++id_bits;
     const int nb = int((int64_t(S) + 1023) / 1024);
     const int batches = (nb + kSortGrid - 1) / kSortGrid;
-    const size_t lds = size_t(E) * kSortCopies * 4;
+    const size_t lds = size_t(E + 1) * kSortCopies * (nb == 1 ? 4 : 8);
     const auto kernel = nb == 1 ? k_sort<true> : k_sort<false>;
     if (lds + 8192 > 65536)
         FRT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
