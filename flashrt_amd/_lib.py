@@ -6,6 +6,7 @@ raises. Build it with `make -C flashrt_amd/csrc` (or __graft_entry__.build()).
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -14,7 +15,23 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "flashrt_moe.h")
 
 _vp, _i, _sz, _u64, _f, _i64 = C.c_void_p, C.c_int, C.c_size_t, C.c_uint64, C.c_float, C.c_int64
 
-# name -> (restype, argtypes)
+
+class _CInt(C.c_int):
+    """A C int argument. ctypes cuts an integer to its low 32 bits without a word (2^32 tokens would be none); here one
+    outside the type is an error (ctypes.ArgumentError), at c_int's own cost."""
+
+    @classmethod
+    def from_param(cls, v):
+        if type(v) is not int:
+            if isinstance(v, C._SimpleCData):
+                return C.c_int.from_param(v)
+            v = operator.index(v)
+        if -0x80000000 <= v <= 0x7fffffff:
+            return v
+        raise OverflowError(f"{v} is outside a C int")
+
+
+# name -> (restype, argtypes); an _i argument is taken as _CInt
 SIGNATURES = {
     "frt_last_error": (C.c_char_p, []),
     "frt_version": (C.c_char_p, []),
@@ -114,7 +131,7 @@ def lib():
         for name, (res, args) in SIGNATURES.items():
             fn = getattr(L, name)
             fn.restype = res
-            fn.argtypes = args
+            fn.argtypes = [_CInt if a is _i else a for a in args]
         _lib = L
     return _lib
 

@@ -148,7 +148,8 @@ def moe_dispatch(ids, T: int, K: int, E: int, bounds, tok_of, slot_of, stream=No
 
 
 # ---------------------------------------------------------------- rows in expert order and back; 4-bit floats
-# These check their tensors (ValueError): type, shape, layout, and that all lie on one GPU, which need not be the current one.
+# These check their tensors (ValueError): type, shape, layout, sizes that the library's ints hold, and that all lie on one GPU,
+# which need not be the current one.
 
 _ROW_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}   # ggml type ids
 
@@ -165,12 +166,15 @@ def _enqueue(fn, dev: int, stream, *args) -> None:
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return _enqueue(fn, dev, stream, *args)
-    if stream is None:
-        rc = fn(_raw_stream(dev), *args)
-    else:
-        if isinstance(stream, torch.cuda.Stream) and stream.device_index != dev:
-            raise ValueError(f"flashrt_amd: the tensors are on GPU {dev}, the stream on GPU {stream.device_index}")
-        rc = fn(_s(stream), *args)
+    try:
+        if stream is None:
+            rc = fn(_raw_stream(dev), *args)
+        else:
+            if isinstance(stream, torch.cuda.Stream) and stream.device_index != dev:
+                raise ValueError(f"flashrt_amd: the tensors are on GPU {dev}, the stream on GPU {stream.device_index}")
+            rc = fn(_s(stream), *args)
+    except C.ArgumentError as e:   # a count that the library's ints cannot hold
+        raise ValueError(f"flashrt_amd: {e}") from None
     if rc:
         check(rc)
 

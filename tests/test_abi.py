@@ -175,3 +175,39 @@ def test_cpp_mirror_host():
     assert os.path.exists(exe), "build first: make -C flashrt_amd/csrc"
     r = subprocess.run([exe, "--host"], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0 and "all passed" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("v", [1 << 31, 1 << 32, (1 << 32) + 2, -(1 << 31) - 1, -(1 << 40)])
+def test_counts_outside_a_c_int_are_refused(v):
+    """A count that a C int cannot hold is refused by every entry that takes one, not cut to its low 32 bits (2^32 tokens
+    would be none, and the call a success)."""
+    L = _lib.lib()
+    p = 1 << 20   # an address that is never read
+    calls = [(L.frt_moe_sort, [None, p, 0, 1, 4, p, p, p, p], (2, 3, 4)),
+             (L.frt_moe_permute, [None, p, 8, 0, 0, 1, 8, p, p, 8], (3, 4, 5, 6)),
+             (L.frt_moe_unpermute_grad, [None, p, 8, p, 8, 0, 0, 1, 8, p, p, p, 8, p], (5, 6, 7, 8)),
+             (L.frt_mx4_quantize, [None, p, 64, 0, 0, 64, p, p], (3, 4, 5)),
+             (L.frt_mx4_product, [None, p, p, 1, None, p, p, None, 1, 0, 8, 32, p, 8, 0], (3, 8, 9, 10, 11, 14)),
+             (L.frt_q2_mat_bytes, [512, 2048], (0, 1)),
+             (L.frt_moe_dispatch_workspace_bytes, [1, 1, 8], (0, 1, 2))]
+    for fn, good, ints in calls:
+        for i in ints:
+            a = list(good)
+            a[i] = v
+            with pytest.raises(C.ArgumentError):
+                fn(*a)
+
+
+def test_counts_of_other_integer_types():
+    """What a C int argument took before it still takes: Python and numpy integers, truth values and ctypes integers; no floats."""
+    np = pytest.importorskip("numpy")
+    L = _lib.lib()
+    want = L.frt_q2_mat_bytes(512, 2048)
+    for kind in (np.int32, np.int64, np.uint16, C.c_int):
+        assert L.frt_q2_mat_bytes(kind(512), kind(2048)) == want
+    assert L.frt_moe_dispatch_workspace_bytes(True, True, 8) == L.frt_moe_dispatch_workspace_bytes(1, 1, 8)
+    for bad in (512.0, "512", None):
+        with pytest.raises(C.ArgumentError):
+            L.frt_q2_mat_bytes(bad, 2048)
+    with pytest.raises(C.ArgumentError):
+        L.frt_q2_mat_bytes(np.int64(1 << 32), 2048)

@@ -418,3 +418,17 @@ def test_more_tokens_than_one_grid_dimension():
     F.moe_unpermute_grad(x, xs, T, 1, row, w, y, dw)
     assert torch.equal(y, (x * w[:, None]).half().flip(0))
     assert torch.equal(dw, x[:, 0].float() ** 2 + x[:, 1].float() ** 2)   # (integers below 2^24)
+
+
+def test_python_refuses_counts_past_the_librarys_ints(monkeypatch):
+    """2^32 tokens, which a C int would cut to none, are a ValueError before anything is launched (the tensors' own checks and
+    the device's are left out here: there is no memory for such rows)."""
+    from flashrt_amd import moe
+    monkeypatch.setattr(moe, "_raw_stream", lambda dev: 0)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    p = 1 << 20
+    for T in (2 ** 31, 2 ** 32):
+        with pytest.raises(ValueError, match="C int"):
+            moe._enqueue(moe.lib().frt_moe_permute, 0, None, p, 1, 1, T, 1, 1, p, p, 1)
+        with pytest.raises(ValueError, match="C int"):
+            moe._enqueue(moe.lib().frt_mx4_product, 0, None, p, p, 1, p, p, p, p, 1, T, 8, 32, p, 8, 0)
