@@ -149,7 +149,9 @@ def moe_dispatch(ids, T: int, K: int, E: int, bounds, tok_of, slot_of, stream=No
 
 # ---------------------------------------------------------------- rows in expert order and back; 4-bit floats
 # These check their tensors (ValueError): type, shape, layout, sizes that the library's ints hold, and that all lie on one GPU,
-# which need not be the current one.
+# which need not be the current one. None of them is recorded by autograd: with gradients enabled, a tensor that requires one is
+# refused, as torch refuses it for an out= argument. The *_grad calls are for the backward of a torch.autograd.Function (whose
+# forward and backward run with gradients disabled).
 
 _ROW_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}   # ggml type ids
 
@@ -187,10 +189,18 @@ def _type(t, what: str) -> int:
     return code
 
 
+def _untracked(t, what: str) -> None:
+    """Refuses a tensor whose gradient would silently be lost."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient, which this call does not record: detach it, disable gradients, or call from a torch.autograd.Function")
+
+
 def _rows(t, rows: int, cols: int, like, dev: int, what: str) -> int:
     """The distance between the rows of a [rows][cols] matrix of like's type on GPU dev, each row's values adjacent."""
     if t.dtype is not like.dtype or t.get_device() != dev:
         raise ValueError(f"{what}: expected {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    if t.requires_grad:
+        _untracked(t, what)
     if t.shape != (rows, cols):
         raise ValueError(f"{what}: expected [{rows}][{cols}], got {list(t.shape)}")
     ld, step = t.stride()
@@ -206,6 +216,13 @@ def _flat(t, count: int, dtype, dev: int, what: str) -> int:
     if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous() or t.numel() < count:
         raise ValueError(f"{what}: expected {count} contiguous {dtype} on GPU {dev}, got {list(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
+
+
+def _weights(t, count: int, dev: int, what: str) -> int:
+    """_flat of float32 values."""
+    if t.requires_grad:
+        _untracked(t, what)
+    return _flat(t, count, torch.float32, dev, what)
 
 
 def moe_sort(ids, T: int, K: int, E: int, bounds, tok_of, slot_of, row_of, stream=None) -> None:
@@ -234,7 +251,7 @@ def moe_unpermute(ys, T: int, K: int, row_of, wts, y, stream=None) -> None:
     """frt_moe_unpermute: y[t] = sum_k wts[t, k] ys[row_of[t * K + k]]; ys [T * K][n], wts T * K float32, y [T][n]."""
     n, dev = ys.shape[-1], ys.get_device()
     _enqueue(lib().frt_moe_unpermute, dev, stream, ys.data_ptr(), _rows(ys, T * K, n, ys, dev, "ys"), _type(ys, "ys"), T, K, n,
-             _flat(row_of, T * K, torch.int32, dev, "row_of"), _flat(wts, T * K, torch.float32, dev, "wts"), y.data_ptr(),
+             _flat(row_of, T * K, torch.int32, dev, "row_of"), _weights(wts, T * K, dev, "wts"), y.data_ptr(),
              _rows(y, T, n, ys, dev, "y"))
 
 
@@ -244,8 +261,8 @@ def moe_unpermute_grad(dy, ys, T: int, K: int, row_of, wts, dys, dwts, stream=No
     n, dev = dy.shape[-1], dy.get_device()
     _enqueue(lib().frt_moe_unpermute_grad, dev, stream, dy.data_ptr(), _rows(dy, T, n, dy, dev, "dy"), ys.data_ptr(),
              _rows(ys, T * K, n, dy, dev, "ys"), _type(dy, "dy"), T, K, n, _flat(row_of, T * K, torch.int32, dev, "row_of"),
-             _flat(wts, T * K, torch.float32, dev, "wts"), dys.data_ptr(), _rows(dys, T * K, n, dy, dev, "dys"),
-             _flat(dwts, T * K, torch.float32, dev, "dwts"))
+             _weights(wts, T * K, dev, "wts"), dys.data_ptr(), _rows(dys, T * K, n, dy, dev, "dys"),
+             _weights(dwts, T * K, dev, "dwts"))
 
 
 def mx4_quantize(x, codes, scales, stream=None) -> None:

@@ -432,3 +432,95 @@ def test_python_refuses_counts_past_the_librarys_ints(monkeypatch):
             moe._enqueue(moe.lib().frt_moe_permute, 0, None, p, 1, 1, T, 1, 1, p, p, 1)
         with pytest.raises(ValueError, match="C int"):
             moe._enqueue(moe.lib().frt_mx4_product, 0, None, p, p, 1, p, p, p, p, 1, T, 8, 32, p, 8, 0)
+
+
+def test_tensors_that_require_a_gradient_are_refused():
+    """The calls record nothing for autograd: with gradients enabled, an input or output that requires one is a ValueError (its
+    gradient would be lost without a word); detached, or with gradients disabled, it is taken (here up to the device's check)."""
+    import flashrt_amd as F
+    x, xs, row = torch.zeros(4, 8), torch.zeros(8, 8), torch.zeros(8, dtype=torch.int32)
+    wts, u8 = torch.ones(8), torch.zeros(64, dtype=torch.uint8)
+    calls = [(F.moe_permute, (x, 4, 2, row, xs)), (F.moe_permute_grad, (xs, 4, 2, row, x)), (F.moe_unpermute, (xs, 4, 2, row, wts, x)),
+             (F.moe_unpermute_grad, (x, xs, 4, 2, row, wts, xs, wts)), (F.mx4_quantize, (torch.zeros(2, 32), u8, u8)),
+             (F.mx4_dequantize, (u8, u8, torch.zeros(2, 32))), (F.mx4_product, (u8.view(4, 16), u8, u8.view(4, 16), u8, torch.zeros(4, 4)))]
+    for fn, args in calls:
+        for i, a in enumerate(args):
+            if not (isinstance(a, torch.Tensor) and a.is_floating_point()):
+                continue
+            with_grad = [b.clone().requires_grad_() if j == i else b for j, b in enumerate(args)]
+            with pytest.raises(ValueError, match="requires a gradient"):
+                fn(*with_grad)
+            with torch.no_grad(), pytest.raises(ValueError, match="device"):
+                fn(*with_grad)
+            with pytest.raises(ValueError, match="device"):
+                fn(*(b.detach() if j == i else b for j, b in enumerate(with_grad)))
+
+
+class _Permute(torch.autograd.Function):
+    """Token rows in expert order, as a user's training code wraps the calls."""
+
+    @staticmethod
+    def forward(ctx, x, row, T, K):
+        import flashrt_amd as F
+        xs = torch.zeros(T * K, x.shape[1], dtype=x.dtype, device=x.device)
+        F.moe_permute(x, T, K, row, xs)
+        ctx.save_for_backward(row)
+        ctx.T, ctx.K = T, K
+        return xs
+
+    @staticmethod
+    def backward(ctx, dxs):
+        import flashrt_amd as F
+        dx = torch.empty(ctx.T, dxs.shape[1], dtype=dxs.dtype, device=dxs.device)
+        F.moe_permute_grad(dxs.contiguous(), ctx.T, ctx.K, ctx.saved_tensors[0], dx)
+        return dx, None, None, None
+
+
+class _Unpermute(torch.autograd.Function):
+    """The weighted sum back into the tokens."""
+
+    @staticmethod
+    def forward(ctx, ys, wts, row, T, K):
+        import flashrt_amd as F
+        y = torch.empty(T, ys.shape[1], dtype=ys.dtype, device=ys.device)
+        F.moe_unpermute(ys, T, K, row, wts, y)
+        ctx.save_for_backward(ys, wts, row)
+        ctx.T, ctx.K = T, K
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        import flashrt_amd as F
+        ys, wts, row = ctx.saved_tensors
+        dys, dw = torch.zeros_like(ys), torch.empty_like(wts)
+        F.moe_unpermute_grad(dy.contiguous(), ys, ctx.T, ctx.K, row, wts, dys, dw)
+        return dys, dw, None, None, None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drop", ["flat", "drop"])
+def test_training_step_through_autograd(drop):
+    """The moves in autograd Functions around an expert's product (row scales here), against autograd of the same in 64 bits on the
+    CPU: the gradients of the tokens, the scales and the routing weights. Errors: a token's row passes the product of three factors
+    and two sums of at most K terms, a weight's gradient a sum of n, so (n + 3 K + 8) roundings of the sum of magnitudes at most."""
+    T, K, E, n = 29, 4, 8, 72
+    ids = slots(T, K, E, drop, 9)
+    _, slot_of, row_of = sorted_slots(ids, E)
+    row = torch.from_numpy(row_of.astype(np.int32)).cuda()
+    g = torch.Generator().manual_seed(2)
+    x, dy, scale, wts = torch.randn(T, n, generator=g), torch.randn(T, n, generator=g), torch.randn(T * K, 1, generator=g), torch.rand(T, K, generator=g)
+    on = [v.cuda().requires_grad_() for v in (x, scale, wts)]
+    y = _Unpermute.apply(_Permute.apply(on[0], row, T, K) * on[1], on[2], row, T, K)
+    y.backward(dy.cuda())
+
+    def plain(x, scale, wts, dy):   # the same from indexing, in 64 bits
+        at, live = torch.from_numpy(np.where(row_of < 0, 0, row_of)), torch.from_numpy(row_of >= 0)
+        leaves = [v.double().requires_grad_() for v in (x, scale, wts)]
+        v = leaves[0].repeat_interleave(K, 0) * leaves[1][at]
+        out = (torch.where(live[:, None], v, 0.0).view(T, K, n) * leaves[2][:, :, None]).sum(1)
+        out.backward(dy.double())
+        return [out.detach()] + [v.grad for v in leaves]
+
+    want, mag = plain(x, scale, wts, dy), plain(x.abs(), scale.abs(), wts, dy.abs())
+    for got, w, m in zip([y] + [v.grad for v in on], want, mag):
+        near(got, w, 1.01 * (n + 3 * K + 8) * U * m)
