@@ -18,6 +18,7 @@ import ctypes as C
 from types import SimpleNamespace
 
 import torch
+from torch.autograd.graph import increment_version
 
 from ._lib import LAYER_NORM_INPUT, FrtArena, FrtError, FrtExpertSlab, FrtLoadStats, FrtMoeLayer, check, lib
 
@@ -151,7 +152,8 @@ def moe_dispatch(ids, T: int, K: int, E: int, bounds, tok_of, slot_of, stream=No
 # These check their tensors (ValueError): type, shape, layout, sizes that the library's ints hold, and that all lie on one GPU,
 # which need not be the current one. None of them is recorded by autograd: with gradients enabled, a tensor that requires one is
 # refused, as torch refuses it for an out= argument. The *_grad calls are for the backward of a torch.autograd.Function (whose
-# forward and backward run with gradients disabled).
+# forward and backward run with gradients disabled). What a call has written counts as changed in place, so that a backward that
+# saved it before says so.
 
 _ROW_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}   # ggml type ids
 
@@ -161,11 +163,15 @@ _ROW_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}   # ggml t
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
+# torch.cuda.current_device() without its check that the GPU is in use: a tensor there says so
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _enqueue(fn, dev: int, stream, *args) -> None:
     """check(fn(stream, *args)) on the stream (by default the current one) of GPU dev."""
     if dev < 0:
         raise ValueError("flashrt_amd: expected a device tensor")
-    if dev != torch.cuda.current_device():
+    if dev != _current_device():
         with torch.cuda.device(dev):
             return _enqueue(fn, dev, stream, *args)
     try:
@@ -231,6 +237,7 @@ def moe_sort(ids, T: int, K: int, E: int, bounds, tok_of, slot_of, row_of, strea
     S, i32, dev = T * K, torch.int32, ids.get_device()
     _enqueue(lib().frt_moe_sort, dev, stream, _flat(ids, S, i32, dev, "ids"), T, K, E, _flat(bounds, E + 1, i32, dev, "bounds"),
              _flat(tok_of, S, i32, dev, "tok_of"), _flat(slot_of, S, i32, dev, "slot_of"), _flat(row_of, S, i32, dev, "row_of"))
+    increment_version((bounds, tok_of, slot_of, row_of))
 
 
 def moe_permute(x, T: int, K: int, row_of, xs, stream=None) -> None:
@@ -238,6 +245,7 @@ def moe_permute(x, T: int, K: int, row_of, xs, stream=None) -> None:
     n, dev = x.shape[-1], x.get_device()
     _enqueue(lib().frt_moe_permute, dev, stream, x.data_ptr(), _rows(x, T, n, x, dev, "x"), _type(x, "x"), T, K, n,
              _flat(row_of, T * K, torch.int32, dev, "row_of"), xs.data_ptr(), _rows(xs, T * K, n, x, dev, "xs"))
+    increment_version(xs)
 
 
 def moe_permute_grad(dxs, T: int, K: int, row_of, dx, stream=None) -> None:
@@ -245,6 +253,7 @@ def moe_permute_grad(dxs, T: int, K: int, row_of, dx, stream=None) -> None:
     n, dev = dxs.shape[-1], dxs.get_device()
     _enqueue(lib().frt_moe_permute_grad, dev, stream, dxs.data_ptr(), _rows(dxs, T * K, n, dxs, dev, "dxs"), _type(dxs, "dxs"), T, K, n,
              _flat(row_of, T * K, torch.int32, dev, "row_of"), dx.data_ptr(), _rows(dx, T, n, dxs, dev, "dx"))
+    increment_version(dx)
 
 
 def moe_unpermute(ys, T: int, K: int, row_of, wts, y, stream=None) -> None:
@@ -253,6 +262,7 @@ def moe_unpermute(ys, T: int, K: int, row_of, wts, y, stream=None) -> None:
     _enqueue(lib().frt_moe_unpermute, dev, stream, ys.data_ptr(), _rows(ys, T * K, n, ys, dev, "ys"), _type(ys, "ys"), T, K, n,
              _flat(row_of, T * K, torch.int32, dev, "row_of"), _weights(wts, T * K, dev, "wts"), y.data_ptr(),
              _rows(y, T, n, ys, dev, "y"))
+    increment_version(y)
 
 
 def moe_unpermute_grad(dy, ys, T: int, K: int, row_of, wts, dys, dwts, stream=None) -> None:
@@ -263,6 +273,7 @@ def moe_unpermute_grad(dy, ys, T: int, K: int, row_of, wts, dys, dwts, stream=No
              _rows(ys, T * K, n, dy, dev, "ys"), _type(dy, "dy"), T, K, n, _flat(row_of, T * K, torch.int32, dev, "row_of"),
              _weights(wts, T * K, dev, "wts"), dys.data_ptr(), _rows(dys, T * K, n, dy, dev, "dys"),
              _weights(dwts, T * K, dev, "dwts"))
+    increment_version((dys, dwts))
 
 
 def mx4_quantize(x, codes, scales, stream=None) -> None:
@@ -270,6 +281,7 @@ def mx4_quantize(x, codes, scales, stream=None) -> None:
     (rows, cols), dev = x.shape, x.get_device()
     _enqueue(lib().frt_mx4_quantize, dev, stream, x.data_ptr(), _rows(x, rows, cols, x, dev, "x"), _type(x, "x"), rows, cols,
              _flat(codes, rows * cols // 2, torch.uint8, dev, "codes"), _flat(scales, rows * cols // 32, torch.uint8, dev, "scales"))
+    increment_version((codes, scales))
 
 
 def mx4_dequantize(codes, scales, out, stream=None) -> None:
@@ -278,6 +290,7 @@ def mx4_dequantize(codes, scales, out, stream=None) -> None:
     _enqueue(lib().frt_mx4_dequantize, dev, stream, _flat(codes, rows * cols // 2, torch.uint8, dev, "codes"),
              _flat(scales, rows * cols // 32, torch.uint8, dev, "scales"), rows, cols, out.data_ptr(),
              _rows(out, rows, cols, out, dev, "out"), _type(out, "out"))
+    increment_version(out)
 
 
 def mx4_product(aq, asc, wq, wsc, out, bounds=None, rows=None, stream=None) -> None:
@@ -293,6 +306,7 @@ def mx4_product(aq, asc, wq, wsc, out, bounds=None, rows=None, stream=None) -> N
              a_rows, None if rows is None else _flat(rows, M, i32, dev, "rows"), _flat(wq, E * N * C // 2, u8, dev, "wq"),
              _flat(wsc, E * N * C // 32, u8, dev, "wsc"), None if bounds is None else _flat(bounds, E + 1, i32, dev, "bounds"), E, M, N, C,
              out.data_ptr(), _rows(out, M, N, out, dev, "out"), _type(out, "out"))
+    increment_version(out)
 
 
 # ---------------------------------------------------------------- prefill grouped GEMM

@@ -425,7 +425,7 @@ def test_python_refuses_counts_past_the_librarys_ints(monkeypatch):
     the device's are left out here: there is no memory for such rows)."""
     from flashrt_amd import moe
     monkeypatch.setattr(moe, "_raw_stream", lambda dev: 0)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(moe, "_current_device", lambda: 0)
     p = 1 << 20
     for T in (2 ** 31, 2 ** 32):
         with pytest.raises(ValueError, match="C int"):
@@ -524,3 +524,35 @@ def test_training_step_through_autograd(drop):
     want, mag = plain(x, scale, wts, dy), plain(x.abs(), scale.abs(), wts, dy.abs())
     for got, w, m in zip([y] + [v.grad for v in on], want, mag):
         near(got, w, 1.01 * (n + 3 * K + 8) * U * m)
+
+
+@pytest.mark.gpu
+def test_written_tensors_count_as_changed():
+    """Every output's version goes up with a call, and no input's; a backward whose saved row map or rows another call has since
+    overwritten says so instead of using them."""
+    import flashrt_amd as F
+    T, K, E, n = 3, 2, 4, 64
+    i32 = lambda m: torch.zeros(m, dtype=torch.int32, device="cuda")  # noqa: E731
+    u8 = lambda *s: torch.zeros(s, dtype=torch.uint8, device="cuda")  # noqa: E731
+    ids = torch.tensor([0, 1, 2, 3, 0, 1], dtype=torch.int32, device="cuda")
+    b, tok, slot, row = i32(E + 1), i32(T * K), i32(T * K), i32(T * K)
+    x, xs, y, dys = (torch.randn(r, n, device="cuda") for r in (T, T * K, T, T * K))
+    w, dw, q, s, h = torch.rand(T, K, device="cuda"), torch.zeros(T, K, device="cuda"), u8(T, n // 2), u8(T, n // 32), torch.zeros(T, T, device="cuda")
+    everything = [ids, b, tok, slot, row, x, xs, y, dys, w, dw, q, s, h]
+    for outs, call in [((b, tok, slot, row), lambda: F.moe_sort(ids, T, K, E, b, tok, slot, row)), ((xs,), lambda: F.moe_permute(x, T, K, row, xs)),
+                       ((y,), lambda: F.moe_permute_grad(xs, T, K, row, y)), ((y,), lambda: F.moe_unpermute(xs, T, K, row, w, y)),
+                       ((dys, dw), lambda: F.moe_unpermute_grad(x, xs, T, K, row, w, dys, dw)), ((q, s), lambda: F.mx4_quantize(x, q, s)),
+                       ((y,), lambda: F.mx4_dequantize(q, s, y)), ((h,), lambda: F.mx4_product(q, s, q, s, h))]:
+        was = [v._version for v in everything]
+        call()
+        for v, old in zip(everything, was):
+            assert v._version == old + any(v is o for o in outs)
+    for overwrite in (lambda: F.moe_sort(ids, T, K, E, b, tok, slot, row), lambda: F.moe_permute(x, T, K, row, xs)):
+        out = _Unpermute.apply(xs, w.clone().requires_grad_(), row, T, K)
+        overwrite()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
+    with torch.inference_mode():   # (tensors without a version)
+        z = torch.empty(T * K, n, device="cuda")
+        F.moe_permute(x, T, K, row, z)
+        assert torch.equal(z, x[tok.long()])
