@@ -472,6 +472,12 @@ static int rows_check(const char* what, const char* name, const void* p, int64_t
     if (reinterpret_cast<uintptr_t>(p) % (type == FRT_GGML_F32 ? 4 : 2)) return set_error(kErrShape, "%s: %s misaligned", what, name);
     return kOk;
 }
+// int32 or fp32 values
+static int words_check(const char* what, const char* name, const void* p) {
+    if (!p) return set_error(kErrNull, "%s: null %s", what, name);
+    if (reinterpret_cast<uintptr_t>(p) % 4) return set_error(kErrShape, "%s: %s misaligned", what, name);
+    return kOk;
+}
 static int move_check(const char* what, int type, int T, int K, int n) {
     if (int rc = type_check(what, type)) return rc;
     if (T < 0 || K < 1 || n < 1 || n > (1 << 30) || int64_t(T) * K > 0x7fffffff)
@@ -627,7 +633,13 @@ int frt_moe_sort(void* stream, const int32_t* ids, int T, int K, int E, int32_t*
                  int32_t* row_of) {
     if (T < 0 || K < 1 || E < 1 || E > 1024 || int64_t(T) * K > 0x7fffffff)
         return set_error(kErrShape, "moe_sort: T=%d K=%d E=%d", T, K, E);
-    if (!bounds || (T > 0 && (!ids || !tok_of || !slot_of || !row_of))) return set_error(kErrNull, "moe_sort: null pointer");
+    if (int rc = words_check("moe_sort", "bounds", bounds)) return rc;
+    if (T > 0) {
+        if (int rc = words_check("moe_sort", "ids", ids)) return rc;
+        if (int rc = words_check("moe_sort", "tok_of", tok_of)) return rc;
+        if (int rc = words_check("moe_sort", "slot_of", slot_of)) return rc;
+        if (int rc = words_check("moe_sort", "row_of", row_of)) return rc;
+    }
     return moe_sort(ids, T, K, E, bounds, tok_of, slot_of, row_of, static_cast<hipStream_t>(stream));
 }
 
@@ -635,7 +647,7 @@ int frt_moe_permute(void* stream, const void* x, int64_t ldx, int type, int T, i
                     int64_t ldxs) {
     if (int rc = move_check("moe_permute", type, T, K, n)) return rc;
     if (T == 0) return kOk;
-    if (!row_of) return set_error(kErrNull, "moe_permute: null row_of");
+    if (int rc = words_check("moe_permute", "row_of", row_of)) return rc;
     if (int rc = rows_check("moe_permute", "x", x, ldx, n, type)) return rc;
     if (int rc = rows_check("moe_permute", "xs", xs, ldxs, n, type)) return rc;
     return moe_permute(type, x, ldx, T, K, n, row_of, xs, ldxs, static_cast<hipStream_t>(stream));
@@ -645,7 +657,7 @@ int frt_moe_permute_grad(void* stream, const void* dxs, int64_t lddxs, int type,
                          void* dx, int64_t lddx) {
     if (int rc = move_check("moe_permute_grad", type, T, K, n)) return rc;
     if (T == 0) return kOk;
-    if (!row_of) return set_error(kErrNull, "moe_permute_grad: null row_of");
+    if (int rc = words_check("moe_permute_grad", "row_of", row_of)) return rc;
     if (int rc = rows_check("moe_permute_grad", "dxs", dxs, lddxs, n, type)) return rc;
     if (int rc = rows_check("moe_permute_grad", "dx", dx, lddx, n, type)) return rc;
     return moe_sum_rows(type, dxs, lddxs, T, K, n, row_of, nullptr, dx, lddx, static_cast<hipStream_t>(stream));
@@ -655,7 +667,8 @@ int frt_moe_unpermute(void* stream, const void* ys, int64_t ldys, int type, int 
                       const float* wts, void* y, int64_t ldy) {
     if (int rc = move_check("moe_unpermute", type, T, K, n)) return rc;
     if (T == 0) return kOk;
-    if (!row_of || !wts) return set_error(kErrNull, "moe_unpermute: null row_of or wts");
+    if (int rc = words_check("moe_unpermute", "row_of", row_of)) return rc;
+    if (int rc = words_check("moe_unpermute", "wts", wts)) return rc;
     if (int rc = rows_check("moe_unpermute", "ys", ys, ldys, n, type)) return rc;
     if (int rc = rows_check("moe_unpermute", "y", y, ldy, n, type)) return rc;
     return moe_sum_rows(type, ys, ldys, T, K, n, row_of, wts, y, ldy, static_cast<hipStream_t>(stream));
@@ -665,7 +678,9 @@ int frt_moe_unpermute_grad(void* stream, const void* dy, int64_t lddy, const voi
                            int n, const int32_t* row_of, const float* wts, void* dys, int64_t lddys, float* dwts) {
     if (int rc = move_check("moe_unpermute_grad", type, T, K, n)) return rc;
     if (T == 0) return kOk;
-    if (!row_of || !wts || !dwts) return set_error(kErrNull, "moe_unpermute_grad: null row_of, wts or dwts");
+    if (int rc = words_check("moe_unpermute_grad", "row_of", row_of)) return rc;
+    if (int rc = words_check("moe_unpermute_grad", "wts", wts)) return rc;
+    if (int rc = words_check("moe_unpermute_grad", "dwts", dwts)) return rc;
     if (int rc = rows_check("moe_unpermute_grad", "dy", dy, lddy, n, type)) return rc;
     if (int rc = rows_check("moe_unpermute_grad", "ys", ys, ldys, n, type)) return rc;
     if (int rc = rows_check("moe_unpermute_grad", "dys", dys, lddys, n, type)) return rc;
@@ -701,6 +716,10 @@ int frt_mx4_product(void* stream, const void* aq, const void* asc, int a_rows, c
     if (a_rows < (rows ? 1 : M)) return set_error(kErrShape, "mx4_product: %d rows of activations for M=%d", a_rows, M);
     if (int rc = codes_check("mx4_product", "activations", aq, asc)) return rc;
     if (int rc = codes_check("mx4_product", "weights", wq, wsc)) return rc;
+    if (rows)
+        if (int rc = words_check("mx4_product", "rows", rows)) return rc;
+    if (bounds)
+        if (int rc = words_check("mx4_product", "bounds", bounds)) return rc;
     if (int rc = rows_check("mx4_product", "out", out, ldout, N, type)) return rc;
     return mx4_product(aq, asc, a_rows, rows, wq, wsc, bounds, E, M, N, C, out, type, ldout, static_cast<hipStream_t>(stream));
 }

@@ -151,7 +151,7 @@ int frt_moe_dispatch(void* stream, const int32_t* ids, int T, int K, int E, int3
  * slot's row or -1.
  * The moves take rows of type FRT_GGML_F32, FRT_GGML_F16 or FRT_GGML_BF16, any n from 1 to 2^30, at ld* elements from one row
  * to the next (ld* >= n), and row_of as frt_moe_sort wrote it (an entry outside [0, S) is a dropped slot's). Sums are fp32,
- * ascending k, rounded once. Inputs and outputs must not overlap.
+ * ascending k, rounded once. Inputs and outputs must not overlap. Every pointer, of the product below too, is aligned to its values.
  *   permute         xs[row_of[s]] = x[s / K]; other rows of xs stay as they were
  *   permute_grad    dx[t] = sum over the token's rows of dxs[row_of[t K + k]]
  *   unpermute       y[t] = sum_k wts[t K + k] ys[row_of[t K + k]], wts fp32; 0 for a token without rows

@@ -556,3 +556,23 @@ def test_written_tensors_count_as_changed():
         z = torch.empty(T * K, n, device="cuda")
         F.moe_permute(x, T, K, row, z)
         assert torch.equal(z, x[tok.long()])
+
+
+def test_misaligned_words_are_refused():
+    """Ids, row maps, bounds, picked rows and weights that are not 4-byte aligned are refused before any launch (the kernels read
+    some of them through scalar loads, which drop an address's low bits)."""
+    from flashrt_amd import _lib
+    L = _lib.lib()
+    p = 1 << 20
+    for fn, good, ptrs in ((L.frt_moe_sort, [None, p, 2, 2, 4, p, p, p, p], (1, 5, 6, 7, 8)),
+                           (L.frt_moe_permute, [None, p, 8, 30, 2, 2, 8, p, p, 8], (7,)),
+                           (L.frt_moe_permute_grad, [None, p, 8, 30, 2, 2, 8, p, p, 8], (7,)),
+                           (L.frt_moe_unpermute, [None, p, 8, 30, 2, 2, 8, p, p, p, 8], (7, 8)),
+                           (L.frt_moe_unpermute_grad, [None, p, 8, p, 8, 30, 2, 2, 8, p, p, p, 8, p], (9, 10, 13)),
+                           (L.frt_mx4_product, [None, p, p, 5, p, p, p, p, 4, 5, 24, 64, p, 24, 30], (4, 7))):
+        for i in ptrs:
+            for off in (1, 2, 3):
+                a = list(good)
+                a[i] = p + off
+                assert fn(*a) == -1, (fn.__name__, i, off, L.frt_last_error())
+                assert b"misaligned" in L.frt_last_error()
