@@ -261,17 +261,18 @@ __global__ void __launch_bounds__(256) k_sum_rows(const T* __restrict__ ys, int6
     const unsigned S = unsigned(n_tok) * K;
     const size_t s0 = size_t(t) * K;
     float acc[V] = {};
-    for (int k0 = 0; k0 < K; k0 += 4) {
+    const uint32_t slots = K;   // (k0 passes 2^31 after the last step where K is near it)
+    for (uint32_t k0 = 0; k0 < slots; k0 += 4) {
         int row[4];
         Piece<T> p[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) row[k] = row_of[s0 + min(k0 + k, K - 1)];
+        for (uint32_t k = 0; k < 4; ++k) row[k] = row_of[s0 + min(k0 + k, slots - 1)];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k0 + k < K && unsigned(row[k]) < S) p[k] = piece_load(ys + row[k] * ldys, c, n);
+        for (uint32_t k = 0; k < 4; ++k)
+            if (k0 + k < slots && unsigned(row[k]) < S) p[k] = piece_load(ys + row[k] * ldys, c, n);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k0 + k < K && unsigned(row[k]) < S) {
+        for (uint32_t k = 0; k < 4; ++k)
+            if (k0 + k < slots && unsigned(row[k]) < S) {
                 const float w = WTS ? wts[s0 + k0 + k] : 1.0f;
 #pragma unroll
                 for (int i = 0; i < V; ++i) acc[i] = WTS ? fmaf(w, float(p[k].v[i]), acc[i]) : acc[i] + float(p[k].v[i]);

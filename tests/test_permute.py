@@ -576,3 +576,27 @@ def test_misaligned_words_are_refused():
                 a[i] = p + off
                 assert fn(*a) == -1, (fn.__name__, i, off, L.frt_last_error())
                 assert b"misaligned" in L.frt_last_error()
+
+
+@pytest.mark.gpu
+def test_tokens_of_many_slots():
+    """Two tokens of 200,003 slots each (no multiple of the four rows in flight): small integers, so that every sum is exact."""
+    import flashrt_amd as F
+    T, K, n = 2, 200003, 3
+    g = torch.Generator().manual_seed(4)
+    row = torch.randperm(T * K, generator=g).to(torch.int32)
+    row[::7] = -1
+    ys = torch.randint(-2, 3, (T * K, n), generator=g).float()
+    wts = torch.randint(0, 3, (T, K), generator=g).float()
+    live = (row >= 0)[:, None]
+    picked = torch.where(live, ys[row.clamp_min(0).long()], 0.0).double().view(T, K, n)
+    y, dx = torch.empty(T, n, device="cuda"), torch.empty(T, n, device="cuda")
+    F.moe_unpermute(ys.cuda(), T, K, row.cuda(), wts.cuda(), y)
+    F.moe_permute_grad(ys.cuda(), T, K, row.cuda(), dx)
+    assert torch.equal(y.cpu().double(), (picked * wts.double()[:, :, None]).sum(1)) and torch.equal(dx.cpu().double(), picked.sum(1))
+    x = torch.randint(-9, 9, (T, n), generator=g).float()
+    xs = torch.full((T * K, n), 77.0, device="cuda")
+    F.moe_permute(x.cuda(), T, K, row.cuda(), xs)
+    want = torch.full((T * K, n), 77.0)
+    want[row[row >= 0].long()] = x.repeat_interleave(K, 0)[row >= 0]
+    assert torch.equal(xs.cpu(), want)
