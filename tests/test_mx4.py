@@ -578,3 +578,171 @@ def test_experts_in_a_run(T):
     h2 = torch.zeros_like(h)
     F.mx4_product(sq, ssc, uq, us, h2, bounds=b)
     assert torch.equal(h, h2)
+
+
+# ---------------------------------------------------------------- the product's limits, for every kernel
+
+def tile_groups(tile, C):
+    """(bounds, features) of a row of TILES at C values, over the 16 MB from which the tiles are taken."""
+    sizes, N = TILES[tile]
+    if len(sizes) > 1:
+        avg = sum(sizes) // len(sizes)
+        sizes = sizes * max(1, -(-(17 << 20) // (-(-avg // 16) * len(sizes) * N * C // 2)))
+    return cut(sizes), N
+
+
+# one group: few rows, and the tiles of 32, 64, 128 and 256 rows by the rule of product_t
+DENSE = {"few": (20, 130, 1056), "rows32": (24, 8200, 2112), "rows64": (48, 20500, 640), "rows128": (200, 16300, 352), "rows256": (300, 16200, 1056)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.float16])
+@pytest.mark.parametrize("shape", list(DENSE))
+def test_one_group_in_every_kernel(shape, kind):
+    """Neither bounds nor rows: one group, each row its own activations."""
+    import flashrt_amd as F
+    M, N, C = DENSE[shape]
+    ops = operands(M, 1, N, C, M)
+    check_product(run_product(F, ops, M, kind, pad=5), ops, M, kind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,kind", [(352, torch.float32), (1024, torch.bfloat16), (1056, torch.float32)])
+def test_largest_tile_with_ragged_groups(C, kind):
+    """Eight groups of 0 to 700 rows, 269 on average: the tiles of 256 rows."""
+    import flashrt_amd as F
+    bounds = cut([257, 700, 0, 1, 512, 300, 255, 130])
+    M, N = bounds[-1] + 3, 1801
+    ops = operands(400, 8, N, C, C)
+    rows = np.random.default_rng(C).integers(-1, 401, M)
+    check_product(run_product(F, ops, M, kind, bounds, rows, pad=2), ops, M, kind, bounds, rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [544, 640])
+@pytest.mark.parametrize("tile", ["few"] + list(TILES))
+def test_scale_extremes(tile, C):
+    """The smallest and largest scale bytes with every code, products in range: 2^-127 times 2^127 is one, 2^-127 times one leaves
+    fp32 results below 2^-126, which are exact (multiples of 2^-129, fewer than 2^24 of them)."""
+    import flashrt_amd as F
+    bounds, N = tile_groups(tile, C) if tile in TILES else (cut([1, 0, 16, 3]), 70)
+    M = bounds[-1]
+    ops = operands(M, len(bounds) - 1, N, C, 9)
+    for a, w in ((0, 254), (254, 0), (1, 253), (0, 127), (127, 0)):
+        o = (ops[0], np.full_like(ops[1], a), ops[2], np.full_like(ops[3], w))
+        got = run_product(F, o, M, torch.float32, bounds)
+        check_product(got, o, M, torch.float32, bounds)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [544, 640])
+@pytest.mark.parametrize("tile", list(TILES))
+def test_nan_scales_in_tiles(tile, C):
+    """A NaN block of a row, in a whole stage or in the last, shorter one, makes that row NaN alone; one of a feature, that feature of its
+    group's rows alone. Everything else is bit for bit what it is without them."""
+    import flashrt_amd as F
+    bounds, N = tile_groups(tile, C)
+    M, nb = bounds[-1], C // 32
+    ops = operands(M, len(bounds) - 1, N, C, 9)
+    o = [v.copy() for v in ops]
+    nan = torch.zeros(M, N, dtype=torch.bool)
+    for r, b in ((0, 0), (7, nb - 1), (M // 2, 3), (M - 1, nb - 1)):
+        o[1][r, b], nan[r] = 255, True
+    for g, f, b in ((0, N - 1, nb - 1), (len(bounds) - 2, 0, 0), (len(bounds) // 3, 67, nb - 2)):
+        o[3][g, f, b], nan[bounds[g]:bounds[g + 1], f] = 255, True
+    got, clean = run_product(F, o, M, torch.float32, bounds).cpu(), run_product(F, ops, M, torch.float32, bounds).cpu()
+    assert torch.equal(got.isnan(), nan) and torch.equal(got[~nan], clean[~nan])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tile", ["few"] + list(TILES))
+def test_half_precision_results_that_overflow(tile):
+    """fp16 results past its largest number are infinities of their sign; the others keep their bound."""
+    import flashrt_amd as F
+    C = 544
+    bounds, N = tile_groups(tile, C) if tile in TILES else (cut([1, 0, 16, 3]), 70)
+    M = bounds[-1]
+    ops = operands(M, len(bounds) - 1, N, C, 2)
+    ops = (ops[0], np.full_like(ops[1], 134), ops[2], np.full_like(ops[3], 128))   # 2^8: sums around 2^16
+    got = run_product(F, ops, M, torch.float16, bounds).cpu()
+    a, w = values(ops[0], ops[1]), values(ops[2], ops[3])
+    seen = 0
+    for g in range(len(bounds) - 1):
+        lo, hi = bounds[g], bounds[g + 1]
+        want = torch.from_numpy(a[lo:hi] @ w[g].T)   # (multiples of 2^6 below 2^30: exact in fp32, whatever the order)
+        assert torch.equal(got[lo:hi], want.half())
+        seen += int(got[lo:hi].isinf().sum())
+    assert 0 < seen < M * N
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tile", list(TILES))
+def test_bounds_out_of_order_in_tiles(tile):
+    """Bounds that no sort gives (past the rows, negative, descending, all the same), in the tile kernels: nothing before or behind the
+    rows is written, and no index leaves the operands (the kernel clamps the bounds to the rows; the results are unspecified)."""
+    import flashrt_amd as F
+    C = 544
+    bounds, N = tile_groups(tile, C)
+    E, M = len(bounds) - 1, bounds[-1]
+    aq, asc, wq, wsc = (torch.from_numpy(v).cuda() for v in operands(M, E, N, C, 1))
+    buf = torch.full((M + 64, N + 3), 77.0, device="cuda")
+    r = np.random.default_rng(E)
+    for cuts in (np.array(bounds) + M // 2, np.array(bounds) - M // 2, np.array(bounds)[::-1], r.integers(-M, 2 * M, E + 1),
+                 np.full(E + 1, M), np.full(E + 1, 2 ** 31 - 1), np.full(E + 1, -2 ** 31), np.resize([0, M], E + 1), np.resize([-2 ** 31, 2 ** 31 - 1], E + 1)):
+        F.mx4_product(aq, asc, wq, wsc, buf[32:32 + M, :N], bounds=torch.from_numpy(cuts.astype(np.int32)).cuda())
+        assert (buf[:32] == 77).all() and (buf[32 + M:] == 77).all() and (buf[:, N:] == 77).all()
+
+
+@pytest.mark.gpu
+def test_few_rows_of_weights_past_32_bits():
+    """The kernel of few rows (four rows: 16 MB of weights to read) on the last two of 1100 experts of 2048 x 4096."""
+    import flashrt_amd as F
+    E, N, C, M = 1100, 2048, 4096, 4
+    wq = torch.zeros((E, N, C // 2), dtype=torch.uint8, device="cuda")
+    wsc = torch.full((E, N, C // 32), 127, dtype=torch.uint8, device="cuda")
+    ops = operands(M, 2, N, C, 8)
+    aq, asc, q, s = (torch.from_numpy(v).cuda() for v in ops)
+    wq[E - 2:], wsc[E - 2:] = q, s
+    bounds = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    bounds[E - 1], bounds[E] = 1, M
+    out = torch.empty(M, N, device="cuda")
+    F.mx4_product(aq, asc, wq, wsc, out, bounds=bounds)
+    check_product(out, ops, M, torch.float32, [0, 1, M])
+
+
+@pytest.mark.gpu
+def test_rows_in_one_kernel_and_across_kernels():
+    """A row's bits do not depend on the rows beside it where the same kernel takes them (few rows: 1 to 300; the tiles of 256: 2049
+    and 4200). Across kernels the order of the sums differs: each is within C u sum |a w| of the exact one."""
+    import flashrt_amd as F
+    N, C = 200, 1056
+    ops = operands(300, 1, N, C, 4)
+    whole = run_product(F, ops, 300, torch.float32)
+    for m in (1, 9, 40, 130):
+        assert torch.equal(run_product(F, (ops[0][:m], ops[1][:m], ops[2], ops[3]), m, torch.float32), whole[:m])
+    N = 4104
+    ops = operands(4200, 1, N, C, 5)
+    whole = run_product(F, ops, 4200, torch.float32)
+    assert torch.equal(run_product(F, (ops[0][:2049], ops[1][:2049], ops[2], ops[3]), 2049, torch.float32), whole[:2049])
+    few = run_product(F, (ops[0][:5], ops[1][:5], ops[2], ops[3]), 5, torch.float32)
+    mag = torch.from_numpy(np.abs(values(ops[0][:5], ops[1][:5])) @ np.abs(values(ops[2][0], ops[3][0])).T)
+    near(few, whole[:5].cpu().double(), 2 * 1.01 * C * U * mag)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tile", ["few"] + list(TILES))
+def test_scales_far_apart_in_a_row(tile):
+    """Blocks of a row whose scales differ by up to 2^60, large ones that cancel among them: the sums keep 24 bits of the largest."""
+    import flashrt_amd as F
+    C = 544
+    bounds, N = tile_groups(tile, C) if tile in TILES else (cut([1, 0, 16, 3]), 70)
+    M = bounds[-1]
+    ops = operands(M, len(bounds) - 1, N, C, 6)
+    r = np.random.default_rng(6)
+    ops = (ops[0], r.integers(112, 143, ops[1].shape).astype(np.uint8), ops[2], r.integers(112, 143, ops[3].shape).astype(np.uint8))
+    got = run_product(F, ops, M, torch.float32, bounds)
+    a, w = values(ops[0], ops[1]), values(ops[2], ops[3])
+    for g in range(len(bounds) - 1):
+        lo, hi = bounds[g], bounds[g + 1]
+        want, mag = a[lo:hi] @ w[g].T, np.abs(a[lo:hi]) @ np.abs(w[g]).T
+        near(got[lo:hi], torch.from_numpy(want), torch.from_numpy(1.01 * (C * U * mag + U * np.abs(want))))
