@@ -106,6 +106,11 @@ struct FastDiv {
     __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return uint32_t((uint64_t(n) * m) >> s); }
 };
 
+// fn<type> of a ggml type id (FRT_GGML_F32, F16 or BF16)
+#define FRT_BY_TYPE(type, fn, ...)                                                            \
+    ((type) == FRT_GGML_F32 ? fn<float>(__VA_ARGS__)                                          \
+                            : (type) == FRT_GGML_F16 ? fn<_Float16>(__VA_ARGS__) : fn<__bf16>(__VA_ARGS__))
+
 inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // ---- device helpers
@@ -214,8 +219,8 @@ __device__ __forceinline__ float half_max(float v) {
     const float b = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
     return (threadIdx.x & 32) ? b : a;
 }
-// A grid of fewer than 2^31 workgroups of up to 256 threads, in two dimensions where one would pass the launch's 2^32 threads; a few
-// workgroups may lie past the last one asked for.
+// A grid of fewer than 2^31 workgroups of up to 256 threads (a launch has fewer than 2^32 threads in a dimension), in two dimensions
+// beyond 2^23 of them; a few workgroups may lie past the last one asked for.
 inline dim3 wide_grid(uint32_t wgs) {
     const uint32_t y = uint32_t((uint64_t(wgs) + (1u << 23) - 1) >> 23);
     return dim3((wgs + y - 1) / y, y);

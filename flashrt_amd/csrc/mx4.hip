@@ -56,7 +56,7 @@ __device__ __forceinline__ float scale_value(uint32_t b) {
 // exponent is amax's; its byte k + 125 is the exponent field of amax less 2, at least 0 (2^-127, all smaller blocks). A value's
 // code is x 2^-(k - 2), an exact product, rounded to nearest even by the conversion instruction, at most 6. A block with
 // an infinity or a NaN (the exponent field 255 in the largest absolute bits) gets the NaN scale and zero codes. Bound by HBM:
-// 20480 x 2560 bf16 24.9 us, 5.4 TB/s.
+// 20480 x 2560 bf16 25 us, 5.3 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(256) k_mx4_quantize(const T* __restrict__ x, int64_t ldx, uint32_t pieces, uint32_t per_row, FastDiv div,
                                                       uint32_t* __restrict__ codes, uint8_t* __restrict__ scales) {
@@ -84,8 +84,8 @@ __global__ void __launch_bounds__(256) k_mx4_quantize(const T* __restrict__ x, i
     if ((i & 3) == 0) scales[i >> 2] = uint8_t(b);
 }
 
-// Eight codes per lane by the conversion instruction (27.4 us for 20480 x 2560 to bf16, 4.9 TB/s; in integer operations the VALU bound
-// it at 35).
+// Eight codes per lane by the conversion instruction: 20480 x 2560 to bf16 25.5 us, 5.2 TB/s (20 with the codes in the last cache, just
+// quantised; in integer operations the VALU bound it at 35).
 template <typename T>
 __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                         uint32_t pieces, uint32_t per_row, FastDiv div, T* __restrict__ out, int64_t ldout) {
@@ -346,17 +346,19 @@ constexpr uint32_t kNoStore = 0x80000000u;
 // row r sits at c ^ (r / 2 % 8), so that the sixteen rows of a read phase take sixteen different columns of the banks.
 // The scales go the same way, 2 SS words of each row at a time (side by side: the loads' cost is lines, not bytes): those of SS stages
 // where the rows of scales are words (WORDS: a multiple of 128 values), else the aligned words around those of SS - 1 stages, of
-// which a lane takes its bytes by a shift (a row's first and last word may reach three bytes past the row). In step t (0..3) lane half h
+// which a lane takes its bytes by a shift (a row's first and last word may reach three bytes past the row, the tensor's too: in the same
+// aligned word, and unused; reading the bytes within one by one instead cost 4 to 8% of the calls that have such a word). In step t (0..3) lane half h
 // multiplies block 4 h + t of its rows, so that a lane's four scales of a stage are one word and the step picks its byte. Step t +
 // 1's operands are read before step t's products, the next stage's first ones before the last step's, past the barrier. The
 // stages of the feature tiles form one sequence: the next tile's first stages load while this one's results are written.
 //
 // What bounds it: with few rows to a group the weights' stream (2030 rows over 512 experts, N 1024, C 2048: 68 us, 7.3 TB/s of
 // weights); with tens of rows what a CU's loads bring in from beyond L2, about 30 bytes per ns (20480 rows 124 us, 0.57 GB of weights
-// and as much again of activations and results); with one large group the matrix cores, 43% busy at the 1.97 GHz that the card keeps
-// under them, the rest barriers, LDS reads and the loads' issue (8192 rows, N 8192, C 4096: 149 us, 3.7 PFLOP/s). Measured without
-// gain: stages of 128 values with twice the slots (20480 rows 139 -> 158 us), eight waves for the smaller tiles, another first stage
-// in each workgroup.
+// and as much again of activations and results; the matrix cores 16% busy); with one large group the matrix cores, 43% busy at the 1.98
+// GHz that the card keeps under them, and LDS: a stage's reads and direct loads are 256 KB, at 128 bytes a clock the products' own 2048
+// clocks, and two slots with a barrier per stage overlap the two in part (8192 rows, N 8192, C 4096: 149 us, 3.7 PFLOP/s). Measured
+// without gain: stages of 128 values with twice the slots (20480 rows 139 -> 158 us), eight waves for the smaller tiles, another first
+// stage in each workgroup. The 256-row tile spills 3 VGPRs with scales at any byte, and 1 and 6 SGPRs with fp32 results and whole words.
 template <typename T, int BM, int BN, int WM, int WN, int ST, int SS, int PT, bool WORDS>
 __global__ void __launch_bounds__(64 * WM * WN) k_mx4_tiles(Mx4Args p, int ntile, int per, FastDiv chunks, uint32_t nchunk, int stream) {
     constexpr int NW = WM * WN;
@@ -767,9 +769,6 @@ static int product_t(const Mx4Args& p, hipStream_t stream) {
     return nb >= 64 ? rows_t<T, 4>(p, stream) : nb >= 32 ? rows_t<T, 2>(p, stream) : rows_t<T, 1>(p, stream);
 }
 
-#define FRT_BY_TYPE(type, fn, ...)                                                            \
-    ((type) == FRT_GGML_F32 ? fn<float>(__VA_ARGS__)                                          \
-                            : (type) == FRT_GGML_F16 ? fn<_Float16>(__VA_ARGS__) : fn<__bf16>(__VA_ARGS__))
 int mx4_quantize(int type, const void* x, int64_t ldx, int64_t rows, int cols, void* codes, void* scales, hipStream_t stream) {
     return FRT_BY_TYPE(type, quantize_t, x, ldx, rows, cols, codes, scales, stream);
 }

@@ -59,7 +59,8 @@ constexpr int kSortCopies = 16;    // histogram copies, one per lane of a row of
 constexpr int kSortGrid = 256;     // workgroups at most
 
 // Up to 64 slots (a decode step): every wave has all ids, one per lane. A group's first row is the number of ids below it, a slot's
-// row the number of ids that sort before it: no histogram, scan or barrier. One token's 10 slots 8.2 -> 2.6 us.
+// row the number of ids that sort before it: no histogram, scan or barrier. One token's 10 slots 2.4 us, launches back to back (8.2 with the
+// kernel below).
 __global__ void __launch_bounds__(1024) k_sort_few(const int32_t* __restrict__ ids, int S, int K, int E, int32_t* __restrict__ bounds,
                                                    int32_t* __restrict__ tok_of, int32_t* __restrict__ slot_of,
                                                    int32_t* __restrict__ row_of) {
@@ -90,9 +91,12 @@ __global__ void __launch_bounds__(1024) k_sort_few(const int32_t* __restrict__ i
 // the totals over the experts gives the groups' first rows, and the workgroup ranks its own slots in batches of 1024, a wave of
 // 64 at a time by ballots over the id bits (stable). Integer counts: the result does not depend on the atomics' order. The
 // counting reads 16 ids per thread at once and spends three instructions on an id: ids outside are counted in a bin of their own,
-// and the histogram is the wave's choice (81920 slots of 512 experts 11.8 us; with two passes and a branch per id 13.7, reading
-// one by one 22.4; many more slots are bound by the LDS atomics, about 8 clocks per 64 ids). One launch instead of the dispatch's four costs each workgroup the whole list, 328 KB from L2 at 81920
-// slots. ONE: a single batch, whose ranking counts it.
+// and the histogram is the wave's choice (81920 slots of 512 experts, launches back to back, 11.8 us, of which 4.9 are the LDS atomics,
+// about 8 clocks per 64 ids; with two passes and a branch per id 13.7, reading one by one 22.4; a launch alone in a trace takes 13.2).
+// One launch instead of the dispatch's four costs each workgroup the whole list, 328 KB from L2 at 81920 slots, so the time grows
+// with the list, bound by the atomics; the dispatch stays behind it (us, this and the dispatch: 2048 slots 7.4 / 10.3, 20480 9.0 / 19.2,
+// 81920 11.5 / 25.3, 2^18 21 / 44, 2^20 61 / 139, 2^23 430 / 966, 2^26 3863 / 10898).
+// ONE: a single batch, whose ranking counts it.
 template <bool ONE>
 __global__ void __launch_bounds__(1024) k_sort(const int32_t* __restrict__ ids, int S, int K, int E, int id_bits, int batches,
                                                int32_t* __restrict__ bounds, int32_t* __restrict__ tok_of,
@@ -377,9 +381,6 @@ static int unpermute_grad_t(const void* dy, int64_t lddy, const void* ys, int64_
     return kOk;
 }
 
-#define FRT_BY_TYPE(type, fn, ...)                                                            \
-    ((type) == FRT_GGML_F32 ? fn<float>(__VA_ARGS__)                                          \
-                            : (type) == FRT_GGML_F16 ? fn<_Float16>(__VA_ARGS__) : fn<__bf16>(__VA_ARGS__))
 int moe_permute(int type, const void* x, int64_t ldx, int T, int K, int n, const int32_t* row_of, void* xs, int64_t ldxs,
                 hipStream_t stream) {
     return FRT_BY_TYPE(type, permute_t, x, ldx, T, K, n, row_of, xs, ldxs, stream);

@@ -148,7 +148,7 @@ int frt_moe_dispatch(void* stream, const int32_t* ids, int T, int K, int E, int3
  * dropped: it has no row. T may be 0 (nothing is read; moe_sort then writes bounds of zeros).
  * frt_moe_sort: a stable sort of the slots by expert, as frt_moe_dispatch's, with the inverse map, in one launch without a
  * workspace: bounds [E+1]; slot_of and tok_of (= slot_of / K) [S], of which the first bounds[E] are written; row_of [S], the
- * slot's row or -1.
+ * slot's row or -1. Its time grows with S: 81920 slots 12 us, 2^20 61 us, 2^26 3.9 ms.
  * The moves take rows of type FRT_GGML_F32, FRT_GGML_F16 or FRT_GGML_BF16, any n from 1 to 2^30, at ld* elements from one row
  * to the next (ld* >= n), and row_of as frt_moe_sort wrote it (an entry outside [0, S) is a dropped slot's). Sums are fp32,
  * ascending k, rounded once. Inputs and outputs must not overlap. Every pointer, of the product below too, is aligned to its values.
