@@ -23,9 +23,10 @@ class _CInt(C.c_int):
     @classmethod
     def from_param(cls, v):
         if type(v) is not int:
-            if isinstance(v, C._SimpleCData):
+            try:
+                v = operator.index(v)
+            except TypeError:   # no integer: a ctypes one, or an object's _as_parameter_
                 return C.c_int.from_param(v)
-            v = operator.index(v)
         if -0x80000000 <= v <= 0x7fffffff:
             return v
         raise OverflowError(f"{v} is outside a C int")

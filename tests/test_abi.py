@@ -211,3 +211,11 @@ def test_counts_of_other_integer_types():
             L.frt_q2_mat_bytes(bad, 2048)
     with pytest.raises(C.ArgumentError):
         L.frt_q2_mat_bytes(np.int64(1 << 32), 2048)
+
+
+def test_count_behind_as_parameter():
+    """An object that ctypes takes by its _as_parameter_ is still taken."""
+    class Count:
+        _as_parameter_ = 512
+    L = _lib.lib()
+    assert L.frt_q2_mat_bytes(Count(), 2048) == L.frt_q2_mat_bytes(512, 2048)
