@@ -59,8 +59,8 @@ constexpr int kSortCopies = 16;    // histogram copies, one per lane of a row of
 constexpr int kSortGrid = 256;     // workgroups at most
 
 // Up to 64 slots (a decode step): every wave has all ids, one per lane. A group's first row is the number of ids below it, a slot's
-// row the number of ids that sort before it: no histogram, scan or barrier. One token's 10 slots 2.4 us, launches back to back (8.2 with the
-// kernel below).
+// row the number of ids that sort before it: no histogram, scan or barrier. One token's 10 slots, launches back to back, 2.4 us (8.2 with
+// the kernel below).
 __global__ void __launch_bounds__(1024) k_sort_few(const int32_t* __restrict__ ids, int S, int K, int E, int32_t* __restrict__ bounds,
                                                    int32_t* __restrict__ tok_of, int32_t* __restrict__ slot_of,
                                                    int32_t* __restrict__ row_of) {
