@@ -62,6 +62,13 @@ SIGNATURES = {
     "frt_mx4_quantize": (_i, [_vp, _vp, _i64, _i, _i, _i, _vp, _vp]),
     "frt_mx4_dequantize": (_i, [_vp, _vp, _vp, _i, _i, _vp, _i64, _i]),
     "frt_mx4_product": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _i64, _i]),
+    "frt_moe_product": (_i, [_vp, _vp, _i64, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i64, _i]),
+    "frt_moe_product_grad": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i64, _i]),
+    "frt_moe_product_wgrad": (_i, [_vp, _vp, _i64, _vp, _i64, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _i]),
+    "frt_mx8_quantize": (_i, [_vp, _vp, _i64, _i, _i, _i, _vp, _vp]),
+    "frt_mx8_dequantize": (_i, [_vp, _vp, _vp, _i, _i, _vp, _i64, _i]),
+    "frt_moe_swiglu": (_i, [_vp, _vp, _i64, _i, _i, _i, _vp, _vp, _i64, _vp, _vp]),
+    "frt_moe_swiglu_grad": (_i, [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _i, _i, _i, _vp, _vp, _i64, _vp, _i64]),
     "frt_moe_q2_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "frt_moe_q2_run": (_i, [_vp, _sz, _i, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _sz, _vp, _i, _i]),
     "frt_moe_hits_scratch_bytes": (_sz, [_i, _i, _i]),

@@ -1,5 +1,6 @@
 // The C ABI (include/flashrt_moe.h): argument checks, workspace carving, error strings.
 #include "common.hpp"
+#include "product.hpp"
 
 #include "../../include/flashrt_moe.h"
 
@@ -181,6 +182,13 @@ int mx4_dequantize(int type, const void* codes, const void* scales, int64_t rows
                    hipStream_t stream);
 int mx4_product(const void* aq, const void* as, int a_rows, const int32_t* rows, const void* wq, const void* ws, const int32_t* bounds,
                 int E, int M, int N, int C, void* out, int type, int64_t ldout, hipStream_t stream);
+// mx8.hip
+int mx8_quantize(int type, const void* x, int64_t ldx, int64_t rows, int cols, void* codes, void* scales, hipStream_t stream);
+int mx8_dequantize(int type, const void* codes, const void* scales, int64_t rows, int cols, void* out, int64_t ldout, hipStream_t stream);
+int moe_swiglu(int type, const void* z, int64_t ldz, int64_t rows, int ff, const int32_t* live, void* h, int64_t ldh, void* codes,
+               void* scales, hipStream_t stream);
+int moe_swiglu_grad(int type, const void* dh, int64_t lddh, const void* z, int64_t ldz, const void* codes, const void* scales, int64_t rows,
+                    int ff, const int32_t* live, void* dz, int64_t lddz, void* h, int64_t ldh, hipStream_t stream);
 // decode.hip
 bool dec_shape_templated(int n, int ff);
 bool dec_shape_generic(int n, int ff);
@@ -489,6 +497,20 @@ static int codes_check(const char* what, const char* name, const void* codes, co
     if (reinterpret_cast<uintptr_t>(codes) % 16) return set_error(kErrShape, "%s: %s codes not 16-byte aligned", what, name);
     return kOk;
 }
+static int product_check(const char* what, int type, int out_type, const int32_t* bounds, int E, int M, int N, int C) {
+    if (int rc = type_check(what, type)) return rc;
+    if (int rc = type_check(what, out_type)) return rc;
+    if (M < 0 || M > (1 << 30) || N < 1 || N > (1 << 30) || C < 1 || C > (1 << 30))
+        return set_error(kErrShape, "%s: M=%d N=%d C=%d", what, M, N, C);
+    if (E < 1 || E > 4096 || (!bounds && E != 1)) return set_error(kErrShape, "%s: E=%d%s", what, E, bounds ? "" : " without bounds");
+    return bounds ? words_check(what, "bounds", bounds) : kOk;
+}
+static int swiglu_check(const char* what, int type, int rows, int ff, bool eight) {
+    if (int rc = type_check(what, type)) return rc;
+    if (rows < 0 || ff < 1 || ff > (1 << 29) || (eight && ff % 32))
+        return set_error(kErrShape, "%s: rows=%d ff=%d%s", what, rows, ff, eight ? " (in 8 bits a multiple of 32)" : "");
+    return kOk;
+}
 
 }  // namespace frt
 
@@ -722,6 +744,104 @@ int frt_mx4_product(void* stream, const void* aq, const void* asc, int a_rows, c
         if (int rc = words_check("mx4_product", "bounds", bounds)) return rc;
     if (int rc = rows_check("mx4_product", "out", out, ldout, N, type)) return rc;
     return mx4_product(aq, asc, a_rows, rows, wq, wsc, bounds, E, M, N, C, out, type, ldout, static_cast<hipStream_t>(stream));
+}
+
+int frt_moe_product(void* stream, const void* a, int64_t lda, int a_rows, const int32_t* rows, const void* w, const int32_t* bounds, int E,
+                    int M, int N, int C, int type, void* out, int64_t ldout, int out_type) {
+    if (int rc = product_check("moe_product", type, out_type, bounds, E, M, N, C)) return rc;
+    if (M == 0) return kOk;
+    if (a_rows < (rows ? 1 : M)) return set_error(kErrShape, "moe_product: %d rows of activations for M=%d", a_rows, M);
+    if (int rc = rows_check("moe_product", "a", a, lda, C, type)) return rc;
+    if (int rc = rows_check("moe_product", "w", w, C, C, type)) return rc;
+    if (rows)
+        if (int rc = words_check("moe_product", "rows", rows)) return rc;
+    if (int rc = rows_check("moe_product", "out", out, ldout, N, out_type)) return rc;
+    return moe_product(type, ProductArgs{a, lda, w, C, nullptr, a_rows, rows, bounds, E, M, N, C, out, ldout, out_type, 0},
+                       static_cast<hipStream_t>(stream));
+}
+
+int frt_moe_product_grad(void* stream, const void* dout, int64_t lddout, const void* w, const int32_t* bounds, int E, int M, int N, int C,
+                         int type, void* da, int64_t ldda, int da_type) {
+    if (int rc = product_check("moe_product_grad", type, da_type, bounds, E, M, N, C)) return rc;
+    if (M == 0) return kOk;
+    if (int rc = rows_check("moe_product_grad", "dout", dout, lddout, N, type)) return rc;
+    if (int rc = rows_check("moe_product_grad", "w", w, C, C, type)) return rc;
+    if (int rc = rows_check("moe_product_grad", "da", da, ldda, C, da_type)) return rc;
+    return moe_product_grad(type, ProductArgs{dout, lddout, w, C, nullptr, M, nullptr, bounds, E, M, N, C, da, ldda, da_type, 0},
+                            static_cast<hipStream_t>(stream));
+}
+
+int frt_moe_product_wgrad(void* stream, const void* dout, int64_t lddout, const void* a, int64_t lda, const void* a_scales, int a_rows,
+                          const int32_t* rows, const int32_t* bounds, int E, int M, int N, int C, int type, void* dw, int dw_type, int add) {
+    if (int rc = product_check("moe_product_wgrad", type, dw_type, bounds, E, M, N, C)) return rc;
+    if (M > 0) {
+        if (a_rows < (rows ? 1 : M)) return set_error(kErrShape, "moe_product_wgrad: %d rows of activations for M=%d", a_rows, M);
+        if (int rc = rows_check("moe_product_wgrad", "dout", dout, lddout, N, type)) return rc;
+        if (a_scales) {
+            if (C % 32 || lda != C) return set_error(kErrShape, "moe_product_wgrad: 8-bit rows C=%d (a multiple of 32), %lld apart", C, (long long)lda);
+            if (int rc = codes_check("moe_product_wgrad", "activations", a, a_scales)) return rc;
+        } else if (int rc = rows_check("moe_product_wgrad", "a", a, lda, C, type)) {
+            return rc;
+        }
+        if (rows)
+            if (int rc = words_check("moe_product_wgrad", "rows", rows)) return rc;
+    }
+    if (int rc = rows_check("moe_product_wgrad", "dw", dw, C, C, dw_type)) return rc;
+    return moe_product_wgrad(type,
+                             ProductArgs{dout, lddout, a, lda, static_cast<const uint8_t*>(a_scales), a_rows, rows, bounds, E, M, N, C, dw, C, dw_type,
+                                         add != 0},
+                             static_cast<hipStream_t>(stream));
+}
+
+int frt_mx8_quantize(void* stream, const void* x, int64_t ldx, int type, int rows, int cols, void* codes, void* scales) {
+    if (int rc = type_check("mx8_quantize", type)) return rc;
+    if (rows < 0 || cols < 32 || cols % 32) return set_error(kErrShape, "mx8_quantize: rows=%d cols=%d (a multiple of 32)", rows, cols);
+    if (rows == 0) return kOk;
+    if (int rc = rows_check("mx8_quantize", "x", x, ldx, cols, type)) return rc;
+    if (int rc = codes_check("mx8_quantize", "output", codes, scales)) return rc;
+    return mx8_quantize(type, x, ldx, rows, cols, codes, scales, static_cast<hipStream_t>(stream));
+}
+
+int frt_mx8_dequantize(void* stream, const void* codes, const void* scales, int rows, int cols, void* out, int64_t ldout, int type) {
+    if (int rc = type_check("mx8_dequantize", type)) return rc;
+    if (rows < 0 || cols < 32 || cols % 32) return set_error(kErrShape, "mx8_dequantize: rows=%d cols=%d (a multiple of 32)", rows, cols);
+    if (rows == 0) return kOk;
+    if (int rc = codes_check("mx8_dequantize", "input", codes, scales)) return rc;
+    if (int rc = rows_check("mx8_dequantize", "out", out, ldout, cols, type)) return rc;
+    return mx8_dequantize(type, codes, scales, rows, cols, out, ldout, static_cast<hipStream_t>(stream));
+}
+
+int frt_moe_swiglu(void* stream, const void* z, int64_t ldz, int type, int rows, int ff, const int32_t* live, void* h, int64_t ldh,
+                   void* codes, void* scales) {
+    if (int rc = swiglu_check("moe_swiglu", type, rows, ff, codes || scales)) return rc;
+    if (rows == 0) return kOk;
+    if (int rc = rows_check("moe_swiglu", "z", z, ldz, 2 * ff, type)) return rc;
+    if (int rc = rows_check("moe_swiglu", "h", h, ldh, ff, type)) return rc;
+    if (codes || scales)
+        if (int rc = codes_check("moe_swiglu", "output", codes, scales)) return rc;
+    if (live)
+        if (int rc = words_check("moe_swiglu", "live", live)) return rc;
+    return moe_swiglu(type, z, ldz, rows, ff, live, h, ldh, codes, scales, static_cast<hipStream_t>(stream));
+}
+
+int frt_moe_swiglu_grad(void* stream, const void* dh, int64_t lddh, const void* z, int64_t ldz, const void* codes, const void* scales,
+                        int type, int rows, int ff, const int32_t* live, void* dz, int64_t lddz, void* h, int64_t ldh) {
+    const bool kept = codes || scales;
+    if (int rc = swiglu_check("moe_swiglu_grad", type, rows, ff, kept)) return rc;
+    if (z && kept) return set_error(kErrShape, "moe_swiglu_grad: z and its 8-bit form");
+    if (rows == 0) return kOk;
+    if (int rc = rows_check("moe_swiglu_grad", "dh", dh, lddh, ff, type)) return rc;
+    if (kept) {
+        if (int rc = codes_check("moe_swiglu_grad", "input", codes, scales)) return rc;
+    } else if (int rc = rows_check("moe_swiglu_grad", "z", z, ldz, 2 * ff, type)) {
+        return rc;
+    }
+    if (int rc = rows_check("moe_swiglu_grad", "dz", dz, lddz, 2 * ff, type)) return rc;
+    if (h)
+        if (int rc = rows_check("moe_swiglu_grad", "h", h, ldh, ff, type)) return rc;
+    if (live)
+        if (int rc = words_check("moe_swiglu_grad", "live", live)) return rc;
+    return moe_swiglu_grad(type, dh, lddh, z, ldz, codes, scales, rows, ff, live, dz, lddz, h, ldh, static_cast<hipStream_t>(stream));
 }
 
 size_t frt_moe_q2_workspace_bytes(int T, int K, int n, int ff, int E) {

@@ -26,7 +26,8 @@ __all__ = ["FrtError", "ExpertArena", "arena_alloc", "arena_free", "moe_route_to
            "moe_dispatch", "moe_q2", "moe_hits_scratch_bytes", "moe_hits", "MoeLayer", "expert_bytes", "gen",
            "set_option", "layer_sync_error", "MoeStack", "noalloc_scratch_bytes", "q2_repack",
            "q2_repack_expert", "load_experts", "moe_sort", "moe_permute", "moe_permute_grad", "moe_unpermute",
-           "moe_unpermute_grad", "mx4_quantize", "mx4_dequantize", "mx4_product"]
+           "moe_unpermute_grad", "mx4_quantize", "mx4_dequantize", "mx4_product", "moe_product", "moe_product_grad", "moe_product_wgrad",
+           "mx8_quantize", "mx8_dequantize", "moe_swiglu", "moe_swiglu_grad"]
 
 
 def _p(t) -> int | None:
@@ -307,6 +308,116 @@ def mx4_product(aq, asc, wq, wsc, out, bounds=None, rows=None, stream=None) -> N
              _flat(wsc, E * N * C // 32, u8, dev, "wsc"), None if bounds is None else _flat(bounds, E + 1, i32, dev, "bounds"), E, M, N, C,
              out.data_ptr(), _rows(out, M, N, out, dev, "out"), _type(out, "out"))
     increment_version(out)
+
+
+def _experts(w, like, dev: int, what: str) -> tuple:
+    """(address, E, N, C) of contiguous matrices [E][N][C] (or one, [N][C]) on GPU dev, of like's type where that is given."""
+    if w.requires_grad:
+        _untracked(w, what)
+    sw = w.shape
+    if len(sw) not in (2, 3):
+        raise ValueError(f"{what}: expected [E][N][C] or [N][C], got {list(sw)}")
+    return _flat(w, w.numel(), w.dtype if like is None else like.dtype, dev, what), sw[0] if len(sw) == 3 else 1, sw[-2], sw[-1]
+
+
+def _group_list(bounds, E: int, dev: int):
+    return None if bounds is None else _flat(bounds, E + 1, torch.int32, dev, "bounds")
+
+
+def moe_product(a, w, out, bounds=None, rows=None, stream=None) -> None:
+    """frt_moe_product: out[r] = w_g a(r) for the rows r of group g (bounds[g] .. bounds[g + 1], int32; without bounds all rows and
+    one group). a [a_rows][C] and w [E][N][C] (or [N][C]) of one type, out [M][N] of any; rows (M int32): a(r) is row rows[r] of a
+    instead of r."""
+    dev = out.get_device()
+    pw, E, N, C = _experts(w, a, dev, "w")
+    M, a_rows = out.shape[0], a.shape[0]
+    _enqueue(lib().frt_moe_product, dev, stream, a.data_ptr(), _rows(a, a_rows, C, a, dev, "a"), a_rows,
+             None if rows is None else _flat(rows, M, torch.int32, dev, "rows"), pw, _group_list(bounds, E, dev), E, M, N, C, _type(a, "a"),
+             out.data_ptr(), _rows(out, M, N, out, dev, "out"), _type(out, "out"))
+    increment_version(out)
+
+
+def moe_product_grad(dout, w, da, bounds=None, stream=None) -> None:
+    """frt_moe_product_grad: the gradient of moe_product by its rows, da[r] = w_g^T dout[r]; dout [M][N] and w [E][N][C] (or
+    [N][C]) of one type, da [M][C] of any. With rows picked these are the picked rows' gradients (moe_permute_grad sums a token's)."""
+    dev = da.get_device()
+    pw, E, N, C = _experts(w, dout, dev, "w")
+    M = da.shape[0]
+    _enqueue(lib().frt_moe_product_grad, dev, stream, dout.data_ptr(), _rows(dout, M, N, dout, dev, "dout"), pw, _group_list(bounds, E, dev), E,
+             M, N, C, _type(dout, "dout"), da.data_ptr(), _rows(da, M, C, da, dev, "da"), _type(da, "da"))
+    increment_version(da)
+
+
+def moe_product_wgrad(dout, a, dw, bounds=None, rows=None, add: bool = False, stream=None) -> None:
+    """frt_moe_product_wgrad: the gradient of moe_product by its weights, dw_g = the sum of dout[r] a(r)^T over the group's rows (plus
+    what was there, with add). dout [M][N] and a [a_rows][C] of one type, dw [E][N][C] (or [N][C]) of any; a may be the pair (codes,
+    scales) that mx8_quantize wrote: int8 [a_rows][C] and uint8 a_rows * C / 32."""
+    dev = dw.get_device()
+    pw, E, N, C = _experts(dw, None, dev, "dw")
+    M = dout.shape[0]
+    if isinstance(a, (tuple, list)):
+        a, scales = a
+        a_rows = a.shape[0]
+        if a.shape != (a_rows, C):
+            raise ValueError(f"a: expected codes [{a_rows}][{C}], got {list(a.shape)}")
+        pa, lda, ps = _flat(a, a_rows * C, torch.int8, dev, "codes"), C, _flat(scales, a_rows * C // 32, torch.uint8, dev, "scales")
+    else:
+        a_rows = a.shape[0]
+        pa, lda, ps = a.data_ptr(), _rows(a, a_rows, C, dout, dev, "a"), None
+    _enqueue(lib().frt_moe_product_wgrad, dev, stream, dout.data_ptr(), _rows(dout, M, N, dout, dev, "dout"), pa, lda, ps, a_rows,
+             None if rows is None else _flat(rows, M, torch.int32, dev, "rows"), _group_list(bounds, E, dev), E, M, N, C, _type(dout, "dout"), pw,
+             _type(dw, "dw"), 1 if add else 0)
+    increment_version(dw)
+
+
+def _codes8(codes, scales, rows: int, cols: int, dev: int) -> tuple:
+    """The addresses of 8-bit codes (int8 [rows][cols]) and their scales (uint8, one per 32)."""
+    return _flat(codes, rows * cols, torch.int8, dev, "codes"), _flat(scales, rows * cols // 32, torch.uint8, dev, "scales")
+
+
+def mx8_quantize(x, codes, scales, stream=None) -> None:
+    """frt_mx8_quantize: x [rows][cols] in 8 bits, codes rows * cols int8 and scales rows * cols / 32 uint8."""
+    (rows, cols), dev = x.shape, x.get_device()
+    _enqueue(lib().frt_mx8_quantize, dev, stream, x.data_ptr(), _rows(x, rows, cols, x, dev, "x"), _type(x, "x"), rows, cols,
+             *_codes8(codes, scales, rows, cols, dev))
+    increment_version((codes, scales))
+
+
+def mx8_dequantize(codes, scales, out, stream=None) -> None:
+    """frt_mx8_dequantize: the values of 8-bit codes and scales into out [rows][cols]."""
+    (rows, cols), dev = out.shape, out.get_device()
+    _enqueue(lib().frt_mx8_dequantize, dev, stream, *_codes8(codes, scales, rows, cols, dev), rows, cols, out.data_ptr(),
+             _rows(out, rows, cols, out, dev, "out"), _type(out, "out"))
+    increment_version(out)
+
+
+def moe_swiglu(z, h, codes=None, scales=None, live=None, stream=None) -> None:
+    """frt_moe_swiglu: h = silu(gate) up of rows z [rows][2 ff] = gate | up; with codes (rows * 2 ff int8) and scales (rows * ff / 16
+    uint8) z is also written in 8 bits. live (one int32, e.g. bounds[-1:]): the number of rows that count, the others stay as they were."""
+    (rows, ff), dev = h.shape, h.get_device()
+    pc, ps = (None, None) if codes is None and scales is None else _pair(codes, scales, rows, ff, dev)
+    _enqueue(lib().frt_moe_swiglu, dev, stream, z.data_ptr(), _rows(z, rows, 2 * ff, z, dev, "z"), _type(z, "z"), rows, ff,
+             None if live is None else _flat(live, 1, torch.int32, dev, "live"), h.data_ptr(), _rows(h, rows, ff, z, dev, "h"), pc, ps)
+    increment_version(h if codes is None else (h, codes, scales))
+
+
+def _pair(codes, scales, rows: int, ff: int, dev: int) -> tuple:
+    if codes is None or scales is None:
+        raise ValueError("codes and scales: expected both or neither")
+    return _codes8(codes, scales, rows, 2 * ff, dev)
+
+
+def moe_swiglu_grad(dh, dz, z=None, codes=None, scales=None, h=None, live=None, stream=None) -> None:
+    """frt_moe_swiglu_grad: the gradient dz [rows][2 ff] of moe_swiglu from dh [rows][ff] and z, or z's codes and scales; h [rows][ff],
+    where given: h again, of the z that was read. live as in moe_swiglu."""
+    (rows, ff), dev = dh.shape, dh.get_device()
+    if (z is None) == (codes is None and scales is None):
+        raise ValueError("moe_swiglu_grad: expected z, or its codes and scales")
+    pz, ldz, (pc, ps) = (None, 0, _pair(codes, scales, rows, ff, dev)) if z is None else (z.data_ptr(), _rows(z, rows, 2 * ff, dh, dev, "z"), (None, None))
+    _enqueue(lib().frt_moe_swiglu_grad, dev, stream, dh.data_ptr(), _rows(dh, rows, ff, dh, dev, "dh"), pz, ldz, pc, ps, _type(dh, "dh"), rows, ff,
+             None if live is None else _flat(live, 1, torch.int32, dev, "live"), dz.data_ptr(), _rows(dz, rows, 2 * ff, dh, dev, "dz"),
+             None if h is None else h.data_ptr(), 0 if h is None else _rows(h, rows, ff, dh, dev, "h"))
+    increment_version(dz if h is None else (dz, h))
 
 
 # ---------------------------------------------------------------- prefill grouped GEMM

@@ -189,6 +189,46 @@ int frt_mx4_dequantize(void* stream, const void* codes, const void* scales, int 
 int frt_mx4_product(void* stream, const void* aq, const void* asc, int a_rows, const int32_t* rows, const void* wq,
                     const void* wsc, const int32_t* bounds, int E, int M, int N, int C, void* out, int64_t ldout, int type);
 
+/* ---- products of the sorted rows with their experts' matrices, and both gradients (no reference counterpart: its experts are Q2_0, and it
+ * does not train). Operands of type FRT_GGML_F32, F16 or BF16 (both the same), results of any of the three; sums in fp32, rounded once.
+ * Group g < E <= 4096 has the rows r in [bounds[g], bounds[g+1]); bounds (frt_moe_sort's) ascend within [0, M], NULL: one group (E = 1) of M
+ * rows. Rows of no group stay as they were. a(r) is row r of a, or row rows[r] where rows is given (frt_moe_sort's tok_of); an index
+ * outside [0, a_rows) gives a row of zeros. Weights w and dw are [E][N][C]; rows of a, out, dout and da lie ld* elements apart.
+ * M (may be 0), N and C up to 2^30; a_rows >= M, or >= 1 with rows. Inputs and outputs must not overlap.
+ *   product        out[r][j] = sum_k w_g[j][k] a(r)[k], j < N
+ *   product_grad   da[r][k] = sum_j dout[r][j] w_g[j][k], k < C (a sorted row's gradient: frt_moe_permute_grad sums a token's)
+ *   product_wgrad  dw_g[j][k] = sum over the group's rows of dout[r][j] a(r)[k], with add plus what was there; a group without rows has 0 (with
+ *                  add it stays as it was). With a_scales a is in 8 bits (frt_mx8_quantize's codes, lda = C a multiple of 32, and
+ *                  scales): its values, rounded to the type. */
+int frt_moe_product(void* stream, const void* a, int64_t lda, int a_rows, const int32_t* rows, const void* w, const int32_t* bounds, int E,
+                    int M, int N, int C, int type, void* out, int64_t ldout, int out_type);
+int frt_moe_product_grad(void* stream, const void* dout, int64_t lddout, const void* w, const int32_t* bounds, int E, int M, int N, int C,
+                         int type, void* da, int64_t ldda, int da_type);
+int frt_moe_product_wgrad(void* stream, const void* dout, int64_t lddout, const void* a, int64_t lda, const void* a_scales, int a_rows,
+                          const int32_t* rows, const int32_t* bounds, int E, int M, int N, int C, int type, void* dw, int dw_type, int add);
+
+/* ---- activations kept in 8 bits for the backward pass (no reference counterpart). Each 32 consecutive values of a row share a scale
+ * byte b, the power of two 2^(b - 127) (255: NaN), and are signed 8-bit codes: codes [rows][cols], 16-byte aligned; scales
+ * [rows][cols/32]. cols is a multiple of 32. rows may be 0.
+ * frt_mx8_quantize: x of type FRT_GGML_F32 / F16 / BF16, rows ldx elements apart. With a block's largest magnitude m 2^k (1 <= m < 2),
+ * b = max(k - 6, -127) + 127 and a code is x 2^(127 - b) rounded to nearest even, held within -127 .. 127; a block of zeros has b = 0; a
+ * block with an infinity or a NaN has b = 255 and codes 0 (all its values read NaN).
+ * frt_mx8_dequantize: the values, rounded to nearest even where the type cannot hold them.
+ * ---- the experts' gated activation on rows z [rows][2 ff] = gate | up, and its backward pass from z or from z in 8 bits:
+ *   swiglu       h = g s(g) u, s(g) = 1 / (1 + exp(-g)), in fp32, rounded once; with codes and scales (ff then a multiple of 32) z is also
+ *                written in 8 bits, as frt_mx8_quantize would
+ *   swiglu_grad  dz = dg | du, dg = dh u s (1 + g (1 - s)), du = dh g s, from z or from codes and scales (one of them NULL); h (may be NULL):
+ *                h again, of the z that was read
+ * Rows ld* elements apart; ff up to 2^29. live (NULL: all rows): one int32 on the device, the number of rows that count (bounds + E of a
+ * sort); the others stay as they were. Inputs and outputs must not overlap. */
+int frt_mx8_quantize(void* stream, const void* x, int64_t ldx, int type, int rows, int cols, void* codes, void* scales);
+int frt_mx8_dequantize(void* stream, const void* codes, const void* scales, int rows, int cols, void* out, int64_t ldout,
+                       int type);
+int frt_moe_swiglu(void* stream, const void* z, int64_t ldz, int type, int rows, int ff, const int32_t* live, void* h, int64_t ldh,
+                   void* codes, void* scales);
+int frt_moe_swiglu_grad(void* stream, const void* dh, int64_t lddh, const void* z, int64_t ldz, const void* codes, const void* scales,
+                        int type, int rows, int ff, const int32_t* live, void* dz, int64_t lddz, void* h, int64_t ldh);
+
 /* ---- prefill grouped expert GEMM (kernels/cuda/moe_q2.h:20-30 moe_q2::workspace_bytes, run).
  * yd [T*K][n]: slot t*K + k gets down(silu(gate x_t) * up x_t) of expert ids[t*K + k], expert e's
  * blob at experts + e * stride (both multiples of 16: blobs are read in pieces of 16 bytes; an arena's

@@ -503,6 +503,41 @@ inline void product(hipStream_t stream, const void* aq, const void* asc, int a_r
     detail::check(frt_mx4_product(stream, aq, asc, a_rows, rows, wq, wsc, bounds, E, M, N, C, out, ldout, type), "mx4::product");
 }
 }  // namespace mx4
+
+// ---- products of the sorted rows with their experts' matrices and both gradients; activations kept in 8 bits, and the experts' gated
+// activation that writes and reads them (flashrt_moe.h states each call)
+inline void moe_product(hipStream_t stream, const void* a, int64_t lda, int a_rows, const int32_t* rows, const void* w, const int32_t* bounds,
+                        int E, int M, int N, int C, int type, void* out, int64_t ldout, int out_type) {
+    detail::check(frt_moe_product(stream, a, lda, a_rows, rows, w, bounds, E, M, N, C, type, out, ldout, out_type), "moe_product");
+}
+inline void moe_product_grad(hipStream_t stream, const void* dout, int64_t lddout, const void* w, const int32_t* bounds, int E, int M, int N,
+                             int C, int type, void* da, int64_t ldda, int da_type) {
+    detail::check(frt_moe_product_grad(stream, dout, lddout, w, bounds, E, M, N, C, type, da, ldda, da_type), "moe_product_grad");
+}
+inline void moe_product_wgrad(hipStream_t stream, const void* dout, int64_t lddout, const void* a, int64_t lda, const void* a_scales, int a_rows,
+                              const int32_t* rows, const int32_t* bounds, int E, int M, int N, int C, int type, void* dw, int dw_type,
+                              bool add = false) {
+    detail::check(frt_moe_product_wgrad(stream, dout, lddout, a, lda, a_scales, a_rows, rows, bounds, E, M, N, C, type, dw, dw_type, add ? 1 : 0),
+                  "moe_product_wgrad");
+}
+inline void moe_swiglu(hipStream_t stream, const void* z, int64_t ldz, int type, int rows, int ff, const int32_t* live, void* h, int64_t ldh,
+                       void* codes = nullptr, void* scales = nullptr) {
+    detail::check(frt_moe_swiglu(stream, z, ldz, type, rows, ff, live, h, ldh, codes, scales), "moe_swiglu");
+}
+inline void moe_swiglu_grad(hipStream_t stream, const void* dh, int64_t lddh, const void* z, int64_t ldz, const void* codes, const void* scales,
+                            int type, int rows, int ff, const int32_t* live, void* dz, int64_t lddz, void* h = nullptr, int64_t ldh = 0) {
+    detail::check(frt_moe_swiglu_grad(stream, dh, lddh, z, ldz, codes, scales, type, rows, ff, live, dz, lddz, h, ldh), "moe_swiglu_grad");
+}
+
+namespace mx8 {
+inline void quantize(hipStream_t stream, const void* x, int64_t ldx, int type, int rows, int cols, void* codes, void* scales) {
+    detail::check(frt_mx8_quantize(stream, x, ldx, type, rows, cols, codes, scales), "mx8::quantize");
+}
+inline void dequantize(hipStream_t stream, const void* codes, const void* scales, int rows, int cols, void* out, int64_t ldout,
+                       int type) {
+    detail::check(frt_mx8_dequantize(stream, codes, scales, rows, cols, out, ldout, type), "mx8::dequantize");
+}
+}  // namespace mx8
 }  // namespace flashrt
 
 #endif
