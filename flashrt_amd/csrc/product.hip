@@ -46,17 +46,23 @@ __device__ __forceinline__ f16_t mma(Vec<float> y, Vec<float> x, f16_t acc) {
     return acc;
 }
 
-// A stage of an operand in LDS: W rows (or columns) of 128 bytes of contracted values, eight chunks of which step t takes 2 t and 2 t + 1 (one
-// per lane half). ROW: [W][128 bytes], chunk c of row r at c ^ (r / 2 % 8), so that the sixteen rows of a read phase take sixteen different
-// columns of the banks. COL: [128 / sizeof(T)][W], the contracted values apart: chunks of 16 bits are read by the transposing LDS read, four
+// Four 16-bit values of sixteen columns. (Without __restrict, here and at the direct loads, the compiler has these reads wait for every direct
+// load under way, which might write what they read; the waits in the code see to that.)
+__device__ __forceinline__ s4_t read_tr(const uint8_t* __restrict s) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)const_cast<uint8_t*>(s));
+}
+
+// A stage of an operand in LDS: W rows (or columns) of KB chunks of contracted values, of which step t takes 2 t and 2 t + 1 (one per lane
+// half). ROW: [W][KB chunks], chunk c of row r at c ^ (r / (16 / KB) % KB), so that the sixteen rows of a read phase take sixteen different
+// columns of the banks. COL: [KB V][W], the contracted values apart: chunks of 16 bits are read by the transposing LDS read, four
 // values of sixteen columns at a time (a lane's address is a quarter of one row's 32 bytes), 32-bit ones value by value; 32-byte
 // blocks of rows that a read takes together lie in different banks.
-template <typename T, int W, bool COL>
+template <typename T, int W, bool COL, int KB>
 struct Stage {
-    static constexpr int V = Chunk<T>::V, BK = 128 / int(sizeof(T)), bytes = W * 128;
-    static constexpr int row_b = COL ? W * int(sizeof(T)) : 128, PR = row_b / 16;   // bytes and pieces of a stored row
+    static constexpr int V = Chunk<T>::V, BK = KB * V, bytes = W * KB * 16;
+    static constexpr int row_b = COL ? W * int(sizeof(T)) : KB * 16, PR = row_b / 16;   // bytes and pieces of a stored row
     static constexpr int Q = row_b < 256 ? 256 / row_b : 1;
-    static __device__ __forceinline__ int swizzle(int r) { return COL ? ((r / Q & 3) << 2) & (PR - 1) : r / 2 % 8; }
+    static __device__ __forceinline__ int swizzle(int r) { return COL ? ((r / Q & 3) << 2) & (PR - 1) : r / Q % KB; }
     static __device__ __forceinline__ int piece(int r, int p) { return r * row_b + ((p ^ swizzle(r)) << 4); }
     // The lane's chunk of step t of rows (columns) w0 .. w0 + 31
     static __device__ __forceinline__ Vec<T> read(const uint8_t* s, int w0, int t) {
@@ -72,10 +78,9 @@ struct Stage {
             }
             return v;
         } else {
-            typedef __attribute__((address_space(3))) s4_t* lds4;
             const int b = (w0 + (lane & 16) + (lane & 3) * 4) * 2, k = c * V + ((lane & 15) >> 2);
-            const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(s + piece(k, b >> 4) + (b & 15)));
-            const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(s + piece(k + 4, b >> 4) + (b & 15)));
+            const s4_t lo = read_tr(s + piece(k, b >> 4) + (b & 15));
+            const s4_t hi = read_tr(s + piece(k + 4, b >> 4) + (b & 15));
             return __builtin_bit_cast(Vec<T>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
     }
@@ -134,8 +139,8 @@ template <typename T, Mode MODE, bool EIGHT, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN) k_product_any(ProductArgs p, int nx, int ny, FastDiv divx, FastDiv divy) {
     constexpr int NT = 64 * WM * WN, V = Chunk<T>::V, FM = BM / WM / 32, FN = BN / WN / 32;
     constexpr bool XCOL = MODE == kWgrad, YCOL = MODE != kProduct;
-    using SX = Stage<T, BM, XCOL>;
-    using SY = Stage<T, BN, YCOL>;
+    using SX = Stage<T, BM, XCOL, 8>;
+    using SY = Stage<T, BN, YCOL, 8>;
     constexpr int PX = BM * 8 / NT, PY = BN * 8 / NT, BK = SX::BK;
     static_assert(BM * 8 % NT == 0 && BN * 8 % NT == 0, "whole pieces per thread");
     __shared__ __align__(16) uint8_t s_x[SX::bytes], s_y[SY::bytes];
@@ -268,16 +273,459 @@ static int any_go(const char* what, const ProductArgs& p, hipStream_t stream) {
     return kOk;
 }
 
+// ---------------------------------------------------------------- tiles through direct loads
+typedef __amdgpu_buffer_rsrc_t Buffer;
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+typedef int i4_t __attribute__((ext_vector_type(4)));
+// An offset past every buffer's bytes: a load of it gives zeros, a store nothing
+constexpr uint32_t kNone = 0x80000000u;
+__device__ __forceinline__ Buffer buffer(const uint8_t* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, 0x7fffffff, 0x00020000);
+}
+// Direct load of 16 bytes per lane, from base + off + step, to lds + 16 lane (AUX 2: not kept in L2)
+template <int AUX>
+__device__ __forceinline__ void load16(Buffer base, uint32_t off, uint32_t step, uint8_t* __restrict lds) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (lds_ptr_t)lds, 16, off, step, 0, AUX);
+}
+
+// An operand's stages: its pieces (16 bytes, 8 values) go straight into LDS, D loads of 64 pieces per wave and stage, RL stored rows each
+template <typename T, int W, bool COL, int KB, int NW>
+struct Loads {
+    using S = Stage<T, W, COL, KB>;
+    static constexpr int D = W * KB / 64 / NW, RL = 64 / S::PR;
+    static_assert(W * KB % (64 * NW) == 0, "every wave the same loads");
+    static __device__ __forceinline__ int row(int load) { return load * RL + (threadIdx.x & 63) / S::PR; }   // the lane's stored row in it
+    static __device__ __forceinline__ int piece(int load) { return ((threadIdx.x & 63) % S::PR) ^ S::swizzle(row(load)); }
+};
+
+template <int BM, int BN, int NW, int ST, int KB, int OR>
+struct TileShape {
+    static constexpr int stage_b = (BM + BN) * KB * 16, out_b = OR * 128;   // (a wave's results, OR rows of 128 bytes at a time)
+    static constexpr int smem = ST * stage_b + NW * out_b;
+    static_assert(smem <= 160 * 1024, "LDS of a CU");
+};
+
+// A wave's LDS accesses before are done before those after, across its lanes (they complete in order)
+__device__ __forceinline__ void wave_lds_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+}
+// A uniform load through the scalar cache's counter, which the waits on vector loads do not count
+__device__ __forceinline__ int uniform_load(const int32_t* p) { return *(const __attribute__((address_space(4))) int32_t*)p; }
+
+struct TileGrid {
+    int ny, per, nx;         // feature tiles, of a workgroup, row tiles (wgrad)
+    int stream;              // weights that one row tile reads are not kept in L2
+    uint32_t nchunk;
+    FastDiv blocks, divx;
+};
+constexpr int RB = 4;        // row tiles of a block
+// (lambdas of several calls: left to itself the compiler calls the largest, and what they capture goes to memory)
+#define INLINE __attribute__((always_inline))
+
+template <typename T, Mode MODE, int BM, int BN, int WM, int WN, int ST, int KB, int OR, int OCC>
+__global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs p, TileGrid grid) {
+    constexpr int NW = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32, BK = KB * 8, SP = KB / 2;
+    constexpr bool XCOL = MODE == kWgrad, YCOL = MODE != kProduct;
+    using Sh = TileShape<BM, BN, NW, ST, KB, OR>;
+    using LX = Loads<T, BM, XCOL, KB, NW>;
+    using LY = Loads<T, BN, YCOL, KB, NW>;
+    constexpr int DX = LX::D, DY = LY::D, D = DX + DY;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    // Workgroup b runs on XCD b % 8. Each XCD takes an eighth of the row tiles, neighbours, in blocks of RB with their chunks of features: what
+    // runs at once on it reads few different rows of either operand. Where eighths would leave more than a ninth of the chip idle,
+    // the blocks go over all XCDs.
+    int g, x0, xn, K, k_first = 0, chunk = 0;
+    auto order = [&](uint32_t i, int tiles) INLINE {   // the row tile of workgroup i of those of that many row tiles (-1: none), and its chunk
+        uint32_t block = grid.blocks(i), in = i - block * (RB * grid.nchunk), rows = RB;
+        if (int(block) >= tiles / RB) {   // (the last block has fewer rows)
+            in += (block - tiles / RB) * (RB * grid.nchunk);
+            block = tiles / RB;
+            rows = max(tiles % RB, 1);
+        }
+        chunk = int(in / rows);
+        return chunk < int(grid.nchunk) && int(block * RB) < tiles ? int(block * RB + in % rows) : -1;
+    };
+    auto which = [&](int total) INLINE {
+        const int each = (total + 7) / 8;
+        if (each * 8 - total > total / 8) return order(blockIdx.x, total);
+        const int first = int(blockIdx.x & 7) * each, j = order(blockIdx.x >> 3, max(0, min(each, total - first)));
+        return j < 0 ? -1 : first + j;
+    };
+    bool once = grid.stream;
+    if constexpr (MODE == kWgrad) {
+        // (the groups' sizes differ, and with them their tiles' work: the row tiles go round the XCDs)
+        const int xcd = blockIdx.x & 7, j = order(blockIdx.x >> 3, (p.E * grid.nx - xcd + 7) / 8), index = j * 8 + xcd;
+        if (j < 0) return;
+        g = int(grid.divx(uint32_t(index)));
+        x0 = (index - g * grid.nx) * BM;
+        xn = min(BM, p.N - x0);
+        k_first = p.bounds ? min(max(p.bounds[g], 0), p.M) : 0;
+        K = max(0, (p.bounds ? min(max(p.bounds[g + 1], 0), p.M) : p.M) - k_first);
+        if (K == 0 && p.add) return;
+    } else {
+        const RowTile t = find_tile<BM>(p.bounds, p.E, p.M, which);
+        if (t.rows == 0) return;
+        g = t.g;
+        x0 = t.row0;
+        xn = t.rows;
+        K = MODE == kProduct ? p.C : p.N;
+        once = once && t.only;
+    }
+    const int features = MODE == kProduct ? p.N : p.C, nst = max(1, (K + BK - 1) / BK);
+    int ft = chunk * grid.per;
+    const int ft1 = min(ft + grid.per, grid.ny);
+    const bool gather = MODE == kWgrad && p.rows;
+
+    // Where the lane's pieces come from: offsets from a base that moves from stage to stage. ROW operands: one per load, none where there is
+    // no such row. COL ones: the lane's first row and column (none past the last column), a load's rows by a uniform step.
+    const uint8_t *xb, *yb, *y0;
+    uint32_t xo[XCOL ? 2 : DX], yo[YCOL ? 2 : DY];
+    uint32_t xstep, ystep;   // from row to row, in bytes
+    xstep = uint32_t(p.ldx * 2);
+    ystep = uint32_t((MODE == kWgrad ? p.ldy : int64_t(p.C)) * 2);
+    if constexpr (XCOL) {
+        xb = static_cast<const uint8_t*>(p.x) + (int64_t(k_first) * p.ldx + x0) * 2;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int c = LX::piece(wave * DX + i) * 8;
+            xo[i] = x0 + c < p.N ? lane / LX::S::PR * xstep + c * 2 : kNone;
+        }
+    } else {
+        xb = static_cast<const uint8_t*>(p.x) + (p.rows ? 0 : x0 * p.ldx * 2);
+#pragma unroll
+        for (int i = 0; i < DX; ++i) {
+            const int r = LX::row(wave * DX + i);
+            uint32_t a = r;
+            bool in = r < xn;
+            if (p.rows) {
+                a = uint32_t(p.rows[x0 + min(r, xn - 1)]);
+                in = in && a < uint32_t(p.a_rows);
+            }
+            xo[i] = in ? a * xstep + LX::piece(wave * DX + i) * 16 : kNone;
+        }
+    }
+    if constexpr (MODE == kWgrad)
+        y0 = static_cast<const uint8_t*>(p.y) + (gather ? 0 : int64_t(k_first) * p.ldy * 2);
+    else
+        y0 = static_cast<const uint8_t*>(p.y) + int64_t(g) * p.N * p.C * 2;
+    const uint8_t* const x0b = xb;
+    int jf = ft, jst = 0, jslot = 0;   // the next stage to load: of feature tile jf, into slot jslot
+    auto point = [&]() INLINE {
+        xb = x0b;
+        if constexpr (YCOL) {
+            yb = y0 + int64_t(jf) * BN * 2;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int c = LY::piece(wave * DY + i) * 8;
+                yo[i] = jf * BN + c < p.C ? (gather ? 0 : lane / LY::S::PR * ystep) + c * 2 : kNone;
+            }
+        } else {
+            yb = y0 + int64_t(jf) * BN * p.C * 2;
+#pragma unroll
+            for (int i = 0; i < DY; ++i) {
+                const int r = LY::row(wave * DY + i);
+                yo[i] = jf * BN + r < p.N ? r * ystep + LY::piece(wave * DY + i) * 16 : kNone;
+            }
+        }
+    };
+    point();
+    // gather: the rows of a's rows of the next stage, a stage ahead
+    constexpr int NI = MODE == kWgrad ? DY * LY::RL : 1;
+    int index[NI] = {};
+    auto fetch = [&]() INLINE {
+        if (MODE == kWgrad && gather && K > 0) {
+            const int k = k_first + jst * BK + wave * NI;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) index[i] = uniform_load(p.rows + min(k + i, p.M - 1));
+        }
+    };
+    fetch();
+    // Load i of the next stage; past the last stage of the last feature tile zeros are loaded that nothing reads, so that the waits
+    // can count on every load.
+    auto load_y = [&](uint32_t off, uint32_t step, uint8_t* l) INLINE {
+        if (MODE != kWgrad && once)
+            load16<2>(buffer(yb), off, step, l);
+        else
+            load16<0>(buffer(yb), off, step, l);
+    };
+    auto load = [&](int i) INLINE {
+        uint32_t xs = xstep, ys = ystep;
+        asm volatile("" : "+s"(xs), "+s"(ys));   // (steps formed here, not all kept in registers)
+        uint8_t* const s = smem + jslot * Sh::stage_b;
+        const int lim = jf < ft1 ? K - jst * BK : 0;   // the stage's values (rows) before the end
+        if (i < DX) {
+            const int at = wave * DX + i;
+            if constexpr (XCOL)
+                load16<0>(buffer(xb), LX::row(at) < lim ? xo[i & 1] : kNone, uint32_t(at * LX::RL) * xs, s + at * 1024);
+            else
+                load16<0>(buffer(xb), LX::piece(at) * 8 < lim ? xo[i % DX] : kNone, 0, s + at * 1024);
+        } else {
+            const int j = i - DX, at = wave * DY + j;
+            uint8_t* const l = s + BM * KB * 16 + at * 1024;
+            if constexpr (MODE == kProduct) {
+                load_y(LY::piece(at) * 8 < lim ? yo[j % DY] : kNone, 0, l);
+            } else if (gather) {
+                int a = -1;
+#pragma unroll
+                for (int r = 0; r < LY::RL; ++r) a = lane / LY::S::PR == r ? index[(j * LY::RL + r) % NI] : a;
+                const bool in = LY::row(at) < lim && uint32_t(a) < uint32_t(p.a_rows) && yo[j & 1] != kNone;
+                load_y(in ? uint32_t(a) * ys + yo[j & 1] : kNone, 0, l);
+            } else {
+                load_y(LY::row(at) < lim ? yo[j & 1] : kNone, uint32_t(at * LY::RL) * ys, l);
+            }
+        }
+    };
+    auto advance = [&]() INLINE {   // all loads of the stage are issued: on to the next one
+        jslot = jslot == ST - 1 ? 0 : jslot + 1;
+        ++jst;
+        xb += XCOL ? int64_t(BK) * p.ldx * 2 : BK * 2;
+        if (!gather) yb += YCOL ? int64_t(BK) * (MODE == kWgrad ? p.ldy : int64_t(p.C)) * 2 : BK * 2;
+        if (jst == nst) {
+            jst = 0;
+            ++jf;
+            point();
+        }
+        fetch();
+    };
+
+    const int wm = wave / WN * FM * 32, wn = wave % WN * FN * 32;
+    struct Ops {
+        Vec<T> b[FN], a[FM];
+    };
+    f16_t acc[FM][FN];
+    auto read = [&](Ops& o, int slot, int t, int i) INLINE {   // operand i of step t
+        const uint8_t* const s = smem + slot * Sh::stage_b;
+        if (i < FN)
+            o.b[i % FN] = LY::S::read(s + BM * KB * 16, wn + 32 * i, t);
+        else
+            o.a[(i - FN) % FM] = LX::S::read(s, wm + 32 * (i - FN), t);
+    };
+    // A step's products, row by row, with the reads of the next step's operands and part `part` (of SP) of the next stage's loads between them
+    auto step = [&](auto on, const Ops& o, Ops& next, int slot, int t, int part) INLINE {
+#pragma unroll
+        for (int m = 0; m < FM; ++m) {
+            if constexpr (decltype(on)::value) {
+#pragma unroll
+                for (int f = 0; f < FN; ++f) acc[m][f] = mma(o.b[f], o.a[m], acc[m][f]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < FM + FN; ++i)
+                    if (i >= m * (FM + FN) / FM && i < (m + 1) * (FM + FN) / FM) read(next, slot, t, i);
+            }
+#pragma unroll
+            for (int i = 0; i < D; ++i)
+                if (i >= (part * FM + m) * D / (SP * FM) && i < (part * FM + m + 1) * D / (SP * FM)) load(i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    // Waits count the loads: at the end of a stage those of ST - 2 stages were issued behind the next one's, and in a feature tile's first ST
+    // - 1 stages the stores of the tile before (at least kStores per wave; with add, whose stores are not counted on, none).
+    constexpr int kStores = FM * FN * 2, kCap = 63;
+    auto landed = [&](bool stores) INLINE {
+        if (stores)
+            wait_vm<(D * (ST - 2) + kStores < kCap ? D * (ST - 2) + kStores : kCap)>();
+        else
+            wait_vm<(D * (ST - 2) < kCap ? D * (ST - 2) : kCap)>();
+    };
+    auto finish = [&]() INLINE {
+        // The results through LDS, OR rows of QP fourths of a fragment (8 features each) at a time, so that whole lines are stored. Lane l's
+        // value i of a fragment: feature 8 (i / 4) + 4 (l / 32) + i % 4, row l % 32.
+        auto results = [&](auto zero, auto added) INLINE {
+            constexpr bool ADD = decltype(added)::value;   // (in fp32 up to the sum, of the result's type then)
+            typedef decltype(zero) O;
+            constexpr int sz = sizeof(O), QP = 16 / sz < 4 * FN ? 16 / sz : 4 * FN, V = 16 / sz;
+            constexpr int PR = QP * 8 / V, NP = OR * PR / 64;   // pieces of 16 bytes in a row, of a lane; in LDS piece p of row r is at p ^ (r / 2 % 8)
+            static_assert(4 * FN % QP == 0 && FM * (4 * FN / QP) * NP * (32 / OR) >= kStores, "the stores of a wave");
+            typedef O vec4 __attribute__((ext_vector_type(4)));
+            uint8_t* const w = smem + ST * Sh::stage_b + wave * Sh::out_b;
+            O* const out = static_cast<O*>(p.out) + (MODE == kWgrad ? int64_t(g) * p.N * p.C : 0) + x0 * p.ldout;
+            const Buffer to_out = __builtin_amdgcn_make_buffer_rsrc(out, 0, int(((xn - 1) * p.ldout + features) * sz), 0x00020000);
+#pragma unroll
+            for (int m = 0; m < FM; ++m) {
+#pragma unroll
+                for (int q = 0; q < 4 * FN; q += QP) {
+#pragma unroll
+                    for (int e = q / 4; e <= (q + QP - 1) / 4; ++e) asm volatile("" : "+a"(acc[m][e]));   // (read one piece at a time)
+#pragma unroll
+                    for (int pass = 0; pass < 32 / OR; ++pass) {
+                        int ln = lane;
+                        asm volatile("" : "+v"(ln));   // (addresses formed piece by piece, not all kept from before the loop)
+#pragma unroll
+                        for (int i = 0; i < QP; ++i) {
+                            if (OR < 32 && (ln & 31) / OR != pass) break;
+                            vec4 v;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[e] = O(acc[m][(q + i) / 4][(q + i) % 4 * 4 + e]);
+                            const int b = (8 * i + 4 * (ln >> 5)) * sz, r = ln % OR;
+                            *reinterpret_cast<vec4*>(w + r * 128 + (((b >> 4) ^ (r / 2 % 8)) << 4) + (b & 15)) = v;
+                        }
+                        wave_lds_order();
+                        asm volatile("" : "+v"(ln));
+                        const int c = ft * BN + wn + q * 8 + ln % PR * V;
+                        const int r0 = wm + 32 * m + pass * OR + ln / PR;
+                        auto from = [&](int i) INLINE {
+                            const int r = ln / PR + i * (64 / PR);
+                            return w + r * 128 + ((ln % PR ^ (r / 2 % 8)) << 4);
+                        };
+                        if constexpr (ADD) {
+#pragma unroll
+                            for (int i = 0; i < NP; ++i) {
+                                const int r = r0 + i * (64 / PR);
+                                if (r < xn && c < features)
+                                    store4(p, (int64_t(g) * p.N + x0 + r) * p.C + c, *reinterpret_cast<const f4_t*>(from(i)), features - c);
+                            }
+                        } else if (features % V == 0 || (ft + 1) * BN <= features) {
+                            i4_t v[NP];
+#pragma unroll
+                            for (int i = 0; i < NP; ++i) v[i] = *reinterpret_cast<const i4_t*>(from(i));
+#pragma unroll
+                            for (int i = 0; i < NP; ++i) {
+                                const int r = r0 + i * (64 / PR);
+                                const uint32_t to = r < xn && c < features ? uint32_t(r * int(p.ldout) + c) * sz : kNone;
+                                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, v[i]), to_out, to, 0, 2);   // (non-temporal)
+                            }
+                        } else {   // the last feature tile, cut short inside a piece
+                            for (int i = 0; i < NP && r0 + i * (64 / PR) < xn; ++i)
+                                for (int e = 0; e < V && c + e < features; ++e)
+                                    out[(r0 + i * (64 / PR)) * p.ldout + c + e] = *reinterpret_cast<const O*>(from(i) + e * sz);
+                        }
+                        wave_lds_order();
+                    }
+                }
+            }
+        };
+        if (MODE == kWgrad && p.add)
+            results(float(), std::true_type());
+        else if (p.out_type == FRT_GGML_F32)
+            results(float(), std::false_type());
+        else if (p.out_type == FRT_GGML_F16)
+            results(_Float16(), std::false_type());
+        else
+            results(__bf16(), std::false_type());
+    };
+#pragma unroll 1
+    for (int s = 0; s < ST - 1; ++s) {
+#pragma unroll
+        for (int i = 0; i < D; ++i) load(i);
+        advance();
+    }
+#pragma unroll
+    for (int i = 0; i < D / SP; ++i) load(i);
+    wait_vm<(D * (ST - 2) + D / SP < kCap ? D * (ST - 2) + D / SP : kCap)>();
+    ring_barrier();
+    int slot = 0;
+    bool stored = false;   // the tile before left its stores
+    Ops o[2];
+#pragma unroll
+    for (int i = 0; i < FM + FN; ++i) read(o[0], 0, 0, i);
+    lds_reads_done();   // (nothing pending where the loop is entered: its waits are then for its own reads)
+    for (; ft < ft1; ++ft) {
+        // (a wave that has no rows or features in the tile only loads)
+        const bool live = wm < xn && ft * BN + wn < features;
+#pragma unroll
+        for (int m = 0; m < FM; ++m)
+#pragma unroll
+            for (int f = 0; f < FN; ++f)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[m][f][i] = 0.0f;
+        auto stages = [&](auto on) INLINE {
+            for (int st = 0; st < nst; ++st) {
+#pragma unroll
+                for (int t = 0; t < SP - 1; ++t) step(on, o[t & 1], o[(t & 1) ^ 1], slot, t + 1, t + 1);
+                advance();
+                // the end of the stage: the next one has landed, all waves have read this one, and its slot is loaded anew
+                landed(st < ST - 2 && stored);
+                ring_barrier();
+                slot = slot == ST - 1 ? 0 : slot + 1;
+                step(on, o[(SP - 1) & 1], o[0], slot, 0, 0);   // (past the last stage it reads what nothing uses)
+            }
+        };
+        if (live)
+            stages(std::true_type());
+        else
+            stages(std::false_type());
+        if (live) finish();
+        stored = live && !p.add;
+    }
+    // no load into LDS is under way when the workgroup ends (the last tile's stores may be)
+    if (stored)
+        wait_vm<(kStores < kCap ? kStores : kCap)>();
+    else
+        wait_vm<0>();
+}
+
+template <typename T, Mode MODE, int BM, int BN, int WM, int WN, int ST, int KB, int OR, int OCC>
+static int tiles_go(const char* what, const ProductArgs& p, hipStream_t stream) {
+    const int features = MODE == kProduct ? p.N : p.C, ny = (features + BN - 1) / BN, nx = (p.N + BM - 1) / BM;
+    const bool grouped = p.bounds != nullptr;
+    const int64_t groups = grouped ? std::min(p.E, std::max(p.M, 1)) : 1;
+    // feature tiles of a workgroup: about kStages stages, as long as kFill workgroups remain (half a tile of each group empty)
+    const int64_t tiles = MODE == kWgrad ? int64_t(p.E) * nx : tiles_at_most(p.M, p.E, BM, grouped);
+    const int64_t likely = MODE == kWgrad ? tiles : grouped ? std::max<int64_t>(p.M / BM + groups / 2, groups) : tiles;
+    const int64_t K = MODE == kProduct ? p.C : MODE == kGrad ? p.N : p.M / groups;
+    const int nst = int(std::max<int64_t>(1, (K + KB * 8 - 1) / (KB * 8)));
+    // (values in units of 64: one token's down products want several tiles of a short row behind one start, 40 rows of 512 experts one)
+    constexpr int kStages = (MODE == kWgrad ? 16 : 40) * 8 / KB, kFill = 512;
+    int nchunk = std::max(1, std::min(kStages / nst, ny));
+    nchunk = (ny + nchunk - 1) / nchunk;
+    while (nchunk < ny && likely * nchunk < kFill) ++nchunk;
+    const int per = (ny + nchunk - 1) / nchunk;
+    nchunk = (ny + per - 1) / per;
+    const int64_t wgs = (tiles + 7) / 8 * 8 * nchunk;
+    if (wgs * (64 * WM * WN) > 0xffffffff || tiles > 0x7ffff000) return set_error(kErrShape, "%s: M=%d N=%d C=%d E=%d", what, p.M, p.N, p.C, p.E);
+    constexpr int smem = TileShape<BM, BN, WM * WN, ST, KB, OR>::smem;
+    FRT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_product_tiles<T, MODE, BM, BN, WM, WN, ST, KB, OR, OCC>),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, smem));
+    const TileGrid grid{ny, per, nx, MODE != kWgrad, uint32_t(nchunk), FastDiv(uint32_t(RB * nchunk)), FastDiv(uint32_t(nx))};
+    launch_timed(what, k_product_tiles<T, MODE, BM, BN, WM, WN, ST, KB, OR, OCC>, dim3(uint32_t(wgs)), dim3(64 * WM * WN), smem, stream, p, grid);
+    FRT_LAUNCHED(what);
+    return kOk;
+}
+
+// Whether the tiles through direct loads take a call: operands in whole, aligned pieces, offsets within 31 bits
+template <typename T>
+static bool pieces(const ProductArgs& p, int x_cols, bool wgrad) {
+    const auto whole = [](const void* q, int64_t ld) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 8 == 0; };
+    const auto near = [](int64_t rows, int64_t ld) { return ld < (int64_t(1) << 30) / std::max<int64_t>(rows, 1); };   // (twice as many bytes)
+    return sizeof(T) == 2 && x_cols % 8 == 0 && p.C % 8 == 0 && whole(p.x, p.ldx) && whole(p.y, p.ldy) && !p.scales && near(512, p.ldout) &&
+           near(wgrad || !p.rows ? 256 : p.a_rows, p.ldx) && near(wgrad && p.rows ? p.a_rows : 256, p.ldy);
+}
+template <typename T, Mode MODE>
+static int tiles_t(const char* what, const ProductArgs& p, hipStream_t stream) {
+    const int64_t groups = p.bounds ? std::min(p.E, std::max(p.M, 1)) : 1, avg = p.M / groups;
+    const int features = MODE == kProduct ? p.N : p.C;
+    auto tiles = [&](int64_t BM, int64_t BN) {   // were the rows spread evenly
+        return (MODE == kWgrad ? p.E * ((p.N + BM - 1) / BM) : (avg + BM - 1) / BM * groups) * ((features + BN - 1) / BN);
+    };
+    if constexpr (MODE == kWgrad) {
+        if (tiles(256, 256) >= 256) return tiles_go<T, MODE, 256, 256, 2, 4, 4, 4, 32, 2>(what, p, stream);
+    } else {
+        if (avg >= 1024 && tiles(256, 256) >= 512) return tiles_go<T, MODE, 256, 256, 2, 4, 4, 4, 32, 2>(what, p, stream);
+        if (avg > 16 && tiles(128, 256) >= 128) return tiles_go<T, MODE, 128, 256, 2, 4, 3, 8, 16, 2>(what, p, stream);
+    }
+    return tiles_go<T, MODE, 64, 128, 2, 2, 3, 8, 16, 2>(what, p, stream);
+}
+
 template <typename T>
 static int product_t(const ProductArgs& p, hipStream_t stream) {
+    if constexpr (sizeof(T) == 2)
+        if (pieces<T>(p, p.C, false)) return tiles_t<T, kProduct>("moe_product", p, stream);
     return any_go<T, kProduct, false, 64, 64, 2, 2>("moe_product", p, stream);
 }
 template <typename T>
 static int grad_t(const ProductArgs& p, hipStream_t stream) {
+    if constexpr (sizeof(T) == 2)
+        if (pieces<T>(p, p.N, false)) return tiles_t<T, kGrad>("moe_product_grad", p, stream);
     return any_go<T, kGrad, false, 64, 64, 2, 2>("moe_product_grad", p, stream);
 }
 template <typename T>
 static int wgrad_t(const ProductArgs& p, hipStream_t stream) {
+    if constexpr (sizeof(T) == 2)
+        if (pieces<T>(p, p.N, true)) return tiles_t<T, kWgrad>("moe_product_wgrad", p, stream);
     return p.scales ? any_go<T, kWgrad, true, 64, 64, 2, 2>("moe_product_wgrad", p, stream) : any_go<T, kWgrad, false, 64, 64, 2, 2>("moe_product_wgrad", p, stream);
 }
 
