@@ -27,6 +27,9 @@ typedef short s4_t __attribute__((ext_vector_type(4)));
 
 enum Mode { kProduct, kGrad, kWgrad };
 
+// (lambdas of several calls: left to itself the compiler calls the largest, and what they capture goes to memory)
+#define INLINE __attribute__((always_inline))
+
 // 16 bytes of an operand's row: what a lane gives the matrix instructions for one step
 template <typename T>
 struct Chunk {
@@ -321,17 +324,16 @@ struct TileGrid {
     FastDiv blocks, divx;
 };
 constexpr int RB = 4;        // row tiles of a block
-// (lambdas of several calls: left to itself the compiler calls the largest, and what they capture goes to memory)
-#define INLINE __attribute__((always_inline))
 
-template <typename T, Mode MODE, int BM, int BN, int WM, int WN, int ST, int KB, int OR, int OCC>
+template <typename T, Mode MODE, bool EIGHT, int BM, int BN, int WM, int WN, int ST, int KB, int OR, int OCC>
 __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs p, TileGrid grid) {
     constexpr int NW = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32, BK = KB * 8, SP = KB / 2;
     constexpr bool XCOL = MODE == kWgrad, YCOL = MODE != kProduct;
     using Sh = TileShape<BM, BN, NW, ST, KB, OR>;
     using LX = Loads<T, BM, XCOL, KB, NW>;
     using LY = Loads<T, BN, YCOL, KB, NW>;
-    constexpr int DX = LX::D, DY = LY::D, D = DX + DY;
+    // (8-bit rows of a go through registers: CY pieces of 16 codes per thread and stage, NR rows of them per wave)
+    constexpr int DX = LX::D, DY = EIGHT ? 0 : LY::D, D = DX + DY, CY = EIGHT ? BK * BN / (16 * 64 * NW) : 0, NR = 64 / (BN / 16);
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     // Workgroup b runs on XCD b % 8. Each XCD takes an eighth of the row tiles, neighbours, in blocks of RB with their chunks of features: what
@@ -408,13 +410,14 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
         }
     }
     if constexpr (MODE == kWgrad)
-        y0 = static_cast<const uint8_t*>(p.y) + (gather ? 0 : int64_t(k_first) * p.ldy * 2);
+        y0 = static_cast<const uint8_t*>(p.y) + (gather ? 0 : int64_t(k_first) * p.ldy * (EIGHT ? 1 : 2));
     else
         y0 = static_cast<const uint8_t*>(p.y) + int64_t(g) * p.N * p.C * 2;
     const uint8_t* const x0b = xb;
     int jf = ft, jst = 0, jslot = 0;   // the next stage to load: of feature tile jf, into slot jslot
     auto point = [&]() INLINE {
         xb = x0b;
+        if constexpr (EIGHT) return;
         if constexpr (YCOL) {
             yb = y0 + int64_t(jf) * BN * 2;
 #pragma unroll
@@ -433,16 +436,67 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
     };
     point();
     // gather: the rows of a's rows of the next stage, a stage ahead
-    constexpr int NI = MODE == kWgrad ? DY * LY::RL : 1;
+    constexpr int NI = EIGHT ? CY * NR : MODE == kWgrad ? DY * LY::RL : 1;
     int index[NI] = {};
     auto fetch = [&]() INLINE {
-        if (MODE == kWgrad && gather && K > 0) {
+        if (MODE == kWgrad && !EIGHT && gather && K > 0) {
             const int k = k_first + jst * BK + wave * NI;
 #pragma unroll
             for (int i = 0; i < NI; ++i) index[i] = uniform_load(p.rows + min(k + i, p.M - 1));
         }
     };
     fetch();
+    // 8-bit rows of a: the codes and scales of the stage after the next one, and the next one's values into LDS (zeros past the group's rows and a's
+    // columns, and for a row that there is not)
+    int ef = ft, est = 0;   // the stage whose codes are loaded next
+    i4_t codes[EIGHT ? CY : 1];
+    uint32_t scales[EIGHT ? CY : 1];
+    auto fetch8 = [&]() INLINE {
+        const int k0 = est * BK, lim = ef < ft1 ? K - k0 : 0;
+        const Buffer qb = buffer(y0 + (gather ? 0 : int64_t(k0) * p.C)), sb = buffer(p.scales + (gather ? 0 : (int64_t(k_first) + k0) * (p.C / 32)));
+#pragma unroll
+        for (int i = 0; i < CY; ++i) {
+            const int first = (i * NW + wave) * NR, k = first + lane / (BN / 16), c = ef * BN + lane % (BN / 16) * 16;
+            bool in = k < lim && c < p.C;
+            uint32_t a = k;
+            if (gather) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r) a = lane / (BN / 16) == r ? uint32_t(index[(i * NR + r) % NI]) : a;
+                in = in && a < uint32_t(p.a_rows);
+            }
+            codes[i] = __builtin_bit_cast(i4_t, __builtin_amdgcn_raw_buffer_load_b128(qb, in ? a * uint32_t(p.C) + c : kNone, 0, 0));
+            scales[i] = __builtin_amdgcn_raw_buffer_load_b8(sb, in ? a * uint32_t(p.C / 32) + c / 32 : kNone, 0, 0);
+        }
+        if (++est == nst) {
+            est = 0;
+            ++ef;
+        }
+        if (gather && K > 0) {
+            const int k = k_first + est * BK;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) index[i] = uniform_load(p.rows + min(k + (i / NR * NW + wave) * NR + i % NR, p.M - 1));
+        }
+    };
+    auto put8 = [&]() INLINE {
+        uint8_t* const s = smem + jslot * Sh::stage_b + BM * KB * 16;
+#pragma unroll
+        for (int i = 0; i < CY; ++i) {
+            const int k = (i * NW + wave) * NR + lane / (BN / 16), c = lane % (BN / 16) * 2;
+            const float scale = mx8_scale(scales[i]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const auto f = mx8_values(codes[i][2 * h], codes[i][2 * h + 1], scale);
+                *reinterpret_cast<Vec<T>*>(s + LY::S::piece(k, c + h)) = __builtin_convertvector(f, Vec<T>);
+            }
+        }
+    };
+    if constexpr (EIGHT) {
+        if (gather && K > 0) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) index[i] = uniform_load(p.rows + min(k_first + (i / NR * NW + wave) * NR + i % NR, p.M - 1));
+        }
+        fetch8();
+    }
     // Load i of the next stage; past the last stage of the last feature tile zeros are loaded that nothing reads, so that the waits
     // can count on every load.
     auto load_y = [&](uint32_t off, uint32_t step, uint8_t* l) INLINE {
@@ -482,7 +536,7 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
         jslot = jslot == ST - 1 ? 0 : jslot + 1;
         ++jst;
         xb += XCOL ? int64_t(BK) * p.ldx * 2 : BK * 2;
-        if (!gather) yb += YCOL ? int64_t(BK) * (MODE == kWgrad ? p.ldy : int64_t(p.C)) * 2 : BK * 2;
+        if (!gather && !EIGHT) yb += YCOL ? int64_t(BK) * (MODE == kWgrad ? p.ldy : int64_t(p.C)) * 2 : BK * 2;
         if (jst == nst) {
             jst = 0;
             ++jf;
@@ -518,18 +572,23 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
 #pragma unroll
             for (int i = 0; i < D; ++i)
                 if (i >= (part * FM + m) * D / (SP * FM) && i < (part * FM + m + 1) * D / (SP * FM)) load(i);
+            if constexpr (EIGHT)
+                if (part == 0 && m == 0) {
+                    put8();
+                    fetch8();
+                }
             __builtin_amdgcn_sched_barrier(0);
         }
     };
 
     // Waits count the loads: at the end of a stage those of ST - 2 stages were issued behind the next one's, and in a feature tile's first ST
     // - 1 stages the stores of the tile before (at least kStores per wave; with add, whose stores are not counted on, none).
-    constexpr int kStores = FM * FN * 2, kCap = 63;
+    constexpr int kStage = D + 2 * CY, kStores = FM * FN * 2, kCap = 63;
     auto landed = [&](bool stores) INLINE {
         if (stores)
-            wait_vm<(D * (ST - 2) + kStores < kCap ? D * (ST - 2) + kStores : kCap)>();
+            wait_vm<(kStage * (ST - 2) + kStores < kCap ? kStage * (ST - 2) + kStores : kCap)>();
         else
-            wait_vm<(D * (ST - 2) < kCap ? D * (ST - 2) : kCap)>();
+            wait_vm<(kStage * (ST - 2) < kCap ? kStage * (ST - 2) : kCap)>();
     };
     auto finish = [&]() INLINE {
         // The results through LDS, OR rows of QP fourths of a fragment (8 features each) at a time, so that whole lines are stored. Lane l's
@@ -611,11 +670,19 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
     for (int s = 0; s < ST - 1; ++s) {
 #pragma unroll
         for (int i = 0; i < D; ++i) load(i);
+        if constexpr (EIGHT) {
+            put8();
+            fetch8();
+        }
         advance();
     }
 #pragma unroll
     for (int i = 0; i < D / SP; ++i) load(i);
-    wait_vm<(D * (ST - 2) + D / SP < kCap ? D * (ST - 2) + D / SP : kCap)>();
+    if constexpr (EIGHT) {
+        put8();
+        fetch8();
+    }
+    wait_vm<(kStage * (ST - 2) + D / SP < kCap ? kStage * (ST - 2) + D / SP : kCap)>();
     ring_barrier();
     int slot = 0;
     bool stored = false;   // the tile before left its stores
@@ -658,7 +725,7 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
         wait_vm<0>();
 }
 
-template <typename T, Mode MODE, int BM, int BN, int WM, int WN, int ST, int KB, int OR, int OCC>
+template <typename T, Mode MODE, bool EIGHT, int BM, int BN, int WM, int WN, int ST, int KB, int OR, int OCC>
 static int tiles_go(const char* what, const ProductArgs& p, hipStream_t stream) {
     const int features = MODE == kProduct ? p.N : p.C, ny = (features + BN - 1) / BN, nx = (p.N + BM - 1) / BM;
     const bool grouped = p.bounds != nullptr;
@@ -678,11 +745,96 @@ static int tiles_go(const char* what, const ProductArgs& p, hipStream_t stream) 
     const int64_t wgs = (tiles + 7) / 8 * 8 * nchunk;
     if (wgs * (64 * WM * WN) > 0xffffffff || tiles > 0x7ffff000) return set_error(kErrShape, "%s: M=%d N=%d C=%d E=%d", what, p.M, p.N, p.C, p.E);
     constexpr int smem = TileShape<BM, BN, WM * WN, ST, KB, OR>::smem;
-    FRT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_product_tiles<T, MODE, BM, BN, WM, WN, ST, KB, OR, OCC>),
+    FRT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_product_tiles<T, MODE, EIGHT, BM, BN, WM, WN, ST, KB, OR, OCC>),
                                 hipFuncAttributeMaxDynamicSharedMemorySize, smem));
     const TileGrid grid{ny, per, nx, MODE != kWgrad, uint32_t(nchunk), FastDiv(uint32_t(RB * nchunk)), FastDiv(uint32_t(nx))};
-    launch_timed(what, k_product_tiles<T, MODE, BM, BN, WM, WN, ST, KB, OR, OCC>, dim3(uint32_t(wgs)), dim3(64 * WM * WN), smem, stream, p, grid);
+    launch_timed(what, k_product_tiles<T, MODE, EIGHT, BM, BN, WM, WN, ST, KB, OR, OCC>, dim3(uint32_t(wgs)), dim3(64 * WM * WN), smem, stream, p, grid);
     FRT_LAUNCHED(what);
+    return kOk;
+}
+
+// ---------------------------------------------------------------- few rows
+__device__ __forceinline__ f4_t mma16(Vec<_Float16> w, Vec<_Float16> x, f4_t acc) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(w, x, acc, 0, 0, 0); }
+__device__ __forceinline__ f4_t mma16(Vec<__bf16> w, Vec<__bf16> x, f4_t acc) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x, acc, 0, 0, 0); }
+
+// 16 features x 16 rows by KW waves that share the values of a row, straight from global memory into the registers of the matrix
+// instructions. The weights are the first operand, so that a lane's four results are adjacent features of one row. A group of 128 values is 16
+// chunks: step i multiplies chunks 4 i + l / 16 of lane l's feature and row. Wave w takes the groups w, w + KW, ..., two at a time in
+// flight; the waves' sums are added in their order. Rows and features past the end are the last one again, never stored.
+template <typename T, int KW>
+__global__ void __launch_bounds__(256) k_product_rows(ProductArgs p, int ntile, FastDiv ntiles) {
+    constexpr int FW = 4 / KW, V = Chunk<T>::V, P = 2;   // tiles of a workgroup; groups in flight (four: 5% slower)
+    __shared__ f4_t s_sum[4][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
+    const int kw = wave % KW;
+    const uint32_t unit = wide_block() * FW + wave / KW, tile = ntiles(unit);
+    const RowTile t = find_tile<16>(p.bounds, p.E, p.M, [&](int total) { return int(tile) < total ? int(tile) : -1; });
+    const int f0 = int(unit - tile * ntile) * 16, nc = p.C / V, ng = (nc + 15) / 16;
+    f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (t.rows > 0) {   // (uniform over the wave)
+        const int r = t.row0 + min(j, t.rows - 1);
+        int a = r;
+        if (p.rows) a = gld<int>(p.rows + r);   // (under way while the weights' loads are issued)
+        const T* const w = static_cast<const T*>(p.y) + (int64_t(t.g) * p.N + min(f0 + j, p.N - 1)) * p.C;
+        struct Group {
+            Vec<T> w[4], x[4];
+        } u[P];
+        auto load_w = [&](int q, Group& o) INLINE {   // (chunks past the last are the last again: its partner is zeros there)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o.w[i] = gld<Vec<T>>(w + min(16 * q + 4 * i + g, nc - 1) * V);
+        };
+        const T* x = nullptr;
+        auto load_x = [&](int q, Group& o) INLINE {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o.x[i] = gld<Vec<T>>(x + min(16 * q + 4 * i + g, nc - 1) * V);
+        };
+        auto multiply = [&](int q, const Group& o) INLINE {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool in = 16 * q + 4 * i + g < nc;
+                const Vec<T> zero = {};
+                acc = mma16(in ? o.w[i] : zero, in ? o.x[i] : zero, acc);
+            }
+        };
+#pragma unroll
+        for (int k = 0; k < P; ++k)
+            if (kw + k * KW < ng) load_w(kw + k * KW, u[k]);
+        __builtin_amdgcn_sched_barrier(0);
+        const bool ok = unsigned(a) < unsigned(p.a_rows);
+        x = static_cast<const T*>(p.x) + int64_t(ok ? a : 0) * p.ldx;
+#pragma unroll
+        for (int k = 0; k < P; ++k)
+            if (kw + k * KW < ng) load_x(kw + k * KW, u[k]);
+        for (int q = kw; q < ng; q += P * KW) {
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                const int c = q + k * KW, n = c + P * KW;
+                if (c < ng) multiply(c, u[k]);
+                if (n < ng) {
+                    load_w(n, u[k]);
+                    load_x(n, u[k]);
+                }
+            }
+        }
+        if (!ok) acc = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    if constexpr (KW > 1) {
+        s_sum[wave][lane] = acc;
+        __syncthreads();
+        if (kw != 0) return;
+#pragma unroll
+        for (int i = 1; i < KW; ++i) acc += s_sum[wave + i][lane];
+    }
+    if (j < t.rows && f0 + 4 * g < p.N) store4(p, (int64_t(t.row0) + j) * p.ldout + f0 + 4 * g, acc, p.N - f0 - 4 * g);
+}
+
+template <typename T, int KW>
+static int rows_go(const ProductArgs& p, hipStream_t stream) {
+    const int ntile = (p.N + 15) / 16;
+    const int64_t units = tiles_at_most(p.M, p.E, 16, p.bounds != nullptr) * ntile, wgs = (units + 4 / KW - 1) / (4 / KW);
+    if (units > 0x7ffff000) return set_error(kErrShape, "moe_product: M=%d N=%d E=%d", p.M, p.N, p.E);
+    launch_timed("moe_product", k_product_rows<T, KW>, wide_grid(uint32_t(wgs)), dim3(256), 0, stream, p, ntile, FastDiv(uint32_t(ntile)));
+    FRT_LAUNCHED("moe_product");
     return kOk;
 }
 
@@ -691,10 +843,10 @@ template <typename T>
 static bool pieces(const ProductArgs& p, int x_cols, bool wgrad) {
     const auto whole = [](const void* q, int64_t ld) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 8 == 0; };
     const auto near = [](int64_t rows, int64_t ld) { return ld < (int64_t(1) << 30) / std::max<int64_t>(rows, 1); };   // (twice as many bytes)
-    return sizeof(T) == 2 && x_cols % 8 == 0 && p.C % 8 == 0 && whole(p.x, p.ldx) && whole(p.y, p.ldy) && !p.scales && near(512, p.ldout) &&
+    return sizeof(T) == 2 && x_cols % 8 == 0 && p.C % 8 == 0 && whole(p.x, p.ldx) && whole(p.y, p.ldy) && near(512, p.ldout) &&
            near(wgrad || !p.rows ? 256 : p.a_rows, p.ldx) && near(wgrad && p.rows ? p.a_rows : 256, p.ldy);
 }
-template <typename T, Mode MODE>
+template <typename T, Mode MODE, bool EIGHT = false>
 static int tiles_t(const char* what, const ProductArgs& p, hipStream_t stream) {
     const int64_t groups = p.bounds ? std::min(p.E, std::max(p.M, 1)) : 1, avg = p.M / groups;
     const int features = MODE == kProduct ? p.N : p.C;
@@ -702,18 +854,27 @@ static int tiles_t(const char* what, const ProductArgs& p, hipStream_t stream) {
         return (MODE == kWgrad ? p.E * ((p.N + BM - 1) / BM) : (avg + BM - 1) / BM * groups) * ((features + BN - 1) / BN);
     };
     if constexpr (MODE == kWgrad) {
-        if (tiles(256, 256) >= 256) return tiles_go<T, MODE, 256, 256, 2, 4, 4, 4, 32, 2>(what, p, stream);
+        if (tiles(256, 256) >= 256) return tiles_go<T, MODE, EIGHT, 256, 256, 2, 4, 4, 4, 32, 2>(what, p, stream);
     } else {
-        if (avg >= 1024 && tiles(256, 256) >= 512) return tiles_go<T, MODE, 256, 256, 2, 4, 4, 4, 32, 2>(what, p, stream);
-        if (avg > 16 && tiles(128, 256) >= 128) return tiles_go<T, MODE, 128, 256, 2, 4, 3, 8, 16, 2>(what, p, stream);
+        if (avg >= 1024 && tiles(256, 256) >= 512) return tiles_go<T, MODE, EIGHT, 256, 256, 2, 4, 4, 4, 32, 2>(what, p, stream);
+        if (avg > 16 && tiles(128, 256) >= 128) return tiles_go<T, MODE, EIGHT, 128, 256, 2, 4, 3, 8, 16, 2>(what, p, stream);
     }
-    return tiles_go<T, MODE, 64, 128, 2, 2, 3, 8, 16, 2>(what, p, stream);
+    return tiles_go<T, MODE, EIGHT, 64, 128, 2, 2, 3, 8, 16, 2>(what, p, stream);
 }
 
 template <typename T>
 static int product_t(const ProductArgs& p, hipStream_t stream) {
     if constexpr (sizeof(T) == 2)
-        if (pieces<T>(p, p.C, false)) return tiles_t<T, kProduct>("moe_product", p, stream);
+        if (pieces<T>(p, p.C, false)) {
+            // The weights that tiles of 16 rows read: up to 256 MB straight into registers, with the values over the waves where those are
+            // few; beyond, in tiles through LDS. us, one wave / two / four to a row / tiles: one token's ten experts (N 1024, C 2048, 42
+            // MB) 12.9 / 12.9 / 12.3 / 19.5, two tokens' 21.7 / 18.3 / 19.4 / 22.3, four 31 / 29 / 35 / 32, sixteen (600 MB) 114 / 109 /
+            // 122 / 99; N 2560, C 640 9.6 / 11.7 / 14.0 / 12.0; one group (N 8192, C 4096) of a row 20.9 / 20.2 / 15.6 / 34.7
+            const int64_t groups = p.bounds ? std::min(p.E, p.M) : 1, units = (p.M / groups + 15) / 16 * groups * ((p.N + 15) / 16);
+            if (units * 32 * p.C <= int64_t(256) << 20)
+                return units <= 640 && p.C >= 512 ? rows_go<T, 4>(p, stream) : units <= 1280 && p.C >= 256 ? rows_go<T, 2>(p, stream) : rows_go<T, 1>(p, stream);
+            return tiles_t<T, kProduct>("moe_product", p, stream);
+        }
     return any_go<T, kProduct, false, 64, 64, 2, 2>("moe_product", p, stream);
 }
 template <typename T>
@@ -725,7 +886,8 @@ static int grad_t(const ProductArgs& p, hipStream_t stream) {
 template <typename T>
 static int wgrad_t(const ProductArgs& p, hipStream_t stream) {
     if constexpr (sizeof(T) == 2)
-        if (pieces<T>(p, p.N, true)) return tiles_t<T, kWgrad>("moe_product_wgrad", p, stream);
+        if (pieces<T>(p, p.N, true))
+            return p.scales ? tiles_t<T, kWgrad, true>("moe_product_wgrad", p, stream) : tiles_t<T, kWgrad>("moe_product_wgrad", p, stream);
     return p.scales ? any_go<T, kWgrad, true, 64, 64, 2, 2>("moe_product_wgrad", p, stream) : any_go<T, kWgrad, false, 64, 64, 2, 2>("moe_product_wgrad", p, stream);
 }
 
