@@ -88,8 +88,8 @@ def run(op, sizes, N, C, kind, out_kind, gather=0, eight=False, add=False, pad=0
         if v is not None:
             v[live:] = float("nan")
     if op != "wgrad":
-        g = torch.Generator().manual_seed(N + C)
-        w = (torch.randn(E, N, C, generator=g) * 0.1).to(kind).cuda()
+        g = torch.Generator(device="cuda").manual_seed(N + C)
+        w = (torch.randn(E, N, C, generator=g, device="cuda") * 0.1).to(kind)
         arg = w if sizes is not None else w[0]
     buf = out_of(out_rows, out_cols, out_kind, 0 if op == "wgrad" else pad)
     got = buf[:out_rows, :out_cols]
@@ -268,6 +268,65 @@ def test_weight_gradient_without_rows():
         assert (dw == 77).all()
         F.moe_product_wgrad(dout, a, dw, bounds=b)
         assert (dw == 0).all()
+
+
+def ragged(n, lo, hi):
+    """n group sizes between lo and hi, with an empty one and the ends among them."""
+    return [lo + (37 * i) % (hi - lo + 1) for i in range(n - 3)] + [0, hi, lo]
+
+
+# Shapes that each of the kernels for whole, aligned rows takes (op, group sizes, N, C, gather): the rows that are read straight into registers by
+# four, two and one wave to a row, the tiles of 64 x 128, 128 x 256 and 256 x 256, with contracted values that end inside a stage.
+KERNELS = {
+    "rows, four waves": ("product", [1, 0, 3, 16, 17], 136, 520, 0),
+    "rows, two waves": ("product", [1] * 40, 328, 264, 9),
+    "rows, one wave": ("product", [2, 0, 1, 33], 200, 136, 9),
+    "rows, one wave, many": ("product", ragged(30, 1, 20), 1000, 648, 0),
+    "product 64": ("product", ragged(40, 0, 30), 4100, 1928, 50),
+    "product 128": ("product", ragged(33, 1, 140), 1000, 1096, 0),
+    "product 128, picked": ("product", ragged(33, 1, 140), 1004, 1032, 300),
+    "product 256": ("product", [1111, 1300], 13320, 264, 0),
+    "product 256, picked": ("product", [1536, 1027], 13316, 136, 600),
+    "grad 64": ("grad", ragged(20, 0, 70), 200, 328, 0),
+    "grad 128": ("grad", ragged(33, 1, 300), 264, 1000, 0),
+    "grad 256": ("grad", [1111, 1300], 200, 13320, 0),
+    "wgrad 64": ("wgrad", ragged(9, 0, 300), 200, 328, 0),
+    "wgrad 64, picked": ("wgrad", ragged(9, 0, 300), 328, 136, 70),
+    "wgrad 256": ("wgrad", ragged(70, 0, 400), 328, 520, 0),
+    "wgrad 256, picked": ("wgrad", ragged(70, 0, 400), 264, 776, 70),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("shape", list(KERNELS))
+def test_every_kernel(shape, kind):
+    op, sizes, N, C, gather = KERNELS[shape]
+    run(op, sizes, N, C, kind, F32 if kind is F16 else BF16, gather=gather, pad=8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out_kind", TYPES)
+@pytest.mark.parametrize("shape", ["rows, four waves", "product 64", "product 128", "grad 128", "wgrad 64", "wgrad 256"])
+def test_result_types_of_every_kernel(shape, out_kind):
+    op, sizes, N, C, gather = KERNELS[shape]
+    run(op, sizes, N, C, BF16, out_kind, gather=gather, pad=8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("shape,C", [("wgrad 64", 352), ("wgrad 64, picked", 160), ("wgrad 256", 544), ("wgrad 256, picked", 800)])
+def test_8_bit_rows_in_every_kernel(shape, C, kind):
+    op, sizes, N, _, gather = KERNELS[shape]
+    run(op, sizes, N, C, kind, kind, gather=gather, eight=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out_kind", TYPES)
+@pytest.mark.parametrize("shape,eight", [("wgrad 64", False), ("wgrad 256", False), ("wgrad 256", True)])
+def test_added_in_every_kernel(shape, eight, out_kind):
+    op, sizes, N, C, _ = KERNELS[shape]
+    run(op, sizes, N, C // 32 * 32, BF16, out_kind, eight=eight, add=True)
 
 
 # ---------------------------------------------------------------- values, bounds, offsets
