@@ -64,6 +64,39 @@ __device__ __forceinline__ RowTile find_tile(const int32_t* __restrict__ bounds,
     return {__builtin_amdgcn_readlane(g, owner), __builtin_amdgcn_readlane(row0, owner), __builtin_amdgcn_readlane(rows, owner),
             __builtin_amdgcn_readlane(of, owner) == 1};
 }
+// The group of rank r by size, largest first (equal ones in any fixed order), of up to 512 groups, by one wave: the rank's size bit by bit, each bit by
+// counting the groups that have at least that many rows.
+__device__ __forceinline__ int group_by_size(const int32_t* __restrict__ bounds, int E, int M, int rank) {
+    const int lane = threadIdx.x & 63;
+    int at[9], rows[8];
+#pragma unroll
+    for (int i = 0; i < 9; ++i) at[i] = gld<int>(bounds + min(8 * lane + i, E));
+#pragma unroll
+    for (int i = 0; i < 9; ++i) at[i] = min(max(at[i], 0), M);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rows[i] = 8 * lane + i < E ? max(0, at[i + 1] - at[i]) : -1;
+    auto count = [&](int least) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n += __popcll(__ballot(rows[i] >= least));
+        return n;
+    };
+    int size = 0;
+    for (int bit = 31 - __builtin_clz(M | 1); bit >= 0; --bit)
+        if (count(size | 1 << bit) > rank) size |= 1 << bit;
+    int left = rank - count(size + 1);   // of the groups of that size
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        uint64_t same = __ballot(rows[i] == size);
+        const int n = __popcll(same);
+        if (left < n) {
+            for (; left > 0; --left) same &= same - 1;
+            return 8 * __builtin_ctzll(same) + i;
+        }
+        left -= n;
+    }
+    return 0;   // (rank is below E)
+}
 // Tiles of BM rows that M rows in E groups have at most
 inline int64_t tiles_at_most(int64_t M, int64_t E, int BM, bool grouped) {
     const int64_t g = grouped ? (E < M ? E : M) : (M > 0 ? 1 : 0);   // groups with rows

@@ -320,6 +320,7 @@ __device__ __forceinline__ int uniform_load(const int32_t* p) { return *(const _
 struct TileGrid {
     int ny, per, nx;         // feature tiles, of a workgroup, row tiles (wgrad)
     int stream;              // weights that one row tile reads are not kept in L2
+    int sorted;              // wgrad: the groups by size
     uint32_t nchunk;
     FastDiv blocks, divx;
 };
@@ -358,11 +359,17 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
     };
     bool once = grid.stream;
     if constexpr (MODE == kWgrad) {
-        // (the groups' sizes differ, and with them their tiles' work: the row tiles go round the XCDs)
-        const int xcd = blockIdx.x & 7, j = order(blockIdx.x >> 3, (p.E * grid.nx - xcd + 7) / 8), index = j * 8 + xcd;
-        if (j < 0) return;
-        g = int(grid.divx(uint32_t(index)));
-        x0 = (index - g * grid.nx) * BM;
+        int index;
+        if (grid.sorted) {   // the groups' sizes differ, and with them their tiles' work: the largest first, their row tiles round the XCDs
+            const int xcd = blockIdx.x & 7, j = order(blockIdx.x >> 3, (p.E * grid.nx - xcd + 7) / 8);
+            index = j < 0 ? -1 : j * 8 + xcd;
+        } else {
+            index = which(p.E * grid.nx);
+        }
+        if (index < 0) return;
+        const int rank = int(grid.divx(uint32_t(index)));
+        g = grid.sorted ? group_by_size(p.bounds, p.E, p.M, rank) : rank;
+        x0 = (index - rank * grid.nx) * BM;
         xn = min(BM, p.N - x0);
         k_first = p.bounds ? min(max(p.bounds[g], 0), p.M) : 0;
         K = max(0, (p.bounds ? min(max(p.bounds[g + 1], 0), p.M) : p.M) - k_first);
@@ -730,13 +737,15 @@ static int tiles_go(const char* what, const ProductArgs& p, hipStream_t stream) 
     const int features = MODE == kProduct ? p.N : p.C, ny = (features + BN - 1) / BN, nx = (p.N + BM - 1) / BM;
     const bool grouped = p.bounds != nullptr;
     const int64_t groups = grouped ? std::min(p.E, std::max(p.M, 1)) : 1;
+    const bool sorted = MODE == kWgrad && grouped && p.E <= 512 && p.M / groups >= 128;
     // feature tiles of a workgroup: about kStages stages, as long as kFill workgroups remain (half a tile of each group empty)
     const int64_t tiles = MODE == kWgrad ? int64_t(p.E) * nx : tiles_at_most(p.M, p.E, BM, grouped);
     const int64_t likely = MODE == kWgrad ? tiles : grouped ? std::max<int64_t>(p.M / BM + groups / 2, groups) : tiles;
     const int64_t K = MODE == kProduct ? p.C : MODE == kGrad ? p.N : p.M / groups;
     const int nst = int(std::max<int64_t>(1, (K + KB * 8 - 1) / (KB * 8)));
     // (values in units of 64: one token's down products want several tiles of a short row behind one start, 40 rows of 512 experts one)
-    constexpr int kStages = (MODE == kWgrad ? 16 : 40) * 8 / KB, kFill = 512;
+    constexpr int kFill = 512;
+    const int kStages = (MODE == kWgrad ? sorted ? 16 : 8 : 40) * 8 / KB;
     int nchunk = std::max(1, std::min(kStages / nst, ny));
     nchunk = (ny + nchunk - 1) / nchunk;
     while (nchunk < ny && likely * nchunk < kFill) ++nchunk;
@@ -747,7 +756,7 @@ static int tiles_go(const char* what, const ProductArgs& p, hipStream_t stream) 
     constexpr int smem = TileShape<BM, BN, WM * WN, ST, KB, OR>::smem;
     FRT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_product_tiles<T, MODE, EIGHT, BM, BN, WM, WN, ST, KB, OR, OCC>),
                                 hipFuncAttributeMaxDynamicSharedMemorySize, smem));
-    const TileGrid grid{ny, per, nx, MODE != kWgrad, uint32_t(nchunk), FastDiv(uint32_t(RB * nchunk)), FastDiv(uint32_t(nx))};
+    const TileGrid grid{ny, per, nx, MODE != kWgrad, sorted, uint32_t(nchunk), FastDiv(uint32_t(RB * nchunk)), FastDiv(uint32_t(nx))};
     launch_timed(what, k_product_tiles<T, MODE, EIGHT, BM, BN, WM, WN, ST, KB, OR, OCC>, dim3(uint32_t(wgs)), dim3(64 * WM * WN), smem, stream, p, grid);
     FRT_LAUNCHED(what);
     return kOk;
@@ -854,7 +863,8 @@ static int tiles_t(const char* what, const ProductArgs& p, hipStream_t stream) {
         return (MODE == kWgrad ? p.E * ((p.N + BM - 1) / BM) : (avg + BM - 1) / BM * groups) * ((features + BN - 1) / BN);
     };
     if constexpr (MODE == kWgrad) {
-        if (tiles(256, 256) >= 256) return tiles_go<T, MODE, EIGHT, 256, 256, 2, 4, 4, 4, 32, 2>(what, p, stream);
+        if (tiles(256, 256) >= 256)
+            return tiles_go<T, MODE, EIGHT, 256, 256, 2, 4, 4, 4, 32, 2>(what, p, stream);
     } else {
         if (avg >= 1024 && tiles(256, 256) >= 512) return tiles_go<T, MODE, EIGHT, 256, 256, 2, 4, 4, 4, 32, 2>(what, p, stream);
         if (avg > 16 && tiles(128, 256) >= 128) return tiles_go<T, MODE, EIGHT, 128, 256, 2, 4, 3, 8, 16, 2>(what, p, stream);
