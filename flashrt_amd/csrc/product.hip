@@ -337,9 +337,10 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
     constexpr int DX = LX::D, DY = EIGHT ? 0 : LY::D, D = DX + DY, CY = EIGHT ? BK * BN / (16 * 64 * NW) : 0, NR = 64 / (BN / 16);
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    // Workgroup b runs on XCD b % 8. Each XCD takes an eighth of the row tiles, neighbours, in blocks of RB with their chunks of features: what
+    // Workgroup b runs on XCD b % 8 (the grid's rows are whole eights). Each XCD takes an eighth of the row tiles, neighbours, in blocks of RB with their chunks of features: what
     // runs at once on it reads few different rows of either operand. Where eighths would leave more than a ninth of the chip idle,
     // the blocks go over all XCDs.
+    const uint32_t b = wide_block(), xcd = b & 7;
     int g, x0, xn, K, k_first = 0, chunk = 0;
     auto order = [&](uint32_t i, int tiles) INLINE {   // the row tile of workgroup i of those of that many row tiles (-1: none), and its chunk
         uint32_t block = grid.blocks(i), in = i - block * (RB * grid.nchunk), rows = RB;
@@ -353,16 +354,16 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
     };
     auto which = [&](int total) INLINE {
         const int each = (total + 7) / 8;
-        if (each * 8 - total > total / 8) return order(blockIdx.x, total);
-        const int first = int(blockIdx.x & 7) * each, j = order(blockIdx.x >> 3, max(0, min(each, total - first)));
+        if (each * 8 - total > total / 8) return order(b, total);
+        const int first = int(xcd) * each, j = order(b >> 3, max(0, min(each, total - first)));
         return j < 0 ? -1 : first + j;
     };
     bool once = grid.stream;
     if constexpr (MODE == kWgrad) {
         int index;
         if (grid.sorted) {   // the groups' sizes differ, and with them their tiles' work: the largest first, their row tiles round the XCDs
-            const int xcd = blockIdx.x & 7, j = order(blockIdx.x >> 3, (p.E * grid.nx - xcd + 7) / 8);
-            index = j < 0 ? -1 : j * 8 + xcd;
+            const int j = order(b >> 3, (p.E * grid.nx - int(xcd) + 7) / 8);
+            index = j < 0 ? -1 : j * 8 + int(xcd);
         } else {
             index = which(p.E * grid.nx);
         }
@@ -752,12 +753,13 @@ static int tiles_go(const char* what, const ProductArgs& p, hipStream_t stream) 
     const int per = (ny + nchunk - 1) / nchunk;
     nchunk = (ny + per - 1) / per;
     const int64_t wgs = (tiles + 7) / 8 * 8 * nchunk;
-    if (wgs * (64 * WM * WN) > 0xffffffff || tiles > 0x7ffff000) return set_error(kErrShape, "%s: M=%d N=%d C=%d E=%d", what, p.M, p.N, p.C, p.E);
+    if (wgs > 0x7ffff000 || tiles > 0x7ffff000) return set_error(kErrShape, "%s: M=%d N=%d C=%d E=%d", what, p.M, p.N, p.C, p.E);
+    const uint32_t y = uint32_t((wgs + (1 << 22) - 1) >> 22), x = uint32_t(((wgs + y - 1) / y + 7) / 8 * 8);   // (fewer than 2^32 threads in a dimension)
     constexpr int smem = TileShape<BM, BN, WM * WN, ST, KB, OR>::smem;
     FRT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_product_tiles<T, MODE, EIGHT, BM, BN, WM, WN, ST, KB, OR, OCC>),
                                 hipFuncAttributeMaxDynamicSharedMemorySize, smem));
     const TileGrid grid{ny, per, nx, MODE != kWgrad, sorted, uint32_t(nchunk), FastDiv(uint32_t(RB * nchunk)), FastDiv(uint32_t(nx))};
-    launch_timed(what, k_product_tiles<T, MODE, EIGHT, BM, BN, WM, WN, ST, KB, OR, OCC>, dim3(uint32_t(wgs)), dim3(64 * WM * WN), smem, stream, p, grid);
+    launch_timed(what, k_product_tiles<T, MODE, EIGHT, BM, BN, WM, WN, ST, KB, OR, OCC>, dim3(x, y), dim3(64 * WM * WN), smem, stream, p, grid);
     FRT_LAUNCHED(what);
     return kOk;
 }

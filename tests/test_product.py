@@ -444,6 +444,26 @@ def test_rows_far_apart(op):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", [BF16, F32])
+def test_more_rows_than_one_grid_dimension(kind):
+    """Nearly 2^30 rows of eight values (2^28 in fp32): more workgroups than one dimension of a launch holds, offsets past 32 bits. The rows
+    repeat, in small whole numbers, so that every sum is exact."""
+    import flashrt_amd as F
+    n, M = 1 << 16, (1 << 30) - 3 if kind is BF16 else (1 << 28) + 5
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rows = torch.randint(-8, 9, (n, 8), generator=g, device="cuda").to(kind)
+    w = torch.randint(-8, 9, (8, 8), generator=g, device="cuda").to(kind)
+    a = rows.repeat((M + n - 1) // n, 1)[:M]
+    out = torch.empty(M, 8, dtype=kind, device="cuda")
+    F.moe_product(a, w, out)
+    want = (rows.double() @ w.double().t()).to(kind)
+    for r in range(0, M, n):
+        m = min(n, M - r)
+        if r // n % 64 == 0 or m < n:
+            assert torch.equal(out[r:r + m], want[:m]), r
+
+
+@pytest.mark.gpu
 def test_largest_weights_of_the_type():
     """fp16 results beyond the type's range become infinities as a conversion's do, and sums stay in fp32 on the way."""
     import flashrt_amd as F
