@@ -4,7 +4,8 @@
 //   grad      da[r] = w_g^T dout[r]      contracted over N: w's columns
 //   wgrad     dw_g = sum_r dout[r] a(r)^T   contracted over the group's rows: columns of both
 // r in [bounds[g], bounds[g + 1]); a(r) is row r, or row rows[r]. In all three an output tile is X Y^T with X the operand along the output's
-// rows and Y the one along its columns ("features").
+// rows and Y the one along its columns ("features"). Three kernels, by alignment and size: tiles through direct loads into LDS (whole, aligned
+// rows of 16 bits), tiles through registers (any rows, and 32 bits), and rows straight into the matrix instructions (few rows).
 #include "common.hpp"
 #include "groups.hpp"
 #include "lds_dma.hpp"
@@ -137,7 +138,10 @@ __device__ __forceinline__ void store4(const ProductArgs& p, int64_t at, f4_t v,
 }
 
 // Rows at any distance and alignment: a tile of BM rows x BN features by WM x WN waves, one stage of LDS, the next stage's operands in registers
-// while this one is multiplied.
+// while this one is multiplied; what hides the loads' latency is the other workgroups of the CU (eight at 64 x 64). 1542 rows of 128 experts (N
+// 1021, C 1019, fp16, 267 MB of weights) 69 us, about the time of the other kernels at C 1024; 16384 rows 171 us, 200 TFLOP/s, against 148 to 183 with
+// tiles of 32 x 128 to 128 x 256 (rows' gradients 222 / 259 to 364, weights' 268 / 267 to 431). fp32 (8192 rows of 128 experts, N 2048, C 1024) 490
+// us, 70 TFLOP/s of the library's 153 at 8192^3. Whole stages without the checks of single pieces gave nothing.
 template <typename T, Mode MODE, bool EIGHT, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN) k_product_any(ProductArgs p, int nx, int ny, FastDiv divx, FastDiv divy) {
     constexpr int NT = 64 * WM * WN, V = Chunk<T>::V, FM = BM / WM / 32, FN = BN / WN / 32;
@@ -326,6 +330,24 @@ struct TileGrid {
 };
 constexpr int RB = 4;        // row tiles of a block
 
+// BM rows x BN features per tile, `per` feature tiles of one row tile after one another in a workgroup of WM x WN waves. A stage is KB
+// chunks (8 values) of the contracted values of every row, in a ring of ST slots that direct loads fill: offsets per lane from a base that moves
+// with the stages, so that a load costs no address arithmetic, and an offset past the buffer where there is no such row, column or value: it
+// reads nothing and leaves zeros, so that no operand is masked and the number of loads, which the waits count, is fixed. A wave multiplies FM x FN
+// fragments of 32 x 32; the reads of the next step's operands and a part of the loads go between its products. The barrier at a stage's end
+// comes before its last step, whose operands are in registers, and the next stage's first ones are read behind it. The stages of the feature
+// tiles form one sequence: the next tile's first stages load while this one's results are written.
+//
+// What bounds it: with few rows to a group the weights' stream (20480 rows of 512 experts, N 1024, C 2048: 383 us, 5.7 TB/s over 2.1 GB of
+// weights; 2030 rows, N 2560, C 640: 218 us, 7.4 TB/s); with many the loads: alone they bring in 23 bytes per clock and CU (at the matrix cores'
+// peak 256 x 256 needs 32, 128 x 256 needs 48), whether the lines come from L2 or beyond, and the L1's counters say that it
+// stands half of the time for lines under way. 256 x 256: 16384 rows of 8 experts (N, C 4096) 565 us, 970 TFLOP/s, matrix cores 57% busy; one group of
+// 8192 rows (N 8192, C 4096) 476 us, 1155 TFLOP/s, and 365 us of products without the loads. LDS is busy a quarter of the time, without conflicts.
+//
+// Measured: four waves of 128 x 128 instead of eight 505 against 455 us (one group of 8192); stages of 64 values in two slots for the largest
+// tile 476 against 450, of 32 values for 128 x 256 (half a line per row) 545 against 383 (20480 rows); 64 x 256 397, 128 x 128 430; row tiles of a
+// group one by one instead of RB at a time 394 against 305 (loads alone); all groups' weights kept in L2 416 against 383. Without gain: another
+// first stage in each workgroup, lines brought into L2 ahead (a load per line, 480 -> 610 us), other cache policies, longer rings.
 template <typename T, Mode MODE, bool EIGHT, int BM, int BN, int WM, int WN, int ST, int KB, int OR, int OCC>
 __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs p, TileGrid grid) {
     constexpr int NW = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32, BK = KB * 8, SP = KB / 2;
@@ -361,7 +383,10 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
     bool once = grid.stream;
     if constexpr (MODE == kWgrad) {
         int index;
-        if (grid.sorted) {   // the groups' sizes differ, and with them their tiles' work: the largest first, their row tiles round the XCDs
+        // The groups' sizes differ, and with them their tiles' work: the largest first, their row tiles round the XCDs (65536 rows of 128 experts
+        // with 100 to 4800 each, 2048 x 1024: 389 us; in the groups' order 420, a group's tiles on one XCD 759). Short groups' time is their
+        // results', which eighths write better (20480 rows of 512 experts, 1280 x 2560 fp32: 1255 against 1363).
+        if (grid.sorted) {
             const int j = order(b >> 3, (p.E * grid.nx - int(xcd) + 7) / 8);
             index = j < 0 ? -1 : j * 8 + int(xcd);
         } else {
@@ -454,7 +479,9 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
         }
     };
     fetch();
-    // 8-bit rows of a: the codes and scales of the stage after the next one, and the next one's values into LDS (zeros past the group's rows and a's
+    // 8-bit rows of a go through registers, since they have to become values of T, as many bytes again, on the way: a stage's codes are loaded a
+    // stage ahead and written behind the barrier that frees their slot (65536 rows of 128 experts, 2048 x 1024: 515 us against 408 from rows in 16 bits;
+    // through the 64 x 64 tiles 1292). The codes and scales of the stage after the next one, and the next one's values into LDS (zeros past the group's rows and a's
     // columns, and for a row that there is not)
     int ef = ft, est = 0;   // the stage whose codes are loaded next
     i4_t codes[EIGHT ? CY : 1];
@@ -744,7 +771,9 @@ static int tiles_go(const char* what, const ProductArgs& p, hipStream_t stream) 
     const int64_t likely = MODE == kWgrad ? tiles : grouped ? std::max<int64_t>(p.M / BM + groups / 2, groups) : tiles;
     const int64_t K = MODE == kProduct ? p.C : MODE == kGrad ? p.N : p.M / groups;
     const int nst = int(std::max<int64_t>(1, (K + KB * 8 - 1) / (KB * 8)));
-    // (values in units of 64: one token's down products want several tiles of a short row behind one start, 40 rows of 512 experts one)
+    // (in units of 64 values: a workgroup takes about 4 us to begin and end. 40 / 64 / 128 and at least 512 workgroups: 20480 rows, C 2048, 382 / 381 /
+    // 381 us; 2030 rows, C 640, 218 / 218 / 248; 640 rows, C 2048, 227 / 235 / 255; rows' gradients of 17770, N 2048, 187 / 209 / 209. Weights'
+    // gradients of groups by size, 65536 rows: 8 / 16 / 32 425 / 389 / 569; short ones 1259 / 1300 / 1296)
     constexpr int kFill = 512;
     const int kStages = (MODE == kWgrad ? sorted ? 16 : 8 : 40) * 8 / KB;
     int nchunk = std::max(1, std::min(kStages / nst, ny));
@@ -771,7 +800,9 @@ __device__ __forceinline__ f4_t mma16(Vec<__bf16> w, Vec<__bf16> x, f4_t acc) { 
 // 16 features x 16 rows by KW waves that share the values of a row, straight from global memory into the registers of the matrix
 // instructions. The weights are the first operand, so that a lane's four results are adjacent features of one row. A group of 128 values is 16
 // chunks: step i multiplies chunks 4 i + l / 16 of lane l's feature and row. Wave w takes the groups w, w + KW, ..., two at a time in
-// flight; the waves' sums are added in their order. Rows and features past the end are the last one again, never stored.
+// flight; the waves' sums are added in their order. Rows and features past the end are the last one again, never stored. Bound by the chain of
+// trips to memory (bounds, then the row's index and the weights, then the activations): one token's ten experts (N 1024, C 2048, 42 MB)
+// 12.3 us; weights not kept in L2 13.3.
 template <typename T, int KW>
 __global__ void __launch_bounds__(256) k_product_rows(ProductArgs p, int ntile, FastDiv ntiles) {
     constexpr int FW = 4 / KW, V = Chunk<T>::V, P = 2;   // tiles of a workgroup; groups in flight (four: 5% slower)
@@ -864,6 +895,11 @@ static int tiles_t(const char* what, const ProductArgs& p, hipStream_t stream) {
     auto tiles = [&](int64_t BM, int64_t BN) {   // were the rows spread evenly
         return (MODE == kWgrad ? p.E * ((p.N + BM - 1) / BM) : (avg + BM - 1) / BM * groups) * ((features + BN - 1) / BN);
     };
+    // us at 256 x 256 / 128 x 256 / 64 x 128:
+    //   16384 rows of 8 experts (N, C 4096) 570 / 592; 65536 of 128 (N 2048, C 1024) 363 / 370 / 479; one group of 8192 (N 8192, C 4096) 488 / 521
+    //   20480 rows of 512 experts (N 1024, C 2048) 555 / 383 / 416; 2030 rows (N 2560, C 640) 358 / 230 / 221; 640 rows 345 / 247 / 228
+    //   one group of 2048 rows (N, C 2560) 61 / 36 / 48, of 512 61 / 36 / 22; 8 experts of 64 rows (N, C 2048) 48 / 31 / 22
+    //   weights' gradients: 65536 rows of 128 experts 389 / 475; 8192 of 128 (1024 x 1024) 139 / 138 / 143; one group of 4096 (768 x 1408) 94 / 58 / 41
     if constexpr (MODE == kWgrad) {
         if (tiles(256, 256) >= 256)
             return tiles_go<T, MODE, EIGHT, 256, 256, 2, 4, 4, 4, 32, 2>(what, p, stream);
