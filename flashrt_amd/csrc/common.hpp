@@ -219,10 +219,10 @@ __device__ __forceinline__ float half_max(float v) {
     const float b = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
     return (threadIdx.x & 32) ? b : a;
 }
-// A grid of fewer than 2^31 workgroups of up to 256 threads (a launch has fewer than 2^32 threads in a dimension), in two dimensions
-// beyond 2^23 of them; a few workgroups may lie past the last one asked for.
-inline dim3 wide_grid(uint32_t wgs) {
-    const uint32_t y = uint32_t((uint64_t(wgs) + (1u << 23) - 1) >> 23);
+// A grid of fewer than 2^31 workgroups of up to 1024 threads (a launch has fewer than 2^32 threads in a dimension), in two dimensions
+// beyond 2^31 threads; a few workgroups may lie past the last one asked for.
+inline dim3 wide_grid(uint32_t wgs, uint32_t threads = 256) {
+    const uint32_t most = (1u << 31) / threads, y = uint32_t((uint64_t(wgs) + most - 1) / most);
     return dim3((wgs + y - 1) / y, y);
 }
 __device__ __forceinline__ uint32_t wide_block() { return blockIdx.y * gridDim.x + blockIdx.x; }

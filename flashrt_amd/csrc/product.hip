@@ -137,22 +137,25 @@ __device__ __forceinline__ void store4(const ProductArgs& p, int64_t at, f4_t v,
         store4(static_cast<__bf16*>(p.out) + at, v, left, p.add);
 }
 
-// Rows at any distance and alignment: a tile of BM rows x BN features by WM x WN waves, one stage of LDS, the next stage's operands in registers
-// while this one is multiplied; what hides the loads' latency is the other workgroups of the CU (eight at 64 x 64). 1542 rows of 128 experts (N
-// 1021, C 1019, fp16, 267 MB of weights) 69 us, about the time of the other kernels at C 1024; 16384 rows 171 us, 200 TFLOP/s, against 148 to 183 with
-// tiles of 32 x 128 to 128 x 256 (rows' gradients 222 / 259 to 364, weights' 268 / 267 to 431). fp32 (8192 rows of 128 experts, N 2048, C 1024) 490
-// us, 70 TFLOP/s of the library's 153 at 8192^3. Whole stages without the checks of single pieces gave nothing.
-template <typename T, Mode MODE, bool EIGHT, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN) k_product_any(ProductArgs p, int nx, int ny, FastDiv divx, FastDiv divy) {
+// Rows at any distance and alignment, and calls of few tiles: a tile of BM rows x BN features by KS times WM x WN waves, each share of which
+// takes every KS-th stage of the summed values into its own LDS, the next one's operands in registers while this one is multiplied; the shares'
+// sums are added through LDS in their order. What hides the loads' latency is the other shares and the other workgroups of the CU. 1542 rows of
+// 128 experts (N 1021, C 1019, fp16, 267 MB of weights) 62 us, about the time of the other kernels at C 1024; 16384 rows 136 us, 250 TFLOP/s; fp32
+// (8192 rows, N 2048, C 2048) 119 TFLOP/s of the library's 153 at 8192^3. Whole stages without the checks of single pieces gave nothing.
+template <typename T, Mode MODE, bool EIGHT, int BM, int BN, int WM, int WN, int KS>
+__global__ void __launch_bounds__(64 * WM * WN * KS) k_product_any(ProductArgs p, int nx, int ny, FastDiv divx, FastDiv divy) {
     constexpr int NT = 64 * WM * WN, V = Chunk<T>::V, FM = BM / WM / 32, FN = BN / WN / 32;
     constexpr bool XCOL = MODE == kWgrad, YCOL = MODE != kProduct;
     using SX = Stage<T, BM, XCOL, 8>;
     using SY = Stage<T, BN, YCOL, 8>;
     constexpr int PX = BM * 8 / NT, PY = BN * 8 / NT, BK = SX::BK;
     static_assert(BM * 8 % NT == 0 && BN * 8 % NT == 0, "whole pieces per thread");
-    __shared__ __align__(16) uint8_t s_x[SX::bytes], s_y[SY::bytes];
-    __shared__ int s_row[BM];
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int kg = __builtin_amdgcn_readfirstlane(threadIdx.x / NT), tid = threadIdx.x % NT;   // the share of the stages, and the thread in it
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    uint8_t* const s_x = smem + kg * (SX::bytes + SY::bytes);
+    uint8_t* const s_y = s_x + SX::bytes;
+    int* const s_row = reinterpret_cast<int*>(smem + KS * (SX::bytes + SY::bytes));   // [BM]
     const uint32_t unit = wide_block(), outer = divy(unit);
     const int y0 = int(unit - outer * ny) * BN;
     int g, x0, xn, K, k_first = 0;   // the tile's group, first row and rows, and the contracted values (from k_first on)
@@ -171,7 +174,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_product_any(ProductArgs p, int
         x0 = t.row0;
         xn = t.rows;
         K = MODE == kProduct ? p.C : p.N;
-        for (int i = tid; i < BM; i += NT) {
+        for (int i = threadIdx.x; i < BM; i += NT * KS) {
             const int r = x0 + min(i, xn - 1);
             const int a = p.rows ? p.rows[r] : r;
             s_row[i] = i < xn && unsigned(a) < unsigned(p.a_rows) ? a : -1;
@@ -217,15 +220,31 @@ __global__ void __launch_bounds__(64 * WM * WN) k_product_any(ProductArgs p, int
         }
     };
     const int wm = wave / WN * FM * 32, wn = wave % WN * FN * 32;
-    f16_t acc[FM][FN];
+    // Sums of fp32 operands are formed in two steps, of kPart stages (256 values) and of these, so that their error grows with the
+    // two lengths and not with their product; 16-bit ones' add sixteen products at a time as it is.
+    constexpr bool PARTS = sizeof(T) == 4;
+    constexpr int kPart = 8;
+    f16_t acc[FM][FN], sum[FM][FN];
+    auto clear = [&](f16_t (&v)[FM][FN]) INLINE {
 #pragma unroll
-    for (int m = 0; m < FM; ++m)
+        for (int m = 0; m < FM; ++m)
 #pragma unroll
-        for (int f = 0; f < FN; ++f)
+            for (int f = 0; f < FN; ++f)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[m][f][i] = 0.0f;
-    if (K > 0) load(0);
-    for (int k0 = 0; k0 < K; k0 += BK) {
+                for (int i = 0; i < 16; ++i) v[m][f][i] = 0.0f;
+    };
+    auto add = [&](f16_t (&v)[FM][FN], const f16_t (&w)[FM][FN]) INLINE {
+#pragma unroll
+        for (int m = 0; m < FM; ++m)
+#pragma unroll
+            for (int f = 0; f < FN; ++f) v[m][f] += w[m][f];
+    };
+    clear(acc);
+    clear(sum);
+    const int step = BK * KS;   // (a share past the values multiplies zeros)
+    int part = 0;
+    if (K > 0) load(kg * BK);
+    for (int k0 = kg * BK; k0 - kg * BK < K; k0 += step) {
         __syncthreads();   // every wave has read the stage before
 #pragma unroll
         for (int i = 0; i < PX; ++i) {
@@ -238,7 +257,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_product_any(ProductArgs p, int
             *reinterpret_cast<Vec<T>*>(s_y + SY::piece(q / SY::PR, q % SY::PR)) = ry[i];
         }
         __syncthreads();
-        if (K - k0 > BK) load(k0 + BK);
+        if (K - (k0 - kg * BK) > step) load(k0 + step);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             Vec<T> b[FN];
@@ -251,6 +270,30 @@ __global__ void __launch_bounds__(64 * WM * WN) k_product_any(ProductArgs p, int
                 for (int f = 0; f < FN; ++f) acc[m][f] = mma(b[f], a, acc[m][f]);
             }
         }
+        if (PARTS && ++part == kPart) {
+            part = 0;
+            add(sum, acc);
+            clear(acc);
+        }
+    }
+    if constexpr (PARTS) add(acc, sum);
+    if constexpr (KS > 1) {   // the shares' sums, in their order
+        static_assert(BM * BN * 4 <= SX::bytes + SY::bytes, "a share's sums in its stage");
+        __syncthreads();
+        f16_t* const mine = reinterpret_cast<f16_t*>(s_x);
+#pragma unroll
+        for (int m = 0; m < FM; ++m)
+#pragma unroll
+            for (int f = 0; f < FN; ++f) mine[(m * FN + f) * NT + tid] = acc[m][f];
+        __syncthreads();
+        if (kg != 0) return;
+#pragma unroll
+        for (int j = 1; j < KS; ++j)
+#pragma unroll
+            for (int m = 0; m < FM; ++m)
+#pragma unroll
+                for (int f = 0; f < FN; ++f)
+                    acc[m][f] += reinterpret_cast<const f16_t*>(smem + j * (SX::bytes + SY::bytes))[(m * FN + f) * NT + tid];
     }
     // Lane l's value i of a fragment: feature 8 (i / 4) + 4 (l / 32) + i % 4, row l % 32
     const int64_t out0 = MODE == kWgrad ? int64_t(g) * p.N * p.C : 0;
@@ -269,15 +312,47 @@ __global__ void __launch_bounds__(64 * WM * WN) k_product_any(ProductArgs p, int
     }
 }
 
-template <typename T, Mode MODE, bool EIGHT, int BM, int BN, int WM, int WN>
+template <typename T, Mode MODE, bool EIGHT, int BM, int BN, int WM, int WN, int KS>
 static int any_go(const char* what, const ProductArgs& p, hipStream_t stream) {
     const int features = MODE == kProduct ? p.N : p.C, ny = (features + BN - 1) / BN, nx = (p.N + BM - 1) / BM;
     const int64_t units = (MODE == kWgrad ? int64_t(p.E) * nx : tiles_at_most(p.M, p.E, BM, p.bounds != nullptr)) * ny;
+    constexpr int smem = KS * (BM + BN) * 128 + BM * 4;
+    static_assert(smem <= 160 * 1024 && 64 * WM * WN * KS <= 1024, "LDS of a CU, threads of a workgroup");
     if (units > 0x7ffff000) return set_error(kErrShape, "%s: M=%d N=%d C=%d E=%d", what, p.M, p.N, p.C, p.E);
-    launch_timed(what, k_product_any<T, MODE, EIGHT, BM, BN, WM, WN>, wide_grid(uint32_t(units)), dim3(64 * WM * WN), 0, stream, p, nx, ny,
-                 FastDiv(uint32_t(nx)), FastDiv(uint32_t(ny)));
+    if constexpr (smem > 64 * 1024)
+        FRT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_product_any<T, MODE, EIGHT, BM, BN, WM, WN, KS>),
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, smem));
+    launch_timed(what, k_product_any<T, MODE, EIGHT, BM, BN, WM, WN, KS>, wide_grid(uint32_t(units), 64 * WM * WN * KS), dim3(64 * WM * WN * KS), smem,
+                 stream, p, nx, ny, FastDiv(uint32_t(nx)), FastDiv(uint32_t(ny)));
     FRT_LAUNCHED(what);
     return kOk;
+}
+// A group's rows, and the tiles of BM x BN that a call has, were the rows spread evenly over the groups that can have some
+static int64_t even_rows(const ProductArgs& p) { return p.M / (p.bounds ? std::min(p.E, std::max(p.M, 1)) : 1); }
+template <Mode MODE>
+static int64_t even_tiles(const ProductArgs& p, int64_t BM, int64_t BN) {
+    const int64_t groups = p.bounds ? std::min(p.E, std::max(p.M, 1)) : 1;
+    return (MODE == kWgrad ? p.E * ((p.N + BM - 1) / BM) : (even_rows(p) + BM - 1) / BM * groups) * (((MODE == kProduct ? p.N : p.C) + BN - 1) / BN);
+}
+// Up to as many tiles of 64 x 64 as CUs leave CUs or their matrix cores idle, so the summed values are shared out over a workgroup's waves,
+// the more of them the fewer tiles there are; many tiles are read the less often the larger they are.
+// us, 32 x 32 over 16 shares / 64 x 64 over 4 / over 2 / undivided / 128 x 128:
+//   16-bit product, N and C odd: 128 experts of 4 rows (N 1021, C 1019) 40 / 18 / 16 / 19 / 21, of 12 rows 185 / 73 / 62 / 69 / 64; one group of
+//   4096 rows (C 2047, N 2048) 497 / 118 / 99 / 99 / 63, of 1024 rows (N 1024) 126 / 33 / 30 / 36 / 47
+//   weights' gradient (N 511, C 509) of one group of 8192 rows 81 / 132 / 196 / 346 / 533; of 2048 rows each, four groups 87 / 39 / 57 / 96 / 111,
+//   sixteen 346 / 148 / 147 / 143 / 119
+//   fp32 (N 2048, C 2048): one group of 4096 rows 651 / 411 / 377 / 366 / 287 (119 TFLOP/s), of 1024 165 / 105 / 99 / 109 / 159
+// fp32 rows, whose products take their tile's time whether its rows are there or not, in tiles of 32 rows where the groups are shorter:
+// 128 experts (N 1024, C 768) of 8 rows 205 / 176 / 146 / 137, 32 x 64 over 8 shares 131; of one row 28 / 24 / 25 / 32, 18.
+template <typename T, Mode MODE, bool EIGHT = false>
+static int any_t(const char* what, const ProductArgs& p, hipStream_t stream) {
+    const int64_t tiles = even_tiles<MODE>(p, 64, 64), rows = even_rows(p);
+    if (tiles <= 96) return any_go<T, MODE, EIGHT, 32, 32, 1, 1, 16>(what, p, stream);
+    if constexpr (sizeof(T) == 4 && MODE != kWgrad)
+        if (rows <= 32) return any_go<T, MODE, EIGHT, 32, 64, 1, 2, 8>(what, p, stream);
+    if (tiles <= 256) return any_go<T, MODE, EIGHT, 64, 64, 2, 2, 4>(what, p, stream);
+    if (tiles < 1024 || (MODE != kWgrad && rows <= 64)) return any_go<T, MODE, EIGHT, 64, 64, 2, 2, 2>(what, p, stream);
+    return any_go<T, MODE, EIGHT, 128, 128, 2, 4, 1>(what, p, stream);
 }
 
 // ---------------------------------------------------------------- tiles through direct loads
@@ -890,11 +965,12 @@ static bool pieces(const ProductArgs& p, int x_cols, bool wgrad) {
 }
 template <typename T, Mode MODE, bool EIGHT = false>
 static int tiles_t(const char* what, const ProductArgs& p, hipStream_t stream) {
-    const int64_t groups = p.bounds ? std::min(p.E, std::max(p.M, 1)) : 1, avg = p.M / groups;
-    const int features = MODE == kProduct ? p.N : p.C;
-    auto tiles = [&](int64_t BM, int64_t BN) {   // were the rows spread evenly
-        return (MODE == kWgrad ? p.E * ((p.N + BM - 1) / BM) : (avg + BM - 1) / BM * groups) * ((features + BN - 1) / BN);
-    };
+    const int64_t rows = even_rows(p);
+    const auto tiles = [&](int64_t BM, int64_t BN) { return even_tiles<MODE>(p, BM, BN); };
+    // As few tiles as leave CUs idle share the summed values out. us, so / in tiles of 64 x 128: row gradients, one row (N 1024, C 2048) 8.2 / 12.1,
+    // 16 rows (N 2560, C 640) 11.7 / 22.6, 2048 rows (512 x 512) 8.4 / 9.4; weights' gradients, one group of 8192 rows (512 x 512) 33 / 83,
+    // of 2048 10.7 / 26.3. Just beyond: 16 groups of a row (N 768, C 2048) 13.0 / 12.1, 8 groups of 2048 rows 28.9 / 27.5
+    if (tiles(64, 64) <= 256) return any_t<T, MODE, EIGHT>(what, p, stream);
     // us at 256 x 256 / 128 x 256 / 64 x 128:
     //   16384 rows of 8 experts (N, C 4096) 570 / 592; 65536 of 128 (N 2048, C 1024) 363 / 370 / 479; one group of 8192 (N 8192, C 4096) 488 / 521
     //   20480 rows of 512 experts (N 1024, C 2048) 555 / 383 / 416; 2030 rows (N 2560, C 640) 358 / 230 / 221; 640 rows 345 / 247 / 228
@@ -904,8 +980,8 @@ static int tiles_t(const char* what, const ProductArgs& p, hipStream_t stream) {
         if (tiles(256, 256) >= 256)
             return tiles_go<T, MODE, EIGHT, 256, 256, 2, 4, 4, 4, 32, 2>(what, p, stream);
     } else {
-        if (avg >= 1024 && tiles(256, 256) >= 512) return tiles_go<T, MODE, EIGHT, 256, 256, 2, 4, 4, 4, 32, 2>(what, p, stream);
-        if (avg > 16 && tiles(128, 256) >= 128) return tiles_go<T, MODE, EIGHT, 128, 256, 2, 4, 3, 8, 16, 2>(what, p, stream);
+        if (rows >= 1024 && tiles(256, 256) >= 512) return tiles_go<T, MODE, EIGHT, 256, 256, 2, 4, 4, 4, 32, 2>(what, p, stream);
+        if (rows > 16 && tiles(128, 256) >= 128) return tiles_go<T, MODE, EIGHT, 128, 256, 2, 4, 3, 8, 16, 2>(what, p, stream);
     }
     return tiles_go<T, MODE, EIGHT, 64, 128, 2, 2, 3, 8, 16, 2>(what, p, stream);
 }
@@ -917,26 +993,28 @@ static int product_t(const ProductArgs& p, hipStream_t stream) {
             // The weights that tiles of 16 rows read: up to 256 MB straight into registers, with the values over the waves where those are
             // few; beyond, in tiles through LDS. us, one wave / two / four to a row / tiles: one token's ten experts (N 1024, C 2048, 42
             // MB) 12.9 / 12.9 / 12.3 / 19.5, two tokens' 21.7 / 18.3 / 19.4 / 22.3, four 31 / 29 / 35 / 32, sixteen (600 MB) 114 / 109 /
-            // 122 / 99; N 2560, C 640 9.6 / 11.7 / 14.0 / 12.0; one group (N 8192, C 4096) of a row 20.9 / 20.2 / 15.6 / 34.7
-            const int64_t groups = p.bounds ? std::min(p.E, p.M) : 1, units = (p.M / groups + 15) / 16 * groups * ((p.N + 15) / 16);
-            if (units * 32 * p.C <= int64_t(256) << 20)
+            // 122 / 99; N 2560, C 640 9.6 / 11.7 / 14.0 / 12.0; one group (N 8192, C 4096) of a row 20.9 / 20.2 / 15.6 / 34.7.
+            // Weights that more than one tile reads, up to 32 MB. us, so / in tiles: one group of 256 rows (N 512, C 1024, 17 MB) 7.4 /
+            // 8.2, of 128 (N 1024, C 2048, 34 MB) 9.7 / 10.0, of 2048 (512 x 512, 67 MB) 17.2 / 8.3, of 256 (N 2048, C 2048, 134 MB) 31 / 15
+            const int64_t rows = even_rows(p), units = even_tiles<kProduct>(p, 16, 16);
+            if (units <= (int64_t(rows <= 16 ? 256 : 32) << 20) / 32 / p.C)
                 return units <= 640 && p.C >= 512 ? rows_go<T, 4>(p, stream) : units <= 1280 && p.C >= 256 ? rows_go<T, 2>(p, stream) : rows_go<T, 1>(p, stream);
             return tiles_t<T, kProduct>("moe_product", p, stream);
         }
-    return any_go<T, kProduct, false, 64, 64, 2, 2>("moe_product", p, stream);
+    return any_t<T, kProduct>("moe_product", p, stream);
 }
 template <typename T>
 static int grad_t(const ProductArgs& p, hipStream_t stream) {
     if constexpr (sizeof(T) == 2)
         if (pieces<T>(p, p.N, false)) return tiles_t<T, kGrad>("moe_product_grad", p, stream);
-    return any_go<T, kGrad, false, 64, 64, 2, 2>("moe_product_grad", p, stream);
+    return any_t<T, kGrad>("moe_product_grad", p, stream);
 }
 template <typename T>
 static int wgrad_t(const ProductArgs& p, hipStream_t stream) {
     if constexpr (sizeof(T) == 2)
         if (pieces<T>(p, p.N, true))
             return p.scales ? tiles_t<T, kWgrad, true>("moe_product_wgrad", p, stream) : tiles_t<T, kWgrad>("moe_product_wgrad", p, stream);
-    return p.scales ? any_go<T, kWgrad, true, 64, 64, 2, 2>("moe_product_wgrad", p, stream) : any_go<T, kWgrad, false, 64, 64, 2, 2>("moe_product_wgrad", p, stream);
+    return p.scales ? any_t<T, kWgrad, true>("moe_product_wgrad", p, stream) : any_t<T, kWgrad>("moe_product_wgrad", p, stream);
 }
 
 int moe_product(int type, const ProductArgs& p, hipStream_t stream) { return FRT_BY_TYPE(type, product_t, p, stream); }

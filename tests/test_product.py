@@ -287,11 +287,11 @@ KERNELS = {
     "product 128, picked": ("product", ragged(33, 1, 140), 1004, 1032, 300),
     "product 256": ("product", [1111, 1300], 13320, 264, 0),
     "product 256, picked": ("product", [1536, 1027], 13316, 136, 600),
-    "grad 64": ("grad", ragged(20, 0, 70), 200, 328, 0),
+    "grad 64": ("grad", ragged(90, 0, 70), 200, 328, 0),
     "grad 128": ("grad", ragged(33, 1, 300), 264, 1000, 0),
     "grad 256": ("grad", [1111, 1300], 200, 13320, 0),
-    "wgrad 64": ("wgrad", ragged(9, 0, 300), 200, 328, 0),
-    "wgrad 64, picked": ("wgrad", ragged(9, 0, 300), 328, 136, 70),
+    "wgrad 64": ("wgrad", ragged(24, 0, 300), 200, 328, 0),
+    "wgrad 64, picked": ("wgrad", ragged(24, 0, 300), 328, 136, 70),
     "wgrad 256": ("wgrad", ragged(70, 0, 400), 328, 520, 0),
     "wgrad 256, picked": ("wgrad", ragged(70, 0, 400), 264, 776, 70),
 }
@@ -327,6 +327,63 @@ def test_8_bit_rows_in_every_kernel(shape, C, kind):
 def test_added_in_every_kernel(shape, eight, out_kind):
     op, sizes, N, C, _ = KERNELS[shape]
     run(op, sizes, N, C // 32 * 32, BF16, out_kind, eight=eight, add=True)
+
+
+# Shapes that each form of the kernel for rows at any alignment takes, by tile and shares of the summed values; beside these, every call of few tiles
+ANY = {
+    "32 x 64 over 8, fp32": ("product", ragged(40, 0, 20), 201, 333, 0),
+    "32 x 64 over 8, fp32, picked": ("product", ragged(40, 0, 20), 201, 333, 50),
+    "32 x 64 over 8, fp32, gradient": ("grad", ragged(40, 0, 20), 333, 201, 0),
+    "64 x 64 over 4": ("product", [70, 0, 130], 1801, 1300, 0),
+    "64 x 64 over 4, gradient": ("grad", [70, 0, 130], 1300, 1801, 0),
+    "64 x 64 over 4, weights": ("wgrad", [300, 0, 77], 500, 501, 0),
+    "64 x 64 over 2": ("product", ragged(20, 0, 90), 1275, 1111, 60),
+    "64 x 64 over 2, gradient": ("grad", ragged(20, 0, 90), 1111, 1275, 0),
+    "64 x 64 over 2, weights": ("wgrad", [300, 0, 77], 700, 801, 200),
+    "128 x 128": ("product", [300, 0, 411], 8261, 137, 0),
+    "128 x 128, gradient": ("grad", [300, 0, 411], 137, 8261, 0),
+    "128 x 128, weights": ("wgrad", ragged(6, 0, 300), 1021, 1019, 0),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("shape", list(ANY))
+def test_every_form_at_any_alignment(shape, kind):
+    op, sizes, N, C, gather = ANY[shape]
+    run(op, sizes, N, C, kind, kind, gather=gather, pad=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("add", [False, True])
+@pytest.mark.parametrize("shape,N,C", [("64 x 64 over 4, weights", 501, 480), ("64 x 64 over 2, weights", 701, 800), ("128 x 128, weights", 1021, 1024)])
+def test_8_bit_rows_in_every_form(shape, N, C, add, kind):
+    op, sizes, _, _, gather = ANY[shape]
+    run(op, sizes, N, C, kind, F32, gather=gather, eight=True, add=add)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["product", "grad", "wgrad"])
+def test_fp32_sums_of_long_rows(op):
+    """8192 values summed in fp32 in two steps, of 256 and of these, and over shares: within 300 half steps of the sum of the products' sizes, where one
+    after the other may take 8192."""
+    m, n = 8192, 40
+    N, C, M = {"product": (n, m, 70), "grad": (m, n, 70), "wgrad": (n, n, m)}[op]
+    import flashrt_amd as F
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x, d, w = (torch.rand(*s, generator=g, device="cuda") for s in ((M, C), (M, N), (1, N, C)))
+    out = torch.empty({"product": (M, N), "grad": (M, C), "wgrad": (1, N, C)}[op], device="cuda")
+    if op == "product":
+        F.moe_product(x, w[0], out)
+        want = x.double() @ w[0].double().t()
+    elif op == "grad":
+        F.moe_product_grad(d, w[0], out)
+        want = d.double() @ w[0].double()
+    else:
+        F.moe_product_wgrad(d, x, out[0])
+        want = (d.double().t() @ x.double())[None]
+    assert ((out.double() - want).abs() <= 300 * 2.0 ** -24 * want).all()
 
 
 # ---------------------------------------------------------------- values, bounds, offsets
@@ -444,17 +501,17 @@ def test_rows_far_apart(op):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("kind", [BF16, F32])
-def test_more_rows_than_one_grid_dimension(kind):
-    """Nearly 2^30 rows of eight values (2^28 in fp32): more workgroups than one dimension of a launch holds, offsets past 32 bits. The rows
-    repeat, in small whole numbers, so that every sum is exact."""
+@pytest.mark.parametrize("kind,N,M", [(BF16, 8, (1 << 30) - 3), (F32, 8, (1 << 28) + 5), (F32, 2, (1 << 30) - 3)])
+def test_more_rows_than_one_grid_dimension(kind, N, M):
+    """Nearly 2^30 rows of eight values (two, or 2^28 rows, in fp32): more workgroups than one dimension of a launch holds, offsets past 32 bits. The
+    rows repeat, in small whole numbers, so that every sum is exact."""
     import flashrt_amd as F
-    n, M = 1 << 16, (1 << 30) - 3 if kind is BF16 else (1 << 28) + 5
+    n = 1 << 16
     g = torch.Generator(device="cuda").manual_seed(1)
-    rows = torch.randint(-8, 9, (n, 8), generator=g, device="cuda").to(kind)
-    w = torch.randint(-8, 9, (8, 8), generator=g, device="cuda").to(kind)
+    rows = torch.randint(-8, 9, (n, N), generator=g, device="cuda").to(kind)
+    w = torch.randint(-8, 9, (N, N), generator=g, device="cuda").to(kind)
     a = rows.repeat((M + n - 1) // n, 1)[:M]
-    out = torch.empty(M, 8, dtype=kind, device="cuda")
+    out = torch.empty(M, N, dtype=kind, device="cuda")
     F.moe_product(a, w, out)
     want = (rows.double() @ w.double().t()).to(kind)
     for r in range(0, M, n):
