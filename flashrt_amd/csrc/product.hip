@@ -143,7 +143,7 @@ __device__ __forceinline__ void store4(const ProductArgs& p, int64_t at, f4_t v,
 // 128 experts (N 1021, C 1019, fp16, 267 MB of weights) 62 us, about the time of the other kernels at C 1024; 16384 rows 136 us, 250 TFLOP/s; fp32
 // (8192 rows, N 2048, C 2048) 119 TFLOP/s of the library's 153 at 8192^3. Whole stages without the checks of single pieces gave nothing.
 template <typename T, Mode MODE, bool EIGHT, int BM, int BN, int WM, int WN, int KS>
-__global__ void __launch_bounds__(64 * WM * WN * KS) k_product_any(ProductArgs p, int nx, int ny, FastDiv divx, FastDiv divy) {
+__global__ void __launch_bounds__(64 * WM * WN * KS, BM == 128 ? 4 : 1) k_product_any(ProductArgs p, int nx, int ny, FastDiv divx, FastDiv divy) {
     constexpr int NT = 64 * WM * WN, V = Chunk<T>::V, FM = BM / WM / 32, FN = BN / WN / 32;
     constexpr bool XCOL = MODE == kWgrad, YCOL = MODE != kProduct;
     using SX = Stage<T, BM, XCOL, 8>;
