@@ -9,16 +9,17 @@ namespace frt {
 __device__ __forceinline__ float mx8_scale(uint32_t b) {
     return __builtin_bit_cast(float, b == 255u ? 0x7fc00000u : b ? b << 23 : 0x00400000u);
 }
-// Eight codes' values, two words of four codes each
-__device__ __forceinline__ auto mx8_values(uint32_t lo, uint32_t hi, float scale) {
-    typedef float f8 __attribute__((ext_vector_type(8)));
-    f8 v;
+// Four codes' values, of a word, and eight, of two
+__device__ __forceinline__ auto mx8_values(uint32_t w, float scale) {
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    f4 v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        v[j] = float(int(lo << (24 - 8 * j)) >> 24) * scale;
-        v[j + 4] = float(int(hi << (24 - 8 * j)) >> 24) * scale;
-    }
+    for (int j = 0; j < 4; ++j) v[j] = float(int(w << (24 - 8 * j)) >> 24) * scale;
     return v;
+}
+__device__ __forceinline__ auto mx8_values(uint32_t lo, uint32_t hi, float scale) {
+    const auto l = mx8_values(lo, scale), h = mx8_values(hi, scale);
+    return __builtin_shufflevector(l, h, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 }  // namespace frt

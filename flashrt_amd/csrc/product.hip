@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
         K = MODE == kProduct ? p.C : p.N;
         once = once && t.only;
     }
-    const int features = MODE == kProduct ? p.N : p.C, nst = max(1, (K + BK - 1) / BK);
+    const int features = MODE == kProduct ? p.N : p.C, nst = EIGHT ? max(1, (K + 2 * BK - 1) / (2 * BK)) * 2 : max(1, (K + BK - 1) / BK);   // (8-bit rows: two by two)
     int ft = chunk * grid.per;
     const int ft1 = min(ft + grid.per, grid.ny);
     const bool gather = MODE == kWgrad && p.rows;
@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
     };
     point();
     // gather: the rows of a's rows of the next stage, a stage ahead
-    constexpr int NI = EIGHT ? CY * NR : MODE == kWgrad ? DY * LY::RL : 1;
+    constexpr int NI = MODE == kWgrad && !EIGHT ? DY * LY::RL : 1;
     int index[NI] = {};
     auto fetch = [&]() INLINE {
         if (MODE == kWgrad && !EIGHT && gather && K > 0) {
@@ -554,58 +554,60 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
         }
     };
     fetch();
-    // 8-bit rows of a go through registers, since they have to become values of T, as many bytes again, on the way: a stage's codes are loaded a
-    // stage ahead and written behind the barrier that frees their slot (65536 rows of 128 experts, 2048 x 1024: 515 us against 408 from rows in 16 bits;
-    // through the 64 x 64 tiles 1292). The codes and scales of the stage after the next one, and the next one's values into LDS (zeros past the group's rows and a's
-    // columns, and for a row that there is not)
-    int ef = ft, est = 0;   // the stage whose codes are loaded next
-    i4_t codes[EIGHT ? CY : 1];
-    uint32_t scales[EIGHT ? CY : 1];
-    auto fetch8 = [&]() INLINE {
-        const int k0 = est * BK, lim = ef < ft1 ? K - k0 : 0;
-        const Buffer qb = buffer(y0 + (gather ? 0 : int64_t(k0) * p.C)), sb = buffer(p.scales + (gather ? 0 : (int64_t(k_first) + k0) * (p.C / 32)));
+    // 8-bit rows of a go through registers, since they have to become values of T, as many bytes again, on the way: a stage's codes are loaded two
+    // stages ahead into one of two sets (loads complete in order, so a wait for newer codes would wait for the operands behind them, too), the
+    // rows' indices two stages before those, and written between the products that follow the barrier that frees their slot (zeros past
+    // the group's rows and a's columns, and for a row that there is not). 65536 rows of 128 experts, 2048 x 1024: 424 us against 397 from rows in
+    // 16 bits; with one set 515, with indices in scalar registers, whose loads share a counter with LDS, 525; through the 64 x 64 tiles 1292.
+    const uint32_t blocks = uint32_t(p.C) / 32;
+    const uint8_t* const s0 = EIGHT ? p.scales + (gather ? 0 : int64_t(k_first) * blocks) : nullptr;
+    int ef = ft, est = 0;   // the feature tile and stage whose codes are loaded next
+    i4_t codes[2][EIGHT ? CY : 1];
+    uint32_t scales[2][EIGHT ? CY : 1], picks[2][EIGHT ? CY : 1];
+    auto pick8 = [&](int set, int st) INLINE {   // stage st's rows of a (in every call, so that the waits can count on it)
+        uint32_t ln = lane;
+        asm volatile("" : "+v"(ln));   // (addresses formed here, not all kept)
+        const Buffer rb = buffer(reinterpret_cast<const uint8_t*>(p.rows + (gather ? int64_t(k_first) + int64_t(st) * BK : 0)));
+        const int lim = gather ? K - st * BK : 0;
 #pragma unroll
         for (int i = 0; i < CY; ++i) {
-            const int first = (i * NW + wave) * NR, k = first + lane / (BN / 16), c = ef * BN + lane % (BN / 16) * 16;
-            bool in = k < lim && c < p.C;
-            uint32_t a = k;
-            if (gather) {
-#pragma unroll
-                for (int r = 0; r < NR; ++r) a = lane / (BN / 16) == r ? uint32_t(index[(i * NR + r) % NI]) : a;
-                in = in && a < uint32_t(p.a_rows);
-            }
-            codes[i] = __builtin_bit_cast(i4_t, __builtin_amdgcn_raw_buffer_load_b128(qb, in ? a * uint32_t(p.C) + c : kNone, 0, 0));
-            scales[i] = __builtin_amdgcn_raw_buffer_load_b8(sb, in ? a * uint32_t(p.C / 32) + c / 32 : kNone, 0, 0);
+            const int k = (i * NW + wave) * NR + ln / (BN / 16);
+            picks[set][i] = __builtin_amdgcn_raw_buffer_load_b32(rb, k < lim ? uint32_t(k) * 4 : kNone, 0, 0);
         }
+    };
+    auto fetch8 = [&](int set) INLINE {
+        uint32_t ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int k0 = est * BK, lim = ef < ft1 ? K - k0 : 0;
+        const Buffer qb = buffer(y0 + (gather ? 0 : int64_t(k0) * p.C)), sb = buffer(s0 + (gather ? 0 : int64_t(k0) * blocks));
+#pragma unroll
+        for (int i = 0; i < CY; ++i) {
+            const int k = (i * NW + wave) * NR + ln / (BN / 16), c = ef * BN + ln % (BN / 16) * 16;
+            const uint32_t a = gather ? picks[set][i] : uint32_t(k);
+            const bool in = (k < lim) & (c < p.C) & (!gather | (a < uint32_t(p.a_rows)));
+            uint32_t qo = in ? a * uint32_t(p.C) + c : kNone, so = in ? a * blocks + c / 32 : kNone;
+            asm volatile("" : "+v"(qo), "+v"(so));   // (one load whatever `in` is: with one on each side of a branch the second waits for the first)
+            codes[set][i] = __builtin_bit_cast(i4_t, __builtin_amdgcn_raw_buffer_load_b128(qb, qo, 0, 0));
+            scales[set][i] = __builtin_amdgcn_raw_buffer_load_b8(sb, so, 0, 0);
+        }
+        pick8(set, est + 2 < nst ? est + 2 : est + 2 - nst);
         if (++est == nst) {
             est = 0;
             ++ef;
         }
-        if (gather && K > 0) {
-            const int k = k_first + est * BK;
-#pragma unroll
-            for (int i = 0; i < NI; ++i) index[i] = uniform_load(p.rows + min(k + (i / NR * NW + wave) * NR + i % NR, p.M - 1));
-        }
     };
-    auto put8 = [&]() INLINE {
-        uint8_t* const s = smem + jslot * Sh::stage_b + BM * KB * 16;
-#pragma unroll
-        for (int i = 0; i < CY; ++i) {
-            const int k = (i * NW + wave) * NR + lane / (BN / 16), c = lane % (BN / 16) * 2;
-            const float scale = mx8_scale(scales[i]);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const auto f = mx8_values(codes[i][2 * h], codes[i][2 * h + 1], scale);
-                *reinterpret_cast<Vec<T>*>(s + LY::S::piece(k, c + h)) = __builtin_convertvector(f, Vec<T>);
-            }
-        }
+    auto put8 = [&](int set, int half) INLINE {   // eight codes (one of 2 CY)
+        uint32_t ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int i = half / 2, h = half % 2, k = (i * NW + wave) * NR + ln / (BN / 16), c = ln % (BN / 16) * 2;
+        const auto f = mx8_values(codes[set][i][2 * h], codes[set][i][2 * h + 1], mx8_scale(scales[set][i]));
+        *reinterpret_cast<Vec<T>*>(smem + jslot * Sh::stage_b + BM * KB * 16 + LY::S::piece(k, c + h)) = __builtin_convertvector(f, Vec<T>);
     };
     if constexpr (EIGHT) {
-        if (gather && K > 0) {
-#pragma unroll
-            for (int i = 0; i < NI; ++i) index[i] = uniform_load(p.rows + min(k_first + (i / NR * NW + wave) * NR + i % NR, p.M - 1));
-        }
-        fetch8();
+        pick8(0, 0);
+        pick8(1, 1);
+        fetch8(0);
+        fetch8(1);
     }
     // Load i of the next stage; past the last stage of the last feature tile zeros are loaded that nothing reads, so that the waits
     // can count on every load.
@@ -668,7 +670,7 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
             o.a[(i - FN) % FM] = LX::S::read(s, wm + 32 * (i - FN), t);
     };
     // A step's products, row by row, with the reads of the next step's operands and part `part` (of SP) of the next stage's loads between them
-    auto step = [&](auto on, const Ops& o, Ops& next, int slot, int t, int part) INLINE {
+    auto step = [&](auto on, const Ops& o, Ops& next, int slot, int t, int part, int set) INLINE {
 #pragma unroll
         for (int m = 0; m < FM; ++m) {
             if constexpr (decltype(on)::value) {
@@ -683,9 +685,11 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
             for (int i = 0; i < D; ++i)
                 if (i >= (part * FM + m) * D / (SP * FM) && i < (part * FM + m + 1) * D / (SP * FM)) load(i);
             if constexpr (EIGHT)
-                if (part == 0 && m == 0) {
-                    put8();
-                    fetch8();
+                if (part == 0) {
+#pragma unroll
+                    for (int h = 0; h < 2 * CY; ++h)
+                        if (h >= m * 2 * CY / FM && h < (m + 1) * 2 * CY / FM) put8(set, h);
+                    if (m == FM - 1) fetch8(set);
                 }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -693,7 +697,7 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
 
     // Waits count the loads: at the end of a stage those of ST - 2 stages were issued behind the next one's, and in a feature tile's first ST
     // - 1 stages the stores of the tile before (at least kStores per wave; with add, whose stores are not counted on, none).
-    constexpr int kStage = D + 2 * CY, kStores = FM * FN * 2, kCap = 63;
+    constexpr int kStage = D + 3 * CY, kStores = FM * FN * 2, kCap = 63;
     auto landed = [&](bool stores) INLINE {
         if (stores)
             wait_vm<(kStage * (ST - 2) + kStores < kCap ? kStage * (ST - 2) + kStores : kCap)>();
@@ -776,21 +780,23 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
         else
             results(__bf16(), std::false_type());
     };
-#pragma unroll 1
+#pragma unroll(EIGHT ? ST - 1 : 1)
     for (int s = 0; s < ST - 1; ++s) {
 #pragma unroll
         for (int i = 0; i < D; ++i) load(i);
         if constexpr (EIGHT) {
-            put8();
-            fetch8();
+#pragma unroll
+            for (int h = 0; h < 2 * CY; ++h) put8(s & 1, h);
+            fetch8(s & 1);
         }
         advance();
     }
 #pragma unroll
     for (int i = 0; i < D / SP; ++i) load(i);
     if constexpr (EIGHT) {
-        put8();
-        fetch8();
+#pragma unroll
+        for (int h = 0; h < 2 * CY; ++h) put8((ST - 1) & 1, h);
+        fetch8((ST - 1) & 1);
     }
     wait_vm<(kStage * (ST - 2) + D / SP < kCap ? kStage * (ST - 2) + D / SP : kCap)>();
     ring_barrier();
@@ -809,16 +815,24 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
             for (int f = 0; f < FN; ++f)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[m][f][i] = 0.0f;
-        auto stages = [&](auto on) INLINE {
-            for (int st = 0; st < nst; ++st) {
+        auto stage = [&](auto on, int st, int set) INLINE {
 #pragma unroll
-                for (int t = 0; t < SP - 1; ++t) step(on, o[t & 1], o[(t & 1) ^ 1], slot, t + 1, t + 1);
-                advance();
-                // the end of the stage: the next one has landed, all waves have read this one, and its slot is loaded anew
-                landed(st < ST - 2 && stored);
-                ring_barrier();
-                slot = slot == ST - 1 ? 0 : slot + 1;
-                step(on, o[(SP - 1) & 1], o[0], slot, 0, 0);   // (past the last stage it reads what nothing uses)
+            for (int t = 0; t < SP - 1; ++t) step(on, o[t & 1], o[(t & 1) ^ 1], slot, t + 1, t + 1, set);
+            advance();
+            // the end of the stage: the next one has landed, all waves have read this one, and its slot is loaded anew
+            landed(st < ST - 2 && stored);
+            ring_barrier();
+            slot = slot == ST - 1 ? 0 : slot + 1;
+            step(on, o[(SP - 1) & 1], o[0], slot, 0, 0, set);   // (past the last stage it reads what nothing uses)
+        };
+        auto stages = [&](auto on) INLINE {
+            if constexpr (EIGHT) {
+                for (int st = 0; st < nst; st += 2) {   // (two by two, so that the registers of each set are known)
+                    stage(on, st, ST & 1);
+                    stage(on, st + 1, (ST & 1) ^ 1);
+                }
+            } else {
+                for (int st = 0; st < nst; ++st) stage(on, st, 0);
             }
         };
         if (live)
