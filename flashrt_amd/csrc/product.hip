@@ -357,6 +357,7 @@ static int any_t(const char* what, const ProductArgs& p, hipStream_t stream) {
 
 // ---------------------------------------------------------------- tiles through direct loads
 typedef __amdgpu_buffer_rsrc_t Buffer;
+typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef int i4_t __attribute__((ext_vector_type(4)));
 // An offset past every buffer's bytes: a load of it gives zeros, a store nothing
@@ -707,16 +708,17 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
     auto finish = [&]() INLINE {
         // The results through LDS, OR rows of QP fourths of a fragment (8 features each) at a time, so that whole lines are stored. Lane l's
         // value i of a fragment: feature 8 (i / 4) + 4 (l / 32) + i % 4, row l % 32.
-        auto results = [&](auto zero, auto added) INLINE {
+        auto results = [&](auto staged, auto zero, auto added) INLINE {
             constexpr bool ADD = decltype(added)::value;   // (in fp32 up to the sum, of the result's type then)
-            typedef decltype(zero) O;
+            typedef decltype(staged) O;
+            typedef decltype(zero) R;
             constexpr int sz = sizeof(O), QP = 16 / sz < 4 * FN ? 16 / sz : 4 * FN, V = 16 / sz;
             constexpr int PR = QP * 8 / V, NP = OR * PR / 64;   // pieces of 16 bytes in a row, of a lane; in LDS piece p of row r is at p ^ (r / 2 % 8)
             static_assert(4 * FN % QP == 0 && FM * (4 * FN / QP) * NP * (32 / OR) >= kStores, "the stores of a wave");
             typedef O vec4 __attribute__((ext_vector_type(4)));
             uint8_t* const w = smem + ST * Sh::stage_b + wave * Sh::out_b;
-            O* const out = static_cast<O*>(p.out) + (MODE == kWgrad ? int64_t(g) * p.N * p.C : 0) + x0 * p.ldout;
-            const Buffer to_out = __builtin_amdgcn_make_buffer_rsrc(out, 0, int(((xn - 1) * p.ldout + features) * sz), 0x00020000);
+            R* const out = static_cast<R*>(p.out) + (MODE == kWgrad ? int64_t(g) * p.N * p.C : 0) + x0 * p.ldout;
+            const Buffer to_out = __builtin_amdgcn_make_buffer_rsrc(out, 0, int(((xn - 1) * p.ldout + features) * sizeof(R)), 0x00020000);
 #pragma unroll
             for (int m = 0; m < FM; ++m) {
 #pragma unroll
@@ -745,11 +747,32 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
                             return w + r * 128 + ((ln % PR ^ (r / 2 % 8)) << 4);
                         };
                         if constexpr (ADD) {
+                            // Four results a lane, whole ones (C is a multiple of eight); what is there is read for NP rows before the first
+                            // is written. 20480 rows of 512 experts, 1280 x 2560: fp32 2.59 ms (13.4 GB read and written; row by row
+                            // 3.48), bf16 2.44 (2.66), which waits for the stores of the step before; with steps read ahead 2.58 and 2.18, but registers spill
+                            typedef R vec __attribute__((ext_vector_type(4)));
+                            typedef std::conditional_t<sizeof(R) == 4, u4_t, u2_t> Raw;
+                            uint32_t to[NP];
+                            Raw old[NP];
 #pragma unroll
                             for (int i = 0; i < NP; ++i) {
                                 const int r = r0 + i * (64 / PR);
-                                if (r < xn && c < features)
-                                    store4(p, (int64_t(g) * p.N + x0 + r) * p.C + c, *reinterpret_cast<const f4_t*>(from(i)), features - c);
+                                to[i] = r < xn && c < features ? uint32_t(r * int(p.ldout) + c) * sizeof(R) : kNone;
+                                asm volatile("" : "+v"(to[i]));
+                                if constexpr (sizeof(R) == 4)
+                                    old[i] = __builtin_amdgcn_raw_buffer_load_b128(to_out, to[i], 0, 2);
+                                else
+                                    old[i] = __builtin_amdgcn_raw_buffer_load_b64(to_out, to[i], 0, 2);
+                            }
+                            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                            for (int i = 0; i < NP; ++i) {
+                                const f4_t v = *reinterpret_cast<const f4_t*>(from(i)) + __builtin_convertvector(__builtin_bit_cast(vec, old[i]), f4_t);
+                                const Raw raw = __builtin_bit_cast(Raw, __builtin_convertvector(v, vec));
+                                if constexpr (sizeof(R) == 4)
+                                    __builtin_amdgcn_raw_buffer_store_b128(raw, to_out, to[i], 0, 2);
+                                else
+                                    __builtin_amdgcn_raw_buffer_store_b64(raw, to_out, to[i], 0, 2);
                             }
                         } else if (features % V == 0 || (ft + 1) * BN <= features) {
                             i4_t v[NP];
@@ -771,14 +794,18 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
                 }
             }
         };
-        if (MODE == kWgrad && p.add)
-            results(float(), std::true_type());
-        else if (p.out_type == FRT_GGML_F32)
-            results(float(), std::false_type());
+        auto as = [&](auto zero) INLINE {
+            if (MODE == kWgrad && p.add)
+                results(float(), zero, std::true_type());
+            else
+                results(zero, zero, std::false_type());
+        };
+        if (p.out_type == FRT_GGML_F32)
+            as(float());
         else if (p.out_type == FRT_GGML_F16)
-            results(_Float16(), std::false_type());
+            as(_Float16());
         else
-            results(__bf16(), std::false_type());
+            as(__bf16());
     };
 #pragma unroll(EIGHT ? ST - 1 : 1)
     for (int s = 0; s < ST - 1; ++s) {
