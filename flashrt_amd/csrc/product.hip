@@ -142,6 +142,7 @@ __device__ __forceinline__ void store4(const ProductArgs& p, int64_t at, f4_t v,
 // sums are added through LDS in their order. What hides the loads' latency is the other shares and the other workgroups of the CU. 1542 rows of
 // 128 experts (N 1021, C 1019, fp16, 267 MB of weights) 62 us, about the time of the other kernels at C 1024; 16384 rows 136 us, 250 TFLOP/s; fp32
 // (8192 rows, N 2048, C 2048) 119 TFLOP/s of the library's 153 at 8192^3. Whole stages without the checks of single pieces gave nothing.
+// (Two workgroups of 128 x 128 to a CU: fp32 with 8-bit rows, at one register too many, spills it.)
 template <typename T, Mode MODE, bool EIGHT, int BM, int BN, int WM, int WN, int KS>
 __global__ void __launch_bounds__(64 * WM * WN * KS, BM == 128 ? 4 : 1) k_product_any(ProductArgs p, int nx, int ny, FastDiv divx, FastDiv divy) {
     constexpr int NT = 64 * WM * WN, V = Chunk<T>::V, FM = BM / WM / 32, FN = BN / WN / 32;
@@ -435,9 +436,9 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
     constexpr int DX = LX::D, DY = EIGHT ? 0 : LY::D, D = DX + DY, CY = EIGHT ? BK * BN / (16 * 64 * NW) : 0, NR = 64 / (BN / 16);
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    // Workgroup b runs on XCD b % 8 (the grid's rows are whole eights). Each XCD takes an eighth of the row tiles, neighbours, in blocks of RB with their chunks of features: what
-    // runs at once on it reads few different rows of either operand. Where eighths would leave more than a ninth of the chip idle,
-    // the blocks go over all XCDs.
+    // Workgroup b runs on XCD b % 8 (the grid's rows are whole eights). Each XCD takes an eighth of the row tiles, neighbours, in blocks of RB with
+    // their chunks of features: what runs at once on it reads few different rows of either operand. Where eighths would leave more than
+    // a ninth of the chip idle, the blocks go over all XCDs.
     const uint32_t b = wide_block(), xcd = b & 7;
     int g, x0, xn, K, k_first = 0, chunk = 0;
     auto order = [&](uint32_t i, int tiles) INLINE {   // the row tile of workgroup i of those of that many row tiles (-1: none), and its chunk
