@@ -947,19 +947,20 @@ __global__ void __launch_bounds__(256) k_product_rows(ProductArgs p, int ntile, 
 #pragma unroll
             for (int i = 0; i < 4; ++i) o.x[i] = gld<Vec<T>>(x + min(16 * q + 4 * i + g, nc - 1) * V);
         };
+        bool ok = false;   // the lane's row is one of a's (else zeros, as a factor: an infinite weight gives NaN in every kernel)
         auto multiply = [&](int q, const Group& o) INLINE {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const bool in = 16 * q + 4 * i + g < nc;
                 const Vec<T> zero = {};
-                acc = mma16(in ? o.w[i] : zero, in ? o.x[i] : zero, acc);
+                acc = mma16(in ? o.w[i] : zero, in && ok ? o.x[i] : zero, acc);
             }
         };
 #pragma unroll
         for (int k = 0; k < P; ++k)
             if (kw + k * KW < ng) load_w(kw + k * KW, u[k]);
         __builtin_amdgcn_sched_barrier(0);
-        const bool ok = unsigned(a) < unsigned(p.a_rows);
+        ok = unsigned(a) < unsigned(p.a_rows);
         x = static_cast<const T*>(p.x) + int64_t(ok ? a : 0) * p.ldx;
 #pragma unroll
         for (int k = 0; k < P; ++k)
@@ -975,7 +976,6 @@ __global__ void __launch_bounds__(256) k_product_rows(ProductArgs p, int ntile, 
                 }
             }
         }
-        if (!ok) acc = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
     if constexpr (KW > 1) {
         s_sum[wave][lane] = acc;

@@ -193,7 +193,8 @@ int frt_mx4_product(void* stream, const void* aq, const void* asc, int a_rows, c
  * does not train). Operands of type FRT_GGML_F32, F16 or BF16 (both the same), results of any of the three; sums in fp32, rounded once.
  * Group g < E <= 4096 has the rows r in [bounds[g], bounds[g+1]); bounds (frt_moe_sort's) ascend within [0, M], NULL: one group (E = 1) of M
  * rows. Rows of no group stay as they were. a(r) is row r of a, or row rows[r] where rows is given (frt_moe_sort's tok_of); an index
- * outside [0, a_rows) gives a row of zeros. Weights w and dw are [E][N][C]; rows of a, out, dout and da lie ld* elements apart.
+ * outside [0, a_rows) is a row of zeros in the sums (an infinite or NaN factor times it gives NaN). Weights w and dw are [E][N][C]; rows of a,
+ * out, dout and da lie ld* elements apart.
  * M (may be 0), N and C up to 2^30; a_rows >= M, or >= 1 with rows. Inputs and outputs must not overlap.
  *   product        out[r][j] = sum_k w_g[j][k] a(r)[k], j < N
  *   product_grad   da[r][k] = sum_j dout[r][j] w_g[j][k], k < C (a sorted row's gradient: frt_moe_permute_grad sums a token's)

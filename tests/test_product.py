@@ -610,3 +610,63 @@ def test_gradients_against_differences():
     for got, want, mag in (((f(a + da, w) - f(a, w)), (ga.double() * da.double()).sum(), size(a.abs() + da.abs(), w)),
                            ((f(a, w + dwt) - f(a, w)), (gw.double() * dwt.double()).sum(), size(a, w.abs() + dwt.abs()))):
         assert abs(float(got - want)) <= 1.01 * (2 * (C + 2) + M + N) * STEP * mag, (float(got), float(want))
+
+
+def missing(M, tokens):
+    """Row indices of which every third lies outside [0, tokens), and which those are."""
+    rows = np.random.default_rng(M).integers(0, tokens, M)
+    rows[::3] = np.resize([-1, tokens, -(2 ** 31), 2 ** 31 - 1], rows[::3].size)
+    out = np.zeros(M, bool)
+    out[::3] = True
+    return i32(rows), torch.from_numpy(out).cuda()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("shape", [k for k, v in {**KERNELS, **ANY}.items() if v[0] == "product"])
+def test_missing_rows_times_infinities(shape, kind):
+    """A row whose index lies outside is zeros in the sums of every kernel: an infinite or NaN weight times it gives NaN, a finite one 0. (fp32
+    rows of any of these shapes take the kernel for rows at any alignment.)"""
+    import flashrt_amd as F
+    _, sizes, N, C, _ = {**KERNELS, **ANY}[shape]
+    pad, E, M, tokens = 1 if shape in ANY else 8, len(sizes), sum(sizes), 50
+    x, (rows, out_rows) = rows_of(tokens, C, kind, 1, pad), missing(M, tokens)
+    w = rows_of(E * N, C, kind, 2).contiguous().view(E, N, C)
+    w[:, 1, 3], w[:, N - 1, C - 1] = float("inf"), float("nan")
+    out = out_of(M, N, F32)[:M]
+    F.moe_product(x, w, out, bounds=i32(cut(sizes)), rows=rows)
+    lost = out[out_rows]
+    assert lost[:, [1, N - 1]].isnan().all()
+    lost[:, [1, N - 1]] = 0
+    assert (lost == 0).all()
+    there, a = out[~out_rows], x[rows[~out_rows].long(), 3].float()
+    assert torch.equal(there[:, 1], torch.where(a > 0, torch.inf, -torch.inf)) and there[:, N - 1].isnan().all()
+    there[:, [1, N - 1]] = 0
+    assert torch.isfinite(there).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("shape", [k for k, v in {**KERNELS, **ANY}.items() if v[0] == "wgrad"])
+def test_missing_rows_in_the_weight_gradient(shape, eight, kind):
+    """The same in the weights' gradient: an infinity or a NaN of such a row's output gradient gives NaN in its feature, and its finite ones add
+    nothing."""
+    import flashrt_amd as F
+    _, sizes, N, C, _ = {**KERNELS, **ANY}[shape]
+    pad, E, M, tokens = 1 if shape in ANY else 8, len(sizes), sum(sizes), 50
+    C = C // 32 * 32 if eight else C
+    x, (rows, out_rows) = rows_of(tokens, C, kind, 1, 0 if eight else pad), missing(M, tokens)
+    dout = rows_of(M, N, kind, 3, pad)
+    dout[out_rows, 1], dout[out_rows, N - 1] = float("-inf"), float("nan")
+    clean = dout.clone()
+    clean[out_rows] = 0
+    a = quantized(F, x)[0] if eight else x
+    dw, want = (torch.full((E, N, C), 77.0, device="cuda") for _ in range(2))
+    F.moe_product_wgrad(dout, a, dw, bounds=i32(cut(sizes)), rows=rows)
+    F.moe_product_wgrad(clean, a, want, bounds=i32(cut(sizes)), rows=rows.clamp(0, tokens - 1))
+    at = cut(sizes)
+    hit = torch.tensor([bool(out_rows[lo:hi].any()) for lo, hi in zip(at, at[1:])], device="cuda")
+    assert dw[hit][:, [1, N - 1]].isnan().all()
+    dw[hit, 1], dw[hit, N - 1] = want[hit, 1], want[hit, N - 1]
+    assert torch.isfinite(want).all() and torch.equal(dw, want)
