@@ -698,7 +698,8 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
     };
 
     // Waits count the loads: at the end of a stage those of ST - 2 stages were issued behind the next one's, and in a feature tile's first ST
-    // - 1 stages the stores of the tile before (at least kStores per wave; with add, whose stores are not counted on, none).
+    // - 2 stages the stores of the tile before, where these are of whole pieces (at least kStores per wave whatever is inside; none are counted on
+    // with add, nor of a feature tile that ends inside a piece, whose single values may be fewer).
     constexpr int kStage = D + 3 * CY, kStores = FM * FN * 2, kCap = 63;
     auto landed = [&](bool stores) INLINE {
         if (stores)
@@ -706,6 +707,7 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
         else
             wait_vm<(kStage * (ST - 2) < kCap ? kStage * (ST - 2) : kCap)>();
     };
+    bool stored = false;   // the tile before left kStores stores or more under way
     auto finish = [&]() INLINE {
         // The results through LDS, OR rows of QP fourths of a fragment (8 features each) at a time, so that whole lines are stored. Lane l's
         // value i of a fragment: feature 8 (i / 4) + 4 (l / 32) + i % 4, row l % 32.
@@ -719,6 +721,8 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
             typedef O vec4 __attribute__((ext_vector_type(4)));
             uint8_t* const w = smem + ST * Sh::stage_b + wave * Sh::out_b;
             R* const out = static_cast<R*>(p.out) + (MODE == kWgrad ? int64_t(g) * p.N * p.C : 0) + x0 * p.ldout;
+            const bool whole = features % V == 0 || (ft + 1) * BN <= features;   // the feature tile ends with a piece
+            stored = !ADD && whole;
             const Buffer to_out = __builtin_amdgcn_make_buffer_rsrc(out, 0, int(((xn - 1) * p.ldout + features) * sizeof(R)), 0x00020000);
 #pragma unroll
             for (int m = 0; m < FM; ++m) {
@@ -775,7 +779,7 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
                                 else
                                     __builtin_amdgcn_raw_buffer_store_b64(raw, to_out, to[i], 0, 2);
                             }
-                        } else if (features % V == 0 || (ft + 1) * BN <= features) {
+                        } else if (whole) {
                             i4_t v[NP];
 #pragma unroll
                             for (int i = 0; i < NP; ++i) v[i] = *reinterpret_cast<const i4_t*>(from(i));
@@ -829,7 +833,6 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
     wait_vm<(kStage * (ST - 2) + D / SP < kCap ? kStage * (ST - 2) + D / SP : kCap)>();
     ring_barrier();
     int slot = 0;
-    bool stored = false;   // the tile before left its stores
     Ops o[2];
 #pragma unroll
     for (int i = 0; i < FM + FN; ++i) read(o[0], 0, 0, i);
@@ -867,8 +870,8 @@ __global__ void __launch_bounds__(64 * WM * WN, OCC) k_product_tiles(ProductArgs
             stages(std::true_type());
         else
             stages(std::false_type());
+        stored = false;
         if (live) finish();
-        stored = live && !p.add;
     }
     // no load into LDS is under way when the workgroup ends (the last tile's stores may be)
     if (stored)

@@ -670,3 +670,31 @@ def test_missing_rows_in_the_weight_gradient(shape, eight, kind):
     assert dw[hit][:, [1, N - 1]].isnan().all()
     dw[hit, 1], dw[hit, N - 1] = want[hit, 1], want[hit, N - 1]
     assert torch.isfinite(want).all() and torch.equal(dw, want)
+
+
+# The last feature tile (1, 3 or 5 features in it) ends inside a piece of 16 bytes: its results leave value by value, by as few instructions as one.
+CUT_SHORT = {
+    "product 64": (ragged(40, 0, 30), 4096, 1928),
+    "product 128": (ragged(33, 1, 140), 1024, 1096),
+    "product 256": ([1111, 1300], 13312, 264),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out_kind", TYPES)
+@pytest.mark.parametrize("more", [1, 3, 5])
+@pytest.mark.parametrize("shape", list(CUT_SHORT))
+def test_feature_tiles_cut_inside_a_piece(shape, more, out_kind):
+    """Such a workgroup waits for all its loads into LDS before it ends, which its own results do not show: the same call eight times without a pause,
+    whose workgroups follow one another in the same LDS, gives the same bits eight times, and the values are right."""
+    import flashrt_amd as F
+    sizes, N, C = CUT_SHORT[shape]
+    want = run("product", sizes, N + more, C, BF16, out_kind, behind=0)
+    M, b = sum(sizes), i32(cut(sizes))
+    x = rows_of(M, C, BF16, M + N + more)
+    g = torch.Generator(device="cuda").manual_seed(N + more + C)
+    w = (torch.randn(len(sizes), N + more, C, generator=g, device="cuda") * 0.1).to(BF16)
+    outs = torch.empty(8, M, N + more, dtype=out_kind, device="cuda")
+    for o in outs:
+        F.moe_product(x, w, o, bounds=b)
+    assert all(torch.equal(o, want) for o in outs)
