@@ -108,11 +108,12 @@ __global__ void __launch_bounds__(256) k_mx8_dequantize(const u2_t* __restrict__
 }
 
 // The sigmoid of g. 1 / (1 + exp(-g)) is 0 where exp overflows and NaN for a NaN; rows of 16 bits take the hardware's exponential and reciprocal
-// (a few steps of fp32 off, far below a step of the row's type).
+// (off by a few steps of fp32 and |g| more, far below a step of the row's type); the reciprocal is taken of a fourth, so that the subnormal s of
+// gates below -87.3, which the hardware's would give as 0, is formed by the product.
 template <typename T>
 __device__ __forceinline__ float sigmoid(float g) {
     if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-g));
-    return __builtin_amdgcn_rcpf(1.0f + __expf(-g));
+    return 0.25f * __builtin_amdgcn_rcpf(0.25f * (1.0f + __expf(-g)));
 }
 
 // h = g s(g) u of rows z = g | u, eight values of each half per lane; KEEP: z in 8 bits too (ff a multiple of 32, so that four lanes hold

@@ -380,3 +380,21 @@ def test_written_tensors_count_as_changed():
         call()
         for v, old in zip(everything, was):
             assert v._version == old + any(v is o for o in outs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,u", [(F32, 2.0), (F32, 1e30), (F16, 2.0), (BF16, 2.0), (BF16, 1e30)])
+def test_swiglu_of_subnormal_sigmoids(kind, u):
+    """Gates below -87.3, whose sigmoid is a subnormal number of fp32: off by a step of these (2^-149) more, here times |g u|."""
+    import flashrt_amd as F
+    g = -torch.arange(86.0, 89.0, 0.5, dtype=torch.float64).to(kind)   # (exp(88.5) is the last that fp32 holds)
+    ff, tiny = g.numel(), 2.0 ** -149
+    z = torch.cat([g, torch.full((ff,), u, dtype=kind)])[None]
+    dh = torch.full((1, ff), 0.5, dtype=kind)
+    h, dz = torch.empty(1, ff, dtype=kind, device="cuda"), torch.empty(1, 2 * ff, dtype=kind, device="cuda")
+    F.moe_swiglu(z.cuda(), h)
+    F.moe_swiglu_grad(dh.cuda(), dz, z=z.cuda())
+    want_h, e_h, want_dz, e_dz = ref_swiglu(z.double(), dh.double())
+    assert (want_h != 0).all()
+    near(h, want_h, e_h + tiny * 90 * u, kind)
+    near(dz, want_dz, e_dz + tiny * 90 * max(u, 1.0), kind)
