@@ -698,3 +698,45 @@ def test_feature_tiles_cut_inside_a_piece(shape, more, out_kind):
     for o in outs:
         F.moe_product(x, w, o, bounds=b)
     assert all(torch.equal(o, want) for o in outs)
+
+
+# Shapes of which a workgroup takes several feature tiles one after another, as one sequence of stages: (op, group sizes, N, C), the tile, the feature
+# tiles of a row tile and of a workgroup (the last workgroup of a row tile has fewer in those of 5 / 3 and 5 / 2), the stages of an average group
+SEQUENCES = {
+    "wgrad 256: 3 / 3, 7": ("wgrad", ragged(128, 0, 400), 1032, 544),
+    "wgrad 256: 4 / 4, 1 (short groups)": ("wgrad", ragged(300, 0, 60), 520, 800),
+    "wgrad 64: 5 / 3, 3": ("wgrad", ragged(64, 0, 300), 200, 640),
+    "grad 128: 5 / 2, 4": ("grad", ragged(200, 17, 60), 200, 1040),
+    "grad 64: 9 / 5, 4": ("grad", ragged(300, 0, 30), 200, 1032),
+    "grad 64: 5 / 5, 3": ("grad", ragged(600, 0, 25), 136, 520),
+    "grad 64: 8 / 1, 4 (several row tiles to a group)": ("grad", ragged(20, 0, 200), 200, 1000),
+    "product 128: 4 / 2, 3": ("product", ragged(200, 17, 60), 1021, 136),
+    "product 64: 8 / 3, 11": ("product", ragged(600, 0, 25), 1021, 648),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,out_kind", [(F16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("gather", [0, 70])
+@pytest.mark.parametrize("shape", [k for k, v in SEQUENCES.items() if v[0] != "grad"])
+def test_sequences_of_feature_tiles(shape, gather, kind, out_kind):
+    op, sizes, N, C = SEQUENCES[shape]
+    run(op, sizes, N, C, kind, out_kind, gather=gather, pad=8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,out_kind", [(F16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("shape", [k for k, v in SEQUENCES.items() if v[0] == "grad"])
+def test_sequences_of_feature_tiles_in_the_row_gradient(shape, kind, out_kind):
+    op, sizes, N, C = SEQUENCES[shape]
+    run(op, sizes, N, C, kind, out_kind, pad=8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,out_kind", [(F16, F16), (BF16, F32)])
+@pytest.mark.parametrize("gather", [0, 70])
+@pytest.mark.parametrize("eight,add", [(True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("shape", [k for k, v in SEQUENCES.items() if v[0] == "wgrad"])
+def test_sequences_of_feature_tiles_from_8_bits_and_added(shape, eight, add, gather, kind, out_kind):
+    op, sizes, N, C = SEQUENCES[shape]
+    run(op, sizes, N, C, kind, out_kind, gather=gather, eight=eight, add=add, pad=8)
