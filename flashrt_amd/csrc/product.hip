@@ -337,14 +337,15 @@ static int64_t even_tiles(const ProductArgs& p, int64_t BM, int64_t BN) {
 }
 // Up to as many tiles of 64 x 64 as CUs leave CUs or their matrix cores idle, so the summed values are shared out over a workgroup's waves,
 // the more of them the fewer tiles there are; many tiles are read the less often the larger they are.
-// us, 32 x 32 over 16 shares / 64 x 64 over 4 / over 2 / undivided / 128 x 128:
-//   16-bit product, N and C odd: 128 experts of 4 rows (N 1021, C 1019) 40 / 18 / 16 / 19 / 21, of 12 rows 185 / 73 / 62 / 69 / 64; one group of
-//   4096 rows (C 2047, N 2048) 497 / 118 / 99 / 99 / 63, of 1024 rows (N 1024) 126 / 33 / 30 / 36 / 47
-//   weights' gradient (N 511, C 509) of one group of 8192 rows 81 / 132 / 196 / 346 / 533; of 2048 rows each, four groups 87 / 39 / 57 / 96 / 111,
-//   sixteen 346 / 148 / 147 / 143 / 119
-//   fp32 (N 2048, C 2048): one group of 4096 rows 651 / 411 / 377 / 366 / 287 (119 TFLOP/s), of 1024 165 / 105 / 99 / 109 / 159
+// us, 32 x 32 over 16 shares / 64 x 64 over 4 / over 2 / undivided / 128 x 128, weights from memory:
+//   16-bit product, N and C odd: 128 experts of 4 rows (N 1021, C 1019, 266 MB) 174 / 78 / 64 / 66 / 63, of 12 rows 191 / 81 / 67 / 70 / 67; one group of
+//   4096 rows (C 2047, N 2048) 524 / 141 / 110 / 114 / 74, of 1024 rows (N 1024) 64 / 24 / 27 / 35 / 47
+//   weights' gradient (N 511, C 509) of one group of 8192 rows 77 / 132 / 198 / 348 / 546; of 2048 rows each, four groups 87 / 38 / 57 / 101 / 153,
+//   sixteen 328 / 142 / 170 / 174 / 171, of 1024 rows, 32 groups 152 over 4 / 162 / 114 at 128 x 128; four groups of 2048 (N 1021, C 1019) 143 / 128 / 111
+//   fp32 (N 2048, C 2048): one group of 4096 rows 679 / 413 / 377 / 366 / 289 (119 TFLOP/s), of 1024 172 / 106 / 99 / 109 / 160
 // fp32 rows, whose products take their tile's time whether its rows are there or not, in tiles of 32 rows where the groups are shorter:
-// 128 experts (N 1024, C 768) of 8 rows 205 / 176 / 146 / 137, 32 x 64 over 8 shares 131; of one row 28 / 24 / 25 / 32, 18.
+// 128 experts (N 1024, C 768, 403 MB) of 8 rows 210 / 178 / 146 / 136 / 212, 32 x 64 over 8 shares 134; of one row 204 / 177 / 147 / 137 / 212, 130;
+// 16 experts of one row 29 / 25 / 26 / 33 / 61, 20.
 template <typename T, Mode MODE, bool EIGHT = false>
 static int any_t(const char* what, const ProductArgs& p, hipStream_t stream) {
     const int64_t tiles = even_tiles<MODE>(p, 64, 64), rows = even_rows(p);
@@ -1035,15 +1036,19 @@ template <typename T>
 static int product_t(const ProductArgs& p, hipStream_t stream) {
     if constexpr (sizeof(T) == 2)
         if (pieces<T>(p, p.C, false)) {
-            // The weights that tiles of 16 rows read: up to 256 MB straight into registers, with the values over the waves where those are
-            // few; beyond, in tiles through LDS. us, one wave / two / four to a row / tiles: one token's ten experts (N 1024, C 2048, 42
-            // MB) 12.9 / 12.9 / 12.3 / 19.5, two tokens' 21.7 / 18.3 / 19.4 / 22.3, four 31 / 29 / 35 / 32, sixteen (600 MB) 114 / 109 /
-            // 122 / 99; N 2560, C 640 9.6 / 11.7 / 14.0 / 12.0; one group (N 8192, C 4096) of a row 20.9 / 20.2 / 15.6 / 34.7.
+            // The weights that tiles of 16 rows read: up to 256 MB straight into registers, beyond in tiles through LDS; a row's values over four
+            // waves, or two, while the call has no more than three waves to a SIMD with that and each of them a group of values. us, four / two / one
+            // wave to a row / tiles, weights from memory: experts of a row, N 1024, C 2048, 10 of them (640 units) 14.6 / 15.6 / 18.5 / 20.9, 12
+            // 15.1 / 16.0 / 19.1 / 21.5, 16 20.3 / 18.9 / 21.1 / 24.5, 24 27.4 / 23.9 / 26.3 / 23.6, 32 36 / 32 / 32 / 27, 64 (268 MB) 63 / 70 / 63 / 53; C
+            // 512, 16 of them 8.6 / 7.1 / 6.9 / 11.7, 32 15.9 / 14.4 / 11.7 / 13.2; N 2560, C 640, 8 of them (1280 units) 11.6 / 10.5 / 11.4 / 12.0, 9
+            // 12.9 / 10.9 / 11.4, 10 14.7 / 13.9 / 12.3 / 12.3, 32 37 / 29 / 27 / 29; N 2048, C 4096, 6 (768) 24.8 / 27.1 / 32.1, 12 40 / 46 / 42; one
+            // group of a row, C 4096, N 8192 17.8 / 19.3 / 30.6 / 28.7, N 16384 29.5 / 34.0 / 39.5 / 36.8.
             // Weights that more than one tile reads, up to 32 MB. us, so / in tiles: one group of 256 rows (N 512, C 1024, 17 MB) 7.4 /
             // 8.2, of 128 (N 1024, C 2048, 34 MB) 9.7 / 10.0, of 2048 (512 x 512, 67 MB) 17.2 / 8.3, of 256 (N 2048, C 2048, 134 MB) 31 / 15
+            constexpr int kFew = 3 * 4 * 256;   // waves
             const int64_t rows = even_rows(p), units = even_tiles<kProduct>(p, 16, 16);
             if (units <= (int64_t(rows <= 16 ? 256 : 32) << 20) / 32 / p.C)
-                return units <= 640 && p.C >= 512 ? rows_go<T, 4>(p, stream) : units <= 1280 && p.C >= 256 ? rows_go<T, 2>(p, stream) : rows_go<T, 1>(p, stream);
+                return 4 * units <= kFew && p.C >= 512 ? rows_go<T, 4>(p, stream) : 2 * units <= kFew && p.C >= 256 ? rows_go<T, 2>(p, stream) : rows_go<T, 1>(p, stream);
             return tiles_t<T, kProduct>("moe_product", p, stream);
         }
     return any_t<T, kProduct>("moe_product", p, stream);

@@ -740,3 +740,12 @@ def test_sequences_of_feature_tiles_in_the_row_gradient(shape, kind, out_kind):
 def test_sequences_of_feature_tiles_from_8_bits_and_added(shape, eight, add, gather, kind, out_kind):
     op, sizes, N, C = SEQUENCES[shape]
     run(op, sizes, N, C, kind, out_kind, gather=gather, eight=eight, add=add, pad=8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("N", [768, 769, 1536, 1537])
+@pytest.mark.parametrize("C", [256, 512, 1160])
+def test_few_rows_at_the_limits_of_their_waves(C, N, kind):
+    """Sixteen groups of one row, of as many tiles of 16 x 16 as four or two waves to a row are taken for, and of one more."""
+    run("product", [1] * 16, N, C, kind, kind, gather=9, pad=8)
