@@ -213,7 +213,8 @@ int frt_moe_product_wgrad(void* stream, const void* dout, int64_t lddout, const 
  * [rows][cols/32]. cols is a multiple of 32. rows may be 0.
  * frt_mx8_quantize: x of type FRT_GGML_F32 / F16 / BF16, rows ldx elements apart. With a block's largest magnitude m 2^k (1 <= m < 2),
  * b = max(k - 6, -127) + 127 and a code is x 2^(127 - b) rounded to nearest even, held within -127 .. 127; a block of zeros has b = 0; a
- * block with an infinity or a NaN has b = 255 and codes 0 (all its values read NaN).
+ * block with an infinity or a NaN has b = 255 and codes 0 (all its values read NaN). (Not the published MX format's INT8, whose codes count
+ * 2^-6: its scale byte of the same block is 6 larger.)
  * frt_mx8_dequantize: the values, rounded to nearest even where the type cannot hold them.
  * ---- the experts' gated activation on rows z [rows][2 ff] = gate | up, and its backward pass from z or from z in 8 bits:
  *   swiglu       h = g s(g) u, s(g) = 1 / (1 + exp(-g)), in fp32, rounded once; with codes and scales (ff then a multiple of 32) z is also
