@@ -137,12 +137,12 @@ __device__ __forceinline__ void store4(const ProductArgs& p, int64_t at, f4_t v,
         store4(static_cast<__bf16*>(p.out) + at, v, left, p.add);
 }
 
-// Rows at any distance and alignment, and calls of few tiles: a tile of BM rows x BN features by KS times WM x WN waves, each share of which
-// takes every KS-th stage of the summed values into its own LDS, the next one's operands in registers while this one is multiplied; the shares'
-// sums are added through LDS in their order. What hides the loads' latency is the other shares and the other workgroups of the CU. 1542 rows of
-// 128 experts (N 1021, C 1019, fp16, 267 MB of weights) 62 us (73 from memory), about the time of the other kernels at C 1024; 16384 rows 136 us, 250 TFLOP/s; fp32
-// (8192 rows, N 2048, C 2048) 119 TFLOP/s of the library's 153 at 8192^3. Whole stages without the checks of single pieces gave nothing.
-// (Two workgroups of 128 x 128 to a CU: fp32 with 8-bit rows spills two registers.)
+// Rows at any distance and alignment, and calls of few tiles: a tile of BM rows x BN features by KS times WM x WN waves, each share of which takes
+// every KS-th stage of the summed values into its own LDS, the next one's operands in registers while this one is multiplied; the shares' sums are
+// added through LDS in their order. What hides the loads' latency is the other shares and the other workgroups of the CU. 1542 rows of 128 experts (N
+// 1021, C 1019, fp16, 267 MB of weights) 62 us (73 from memory), about the time of the other kernels at C 1024; 16384 rows 136 us, 250 TFLOP/s; fp32
+// (8192 rows, N 2048, C 2048) 119 TFLOP/s of the library's 153 at 8192^3. Whole stages without the checks of single pieces gave nothing. (Two
+// workgroups of 128 x 128 to a CU: fp32 with 8-bit rows spills two registers.)
 template <typename T, Mode MODE, bool EIGHT, int BM, int BN, int WM, int WN, int KS>
 __global__ void __launch_bounds__(64 * WM * WN * KS, BM == 128 ? 4 : 1) k_product_any(ProductArgs p, int nx, int ny, FastDiv divx, FastDiv divy) {
     constexpr int NT = 64 * WM * WN, V = Chunk<T>::V, FM = BM / WM / 32, FN = BN / WN / 32;
@@ -416,14 +416,14 @@ constexpr int RB = 4;        // row tiles of a block
 // comes before its last step, whose operands are in registers, and the next stage's first ones are read behind it. The stages of the feature
 // tiles form one sequence: the next tile's first stages load while this one's results are written.
 //
-// What bounds it: with few rows to a group the weights' stream (20480 rows of 512 experts, N 1024, C 2048: 383 us, 5.7 TB/s over 2.1 GB of
-// weights; 2030 rows, N 2560, C 640: 218 us, 7.4 TB/s); with many neither the loads nor the products alone, but how far they overlap: the loads alone
-// bring in 23 bytes per clock and CU, whether the lines come from L2 or beyond (the L1 stands half of the time for lines under way), which would
-// be 1.8 PFLOP/s in tiles of 256 x 256 and 1.2 in 128 x 256; the products without the loads take 365 of the 476 to 493 us of one group of 8192 rows (N 8192,
+// What bounds it: with few rows to a group the weights' stream (20480 rows of 512 experts, N 1024, C 2048: 383 us, 5.7 TB/s over 2.1 GB of weights;
+// 2030 rows, N 2560, C 640: 218 us, 7.4 TB/s); with many neither the loads nor the products alone, but how far they overlap: the loads alone bring in
+// 23 bytes per clock and CU, whether the lines come from L2 or beyond (the L1 stands half of the time for lines under way), which would be 1.8
+// PFLOP/s in tiles of 256 x 256 and 1.2 in 128 x 256; the products without the loads take 365 of the 476 to 493 us of one group of 8192 rows (N 8192,
 // C 4096), 1115 to 1155 TFLOP/s. LDS is busy a quarter of the time, without conflicts. A group's last row tile costs a whole one: 8 experts (N, C
 // 4096) of 2048 rows each 521 us, 1.05 PFLOP/s, of 1900 to 2196 575, matrix cores 57% busy; row gradients of 128 experts (N 2048, C 1024, fp16), 128
-// x 256, of 512 rows each 347 us, of 513 400, of 576 410, of 640 430. The weights' gradients spill SGPRs (256 x 256 17, from 8-bit rows 14; 64 x 128 66
-// and 6), no VGPRs.
+// x 256, of 512 rows each 347 us, of 513 400, of 576 410, of 640 430. The weights' gradients spill SGPRs (256 x 256 17, from 8-bit rows 14; 64 x 128
+// 66 and 6), no VGPRs.
 //
 // Measured: four waves of 128 x 128 instead of eight 505 against 455 us (one group of 8192); stages of 64 values in two slots for the largest
 // tile 476 against 450, of 32 values for 128 x 256 (half a line per row) 545 against 383 (20480 rows); 64 x 256 397, 128 x 128 430; row tiles of a
@@ -1041,11 +1041,11 @@ static int product_t(const ProductArgs& p, hipStream_t stream) {
         if (pieces<T>(p, p.C, false)) {
             // The weights that tiles of 16 rows read: up to 256 MB straight into registers, beyond in tiles through LDS; a row's values over four
             // waves, or two, while the call has no more than three waves to a SIMD with that and each of them a group of values. us, four / two / one
-            // wave to a row / tiles, weights from memory: experts of a row, N 1024, C 2048, 10 of them (640 units) 14.6 / 15.6 / 18.5 / 20.9, 12
-            // 15.1 / 16.0 / 19.1 / 21.5, 16 20.3 / 18.9 / 21.1 / 24.5, 24 27.4 / 23.9 / 26.3 / 23.6, 32 36 / 32 / 32 / 27, 64 (268 MB) 63 / 70 / 63 / 53; C
-            // 512, 16 of them 8.6 / 7.1 / 6.9 / 11.7, 32 15.9 / 14.4 / 11.7 / 13.2; N 2560, C 640, 8 of them (1280 units) 11.6 / 10.5 / 11.4 / 12.0, 9
-            // 12.9 / 10.9 / 11.4, 10 14.7 / 13.9 / 12.3 / 12.3, 32 37 / 29 / 27 / 29; N 2048, C 4096, 6 (768) 22 / 26 / 30 / 29, 12 (1536) 43 / 45 / 48 / 46, 13 48 / 53 / 50 / 47; one
-            // group of a row, C 4096, N 8192 17.8 / 19.3 / 30.6 / 28.7, N 16384 29.5 / 34.0 / 39.5 / 36.8.
+            // wave to a row / tiles, weights from memory: experts of a row, N 1024, C 2048, 10 of them (640 units) 14.6 / 15.6 / 18.5 / 20.9, 12 15.1
+            // / 16.0 / 19.1 / 21.5, 16 20.3 / 18.9 / 21.1 / 24.5, 24 27.4 / 23.9 / 26.3 / 23.6, 32 36 / 32 / 32 / 27, 64 (268 MB) 63 / 70 / 63 / 53;
+            // C 512, 16 of them 8.6 / 7.1 / 6.9 / 11.7, 32 15.9 / 14.4 / 11.7 / 13.2; N 2560, C 640, 8 of them (1280 units) 11.6 / 10.5 / 11.4 /
+            // 12.0, 9 12.9 / 10.9 / 11.4, 10 14.7 / 13.9 / 12.3 / 12.3, 32 37 / 29 / 27 / 29; N 2048, C 4096, 6 (768) 22 / 26 / 30 / 29, 12 (1536) 43
+            // / 45 / 48 / 46, 13 48 / 53 / 50 / 47; one group of a row, C 4096, N 8192 17.8 / 19.3 / 30.6 / 28.7, N 16384 29.5 / 34.0 / 39.5 / 36.8.
             // Weights that more than one tile reads, up to 32 MB. us, so / in tiles: one group of 256 rows (N 512, C 1024, 17 MB) 7.4 /
             // 8.2, of 128 (N 1024, C 2048, 34 MB) 9.7 / 10.0, of 2048 (512 x 512, 67 MB) 17.2 / 8.3, of 256 (N 2048, C 2048, 134 MB) 31 / 15
             constexpr int kFew = 3 * 4 * 256;   // waves
